@@ -17,6 +17,9 @@ ABI_VERSION = 2
 OK, INVALID_REQUEST, INCOMPATIBLE_WORKER, RESOURCE_EXHAUSTED = 0, 1, 2, 3
 DEADLINE_EXCEEDED, CANCELLED, INTERNAL = 4, 5, 6
 F32, F16, BF16 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_UNSCALED, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+KV_E4M3, KV_INT8 = 0, 1
 ITEM_SAMPLE, ITEM_TOKEN_FROM_DEVICE, ITEM_LOGPROBS = 1, 2, 4
 STATUS_NAMES = {0: "OK", 1: "INVALID_REQUEST", 2: "INCOMPATIBLE_WORKER", 3: "RESOURCE_EXHAUSTED",
                 4: "DEADLINE_EXCEEDED", 5: "CANCELLED", 6: "INTERNAL"}
@@ -32,7 +35,9 @@ EXPORTS = ("hllm_rocm_last_error", "hllm_rocm_abi_version", "hllm_rocm_stage_cre
            "hllm_rocm_stage_set_graphs", "hllm_rocm_stage_graph_stats", "hllm_rocm_set_gemm_config",
            "hllm_rocm_measure_read_bandwidth", "hllm_rocm_stage_execute_profiled",
            "hllm_rocm_sample_logits_noalloc", "hllm_rocm_device_allocator_metrics",
-           "hllm_rocm_device_reset_peak", "hllm_rocm_device_query", "hllm_rocm_measure_mfma_rate")
+           "hllm_rocm_device_reset_peak", "hllm_rocm_device_query", "hllm_rocm_measure_mfma_rate",
+           "hllm_rocm_rope_plan", "hllm_rocm_rope_apply", "hllm_rocm_kv_append", "hllm_rocm_kv_read",
+           "hllm_rocm_kv_attention", "hllm_rocm_kv_attention_workspace")
 NOALLOC_MAX_VOCABULARY = 262144
 
 
@@ -98,6 +103,37 @@ class Memory(C.Structure):
                 ("pinned_host_bytes", C.c_uint64), ("unified_bytes", C.c_uint64)]
 
 
+class Tensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_uint32), ("heads", C.c_uint32),
+                ("row_stride", C.c_uint64), ("head_stride", C.c_uint64)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("rotary_dimension", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32),
+                ("theta", C.c_double), ("factor", C.c_double), ("original_length", C.c_double),
+                ("low_frequency_factor", C.c_double), ("high_frequency_factor", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("magnitude", C.c_double)]
+
+
+class RopePlan(C.Structure):
+    _fields_ = [("rotary_dimension", C.c_uint32), ("layout", C.c_uint32), ("magnitude", C.c_float),
+                ("reserved", C.c_uint32), ("turns", C.c_uint64 * 128)]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("format", C.c_uint32), ("pages", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dimension", C.c_uint32), ("page_stride", C.c_uint64),
+                ("token_stride", C.c_uint64), ("head_stride", C.c_uint64), ("keys", C.c_void_p),
+                ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p)]
+
+
+class KvAttentionArgs(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("page_table", C.c_void_p), ("table_width", C.c_uint64),
+                ("table_stride", C.c_uint64), ("lengths", C.c_void_p), ("max_length", C.c_uint64),
+                ("scale", C.c_float), ("q", Tensor), ("out", Tensor), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
 _LIB = None
 
 
@@ -154,6 +190,15 @@ def library() -> C.CDLL:
     L.hllm_rocm_device_allocator_metrics.argtypes = [C.c_int32, C.POINTER(AllocatorMetrics)]
     L.hllm_rocm_device_reset_peak.argtypes = [C.c_int32]
     L.hllm_rocm_device_query.argtypes = [C.c_int32, C.POINTER(DeviceInfo)]
+    tensor, i32 = C.POINTER(Tensor), C.c_int32
+    L.hllm_rocm_rope_plan.argtypes = [C.POINTER(RopeConfig), C.POINTER(RopePlan)]
+    L.hllm_rocm_rope_apply.argtypes = [i32, vp, C.POINTER(RopePlan), vp, u64, u32, tensor, tensor,
+                                       tensor, tensor]
+    L.hllm_rocm_kv_append.argtypes = [i32, vp, C.POINTER(KvPages), vp, u64, tensor, tensor,
+                                      C.POINTER(RopePlan), vp, tensor, tensor]
+    L.hllm_rocm_kv_read.argtypes = [i32, vp, C.POINTER(KvPages), vp, u64, tensor, tensor]
+    L.hllm_rocm_kv_attention.argtypes = [i32, vp, C.POINTER(KvPages), C.POINTER(KvAttentionArgs)]
+    L.hllm_rocm_kv_attention_workspace.argtypes = [C.POINTER(KvPages), u64, u32, u64, C.POINTER(u64)]
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is C.c_int or (fn.restype is None and name != "hllm_rocm_stage_destroy"):

@@ -18,13 +18,18 @@
 #include <tuple>
 #include <vector>
 
+#include "abi.hpp"
 #include "gemm.hpp"
 #include "kernels.hpp"
 
 namespace hllm_rocm {
-namespace {
 
-thread_local std::string g_last_error;
+std::string& last_error() {
+  thread_local std::string message;
+  return message;
+}
+
+namespace {
 
 uint64_t pad_to(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
 
@@ -1949,7 +1954,7 @@ void sample_logits(int32_t device, const float* logits, uint64_t rows, uint64_t 
 
 // ========================================================================= C ABI
 
-using hllm_rocm::Failure;
+using hllm_rocm::guarded;
 using hllm_rocm::Stage;
 
 struct hllm_rocm_stage {
@@ -1957,25 +1962,6 @@ struct hllm_rocm_stage {
 };
 
 namespace {
-template <typename F>
-hllm_status guarded(F&& f) {
-  try {
-    f();
-    return HLLM_OK;
-  } catch (const Failure& e) {
-    hllm_rocm::g_last_error = e.what();
-    return e.status;
-  } catch (const std::bad_alloc&) {
-    hllm_rocm::g_last_error = "host allocation failed";
-    return HLLM_RESOURCE_EXHAUSTED;
-  } catch (const std::exception& e) {
-    hllm_rocm::g_last_error = e.what();
-    return HLLM_INTERNAL;
-  } catch (...) {
-    hllm_rocm::g_last_error = "unknown failure";
-    return HLLM_INTERNAL;
-  }
-}
 Stage& impl(hllm_rocm_stage* s) {
   if (!s || !s->impl) hllm_rocm::fail(HLLM_INVALID_REQUEST, "null stage");
   return *s->impl;
@@ -1988,7 +1974,7 @@ const Stage& impl(const hllm_rocm_stage* s) {
 
 extern "C" {
 
-const char* hllm_rocm_last_error(void) { return hllm_rocm::g_last_error.c_str(); }
+const char* hllm_rocm_last_error(void) { return hllm_rocm::last_error().c_str(); }
 uint32_t hllm_rocm_abi_version(void) { return HLLM_ROCM_ABI_VERSION; }
 
 hllm_status hllm_rocm_stage_create(const hllm_rocm_stage_config* config, hllm_rocm_stage** out) {

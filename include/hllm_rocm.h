@@ -334,6 +334,170 @@ hllm_status hllm_rocm_stage_profile_read(hllm_rocm_stage* stage, const char* rec
 hllm_status hllm_rocm_stage_profile_records(hllm_rocm_stage* stage, char* buffer,
                                             uint64_t capacity, uint64_t* needed);
 
+/* ------------------------------------------------------------ operators on device memory
+ *
+ * Rotary positions and an 8-bit paged KV cache for callers that hold their activations and
+ * their cache in device memory of their own: the stage's rotation, K/V append and decode
+ * attention in other forms (positions scaled for long contexts, neighbouring pairs, part of
+ * a head; a cache of one byte a value). No counterpart in the reference.
+ *
+ * Every pointer inside these arguments is device memory of `device` unless it is a host
+ * structure named by a type of this header; `stream` is a hipStream_t of that device (NULL:
+ * its default stream). A call checks its arguments on the host (HLLM_INVALID_REQUEST, nothing
+ * enqueued), enqueues its kernels on `stream` and returns without waiting; it allocates
+ * nothing, keeps nothing between calls, leaves the thread's current device as it was and may
+ * be captured into a graph. `rows` = 0 enqueues nothing. Positions, slots, page tables and
+ * lengths are read by the device when the kernels run, so a captured call takes what they
+ * hold at each replay. Calls may run at once on several streams; what they write must not
+ * overlap. */
+
+/* One tensor [rows][heads][head_dimension]: the last dimension is contiguous, strides are in
+ * elements. `data` is 16-byte aligned and so is every head's vector (strides that are
+ * multiples of 16 bytes). Inputs may repeat memory (strides of 0); the vectors of an output
+ * may not overlap. */
+typedef struct {
+  void* data;
+  uint32_t dtype;        /* HLLM_DTYPE_* */
+  uint32_t heads;        /* 1 .. 1024 */
+  uint64_t row_stride;
+  uint64_t head_stride;
+} hllm_rocm_tensor;
+
+/* Which elements of a head's first `rotary_dimension` make the pairs that are rotated:
+ * (i, i + rotary_dimension / 2), or (2 i, 2 i + 1). */
+typedef enum { HLLM_ROPE_HALF = 0, HLLM_ROPE_INTERLEAVED = 1 } hllm_rope_layout;
+
+/* How pair i's frequency f = theta^(-2 i / rotary_dimension) is changed for contexts longer
+ * than the model was trained on:
+ *   LINEAR  f / factor
+ *   LLAMA3  f / factor for wavelengths 2 pi / f above original_length / low_frequency_factor,
+ *           f below original_length / high_frequency_factor, mixed in between
+ *   YARN    f / factor for pairs that turn less than `beta_slow` times over original_length, f
+ *           for those that turn more than `beta_fast` times, a ramp over the pair indices in
+ *           between; cos and sin times `magnitude` (0: 0.1 ln(factor) + 1) */
+typedef enum {
+  HLLM_ROPE_UNSCALED = 0,
+  HLLM_ROPE_LINEAR = 1,
+  HLLM_ROPE_LLAMA3 = 2,
+  HLLM_ROPE_YARN = 3,
+} hllm_rope_scaling;
+
+typedef struct {
+  uint32_t rotary_dimension;     /* even, 2 .. 256 */
+  uint32_t layout;               /* hllm_rope_layout */
+  uint32_t scaling;              /* hllm_rope_scaling; fields it does not use are not read */
+  double theta;                  /* > 1 */
+  double factor;                 /* >= 1 */
+  double original_length;        /* LLAMA3, YARN: > 0 */
+  double low_frequency_factor;   /* LLAMA3: > 0 */
+  double high_frequency_factor;  /* LLAMA3: > low_frequency_factor */
+  double beta_fast;              /* YARN: > beta_slow; 0 = 32 */
+  double beta_slow;              /* YARN: > 0; 0 = 1 */
+  double magnitude;              /* YARN: >= 0 */
+} hllm_rocm_rope_config;
+
+/* A rotation's plan, host memory filled by hllm_rocm_rope_plan and kept by the caller: each
+ * pair's frequency in turns (angle / 2 pi) a position, as a 64-bit binary fraction. The
+ * fraction of position x frequency is exact in 64-bit integers, so the angles are right to
+ * F32 at every 32-bit position (negative ones too). */
+typedef struct {
+  uint32_t rotary_dimension;
+  uint32_t layout;
+  float magnitude;
+  uint32_t reserved;
+  uint64_t turns[128];
+} hllm_rocm_rope;
+
+hllm_status hllm_rocm_rope_plan(const hllm_rocm_rope_config* config, hllm_rocm_rope* out);
+
+/* q_out = q and k_out = k (NULL, both: none) rotated at `positions` [rows], computed in F32 and
+ * rounded once; elements past the plan's rotary_dimension are copied. head_dimension is a
+ * multiple of 16, at most 256 and at least rotary_dimension; all tensors have one dtype. An output
+ * may be its own input (same data and strides), and otherwise overlaps no input. */
+hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_rope* rope,
+                                 const int32_t* positions, uint64_t rows, uint32_t head_dimension,
+                                 const hllm_rocm_tensor* q, const hllm_rocm_tensor* q_out,
+                                 const hllm_rocm_tensor* k, const hllm_rocm_tensor* k_out);
+
+/* What an 8-bit cache holds of a vector x (a position's key or value of one head): codes and one
+ * F32 scale, x ~= code * scale, with scale = max(|x|max, 2^-100) / c and code = x * (c /
+ * max(|x|max, 2^-100)) rounded to nearest even: c = 448 for E4M3 (OCP, 8-bit floating point: relative
+ * error at most 2^-4, the better for outliers) and 127 for INT8 (whole numbers: error at most
+ * |x|max / 254, the smaller for even distributions). A vector with a value that is not finite
+ * gets the scale NaN and codes 0: it reads back as NaN. */
+typedef enum { HLLM_KV_E4M3 = 0, HLLM_KV_INT8 = 1 } hllm_kv_format;
+
+/* A paged cache in device memory: codes at page * page_stride + position * token_stride + head *
+ * head_stride (bytes, multiples of 16; either of positions and heads inside the other; vectors
+ * may not overlap) and scales [pages][kv_heads][page_tokens], for keys and values alike. A slot
+ * is page * page_tokens + position in the page. All four pointers are 16-byte aligned. */
+typedef struct {
+  uint32_t format;          /* hllm_kv_format */
+  uint32_t pages;           /* pages * page_tokens < 2^31 */
+  uint32_t page_tokens;     /* a power of two, 8 .. 4096 */
+  uint32_t kv_heads;        /* 1 .. 1024 */
+  uint32_t head_dimension;  /* 64, 128 or 256 */
+  uint64_t page_stride;
+  uint64_t token_stride;
+  uint64_t head_stride;
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+} hllm_rocm_kv_pages;
+
+/* Quantises rows of k and v [rows][kv_heads] into the cache at `slots` [rows]. With `rope`, k is rotated at
+ * `positions` first (in F32, not rounded in between) and, with q (NULL, both: none), q_out = q
+ * rotated, as hllm_rocm_rope_apply does; without `rope`, q must be NULL. A row whose slot is not
+ * in [0, pages * page_tokens) is padding: nothing is written for it, q_out included. Slots of
+ * other rows must differ: what is left in a slot that two rows name is not specified. */
+hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                                const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
+                                const hllm_rocm_tensor* v, const hllm_rocm_rope* rope,
+                                const int32_t* positions, const hllm_rocm_tensor* q,
+                                const hllm_rocm_tensor* q_out);
+
+/* The cached vectors at `slots` [rows] (any order, repeats allowed) as k_out and v_out
+ * [rows][kv_heads], code * scale in F32 rounded once. Rows whose slot is not in the cache are
+ * padding and left as they were. */
+hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                              const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k_out,
+                              const hllm_rocm_tensor* v_out);
+
+/* One new token's attention for each row, over a sequence in the cache: out = softmax(scale q
+ * K^T) V with the keys and values of positions 0 .. lengths[row] - 1 of the row's pages; query
+ * heads share KV heads in groups of q.heads / kv_heads. Scores, softmax and sums are F32; products
+ * take codes exactly, and q and the weights as F16 (F16 and BF16 tensors, each vector's largest
+ * weight scaled to 1) or as sums of two F16 values (F32 tensors).
+ *
+ * A row's length counts at most max_length and table_width * page_tokens positions; a length
+ * of 0 gives zeros and a negative one marks a padding row, which is left as it was. Positions in
+ * pages outside [0, pages) take no part, as if they were masked (a dropped page is -1); a row
+ * with no other position gives zeros. What lies in a page behind a row's length is not used,
+ * NaN or not. */
+typedef struct {
+  uint64_t rows;
+  const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */
+  uint64_t table_width;       /* table_width * page_tokens < 2^31 */
+  uint64_t table_stride;
+  const int32_t* lengths;     /* [rows] */
+  uint64_t max_length;        /* the host's bound of the lengths: work is split for it */
+  float scale;
+  hllm_rocm_tensor q;
+  hllm_rocm_tensor out;       /* q's dtype and heads; not overlapping q */
+  void* workspace;            /* 16-byte aligned; used while the call's kernels run, so calls that
+                               * may run at once need one each; no contents are required */
+  uint64_t workspace_bytes;   /* at least hllm_rocm_kv_attention_workspace */
+} hllm_rocm_kv_attention_args;
+
+hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                                   const hllm_rocm_kv_attention_args* args);
+/* The workspace that a call with `rows` rows of `query_heads` heads and this max_length needs
+ * (0: none, and `workspace` may be NULL). Needs no device. */
+hllm_status hllm_rocm_kv_attention_workspace(const hllm_rocm_kv_pages* pages, uint64_t rows,
+                                             uint32_t query_heads, uint64_t max_length,
+                                             uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,282 @@
+"""CPU checks of the operators on device memory: rotation plans against the scalings' formulas,
+every refusal of the C entry points (made before a device is touched) and the ctypes layouts."""
+import ctypes as C
+import math
+import os
+import subprocess
+import tempfile
+
+import pytest
+
+from hllm_amd import capi
+from tests.operator_forms import LLAMA3, YARN, frequencies
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ADDRESS = 1 << 20  # a 16-byte aligned address that no refused call reads
+
+
+def refused(status, text=""):
+    assert status == capi.INVALID_REQUEST, (status, capi.library().hllm_rocm_last_error())
+    assert text.encode() in capi.library().hllm_rocm_last_error(), capi.library().hllm_rocm_last_error()
+
+
+# ------------------------------------------------------------------ plans
+
+
+@pytest.mark.parametrize("rotary,theta", [(128, 1e6), (64, 5e5), (20, 1e4), (2, 10.0), (256, 1000042.0)])
+@pytest.mark.parametrize("scaling", [None, {"rope_type": "linear", "factor": 4.0}, LLAMA3, YARN,
+                                     dict(YARN, beta_fast=16.0, beta_slow=2.0, attention_factor=1.25)])
+def test_plan_holds_the_frequencies(rotary, theta, scaling):
+    from hllm_amd import operators
+
+    plan = operators.Rope(rotary, theta=theta, scaling=scaling).plan
+    expect, magnitude = frequencies(rotary, theta, scaling)
+    for i, f in enumerate(expect):
+        # Frequencies are doubles here: a few roundings of 2^-53, and half a unit of 2^-64 turn.
+        assert math.isclose(plan.turns[i] / 2.0 ** 64, f / (2 * math.pi), rel_tol=1e-14, abs_tol=2.0 ** -65)
+    assert all(t == 0 for t in plan.turns[rotary // 2:])
+    assert plan.magnitude == pytest.approx(magnitude, rel=2.0 ** -23)
+    assert plan.rotary_dimension == rotary and plan.layout == capi.ROPE_HALF
+
+
+def config(**changes):
+    c = capi.RopeConfig(rotary_dimension=64, theta=1e4, factor=2.0, original_length=4096.0, low_frequency_factor=1.0,
+                        high_frequency_factor=4.0)
+    for name, value in changes.items():
+        setattr(c, name, value)
+    return c
+
+
+@pytest.mark.parametrize("changes", [
+    dict(rotary_dimension=0), dict(rotary_dimension=7), dict(rotary_dimension=258), dict(layout=2), dict(scaling=4),
+    dict(theta=1.0), dict(theta=math.nan), dict(theta=math.inf), dict(scaling=capi.ROPE_LINEAR, factor=0.5),
+    dict(scaling=capi.ROPE_LINEAR, factor=math.nan), dict(scaling=capi.ROPE_LLAMA3, original_length=0.0),
+    dict(scaling=capi.ROPE_LLAMA3, low_frequency_factor=-1.0), dict(scaling=capi.ROPE_LLAMA3, high_frequency_factor=1.0),
+    dict(scaling=capi.ROPE_YARN, original_length=-1.0), dict(scaling=capi.ROPE_YARN, beta_fast=1.0),
+    dict(scaling=capi.ROPE_YARN, beta_slow=-2.0), dict(scaling=capi.ROPE_YARN, magnitude=-1.0),
+    dict(scaling=capi.ROPE_YARN, magnitude=math.nan)])
+def test_plan_refuses(changes):
+    lib = capi.library()
+    assert lib.hllm_rocm_rope_plan(C.byref(config()), C.byref(capi.RopePlan())) == capi.OK
+    plan = capi.RopePlan(rotary_dimension=5)
+    refused(lib.hllm_rocm_rope_plan(C.byref(config(**changes)), C.byref(plan)))
+    assert plan.rotary_dimension == 5  # untouched
+    refused(lib.hllm_rocm_rope_plan(None, C.byref(plan)), "null")
+    refused(lib.hllm_rocm_rope_plan(C.byref(config()), None), "null")
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "dynamic", "factor": 2.0}, {"factor": 2.0}, {"rope_type": "linear"},
+    {"rope_type": "linear", "factor": 2.0, "mscale": 1.0}, {"rope_type": "default", "factor": 2.0},
+    {"rope_type": "llama3", "factor": 8.0}, {"rope_type": "yarn", "type": "linear", "factor": 2.0},
+    dict(YARN, truncate=False)])
+def test_rope_refuses_scalings_it_does_not_know(scaling):
+    from hllm_amd import operators
+
+    with pytest.raises(ValueError):
+        operators.Rope(64, scaling=scaling)
+
+
+def test_rope_takes_checkpoint_forms():
+    from hllm_amd import operators
+
+    plain = operators.Rope(64, theta=1e4)
+    for scaling in ({}, {"rope_type": "default"}, {"type": "default"}):
+        assert list(operators.Rope(64, theta=1e4, scaling=scaling).plan.turns) == list(plain.plan.turns)
+    both = operators.Rope(64, scaling={"rope_type": "linear", "type": "linear", "factor": 2.0})
+    assert both.plan.turns[0] == plain.plan.turns[0] // 2
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def tensor(heads=8, dim=128, dtype=capi.F16, **changes):
+    t = capi.Tensor(ADDRESS, dtype, heads, heads * dim, dim)
+    for name, value in changes.items():
+        setattr(t, name, value)
+    return t
+
+
+def cache(**changes):
+    c = capi.KvPages(capi.KV_E4M3, 10, 64, 8, 128, 8 * 64 * 128, 128, 64 * 128, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+    for name, value in changes.items():
+        setattr(c, name, value)
+    return c
+
+
+def plan(**changes):
+    p = capi.RopePlan()
+    capi.check(capi.library().hllm_rocm_rope_plan(C.byref(config(**changes)), C.byref(p)))
+    return p
+
+
+def by(x):
+    return None if x is None else C.byref(x)
+
+
+BAD_TENSORS = [(None, "null"), (dict(data=None), "no memory"), (dict(data=ADDRESS + 8), "aligned"), (dict(dtype=3), "dtype"),
+               (dict(heads=0), "heads"), (dict(row_stride=1028), "16 bytes"), (dict(head_stride=1 << 41), "too large")]
+BAD_OUTPUTS = BAD_TENSORS + [(dict(row_stride=0), "overlap"), (dict(head_stride=64), "overlap"), (dict(row_stride=512), "overlap")]
+BAD_PAGES = [(None, "null"), (dict(format=2), "format"), (dict(head_dimension=96), "head dimension"), (dict(kv_heads=0), "heads"),
+             (dict(page_tokens=48), "power of two"), (dict(page_tokens=4), "power of two"), (dict(page_tokens=8192), "power of two"),
+             (dict(pages=0), "slots"), (dict(pages=1 << 25), "slots"), (dict(keys=None), "null"), (dict(value_scales=None), "null"),
+             (dict(values=ADDRESS + 4), "aligned"), (dict(key_scales=ADDRESS + 4), "aligned"), (dict(token_stride=136), "16 bytes"),
+             (dict(page_stride=8 * 64 * 128 - 16), "overlap"), (dict(token_stride=64), "overlap"), (dict(head_stride=128), "overlap"),
+             (dict(page_stride=1 << 41), "too large")]
+
+
+def pages_or_none(changes):
+    return None if changes is None else cache(**changes)
+
+
+def test_rope_apply_refuses():
+    lib = capi.library()
+
+    def call(device=0, rope=plan(), positions=ADDRESS, rows=4, dim=128, q=tensor(), q_out=tensor(), k=None, k_out=None):
+        return lib.hllm_rocm_rope_apply(device, None, by(rope), positions, rows, dim, by(q), by(q_out), by(k), by(k_out))
+
+    assert call(rows=0) == capi.OK
+    for changes, text in BAD_TENSORS:
+        bad = None if changes is None else tensor(**changes)
+        refused(call(q=bad), text)
+        if changes is not None:
+            refused(call(k=bad, k_out=tensor()), text)
+    for changes, text in BAD_OUTPUTS:
+        bad = None if changes is None else tensor(**changes)
+        refused(call(q_out=bad), text)
+        if changes is not None:
+            refused(call(k=tensor(data=2 * ADDRESS), k_out=bad), text)
+    refused(call(device=-1), "device")
+    refused(call(rope=None), "rope")
+    refused(call(rope=capi.RopePlan()), "plan")
+    refused(call(positions=None), "positions")
+    refused(call(rows=(1 << 20) + 1), "rows")
+    for dim in (0, 8, 72, 272):
+        refused(call(dim=dim), "head dimension")
+    refused(call(dim=48), "rotary")
+    refused(call(k=tensor()), "together")
+    refused(call(k_out=tensor()), "together")
+    refused(call(q_out=tensor(dtype=capi.BF16)), "dtype")
+    refused(call(q_out=tensor(heads=4)), "heads")
+    refused(call(k=tensor(dtype=capi.F32), k_out=tensor(dtype=capi.F32)), "one dtype")
+    refused(call(q_out=tensor(row_stride=2048)), "strides")  # q's memory at other strides
+
+
+def test_kv_append_refuses():
+    lib = capi.library()
+
+    def call(device=0, pages=cache(), slots=ADDRESS, rows=4, k=tensor(), v=tensor(), rope=None, positions=None, q=None, q_out=None):
+        return lib.hllm_rocm_kv_append(device, None, by(pages), slots, rows, by(k), by(v), by(rope), positions, by(q), by(q_out))
+
+    assert call(rows=0) == capi.OK
+    for changes, text in BAD_PAGES:
+        refused(call(pages=pages_or_none(changes)), text)
+    for changes, text in BAD_TENSORS:
+        bad = None if changes is None else tensor(**changes)
+        refused(call(k=bad), text)
+        refused(call(v=bad), text)
+    refused(call(device=-2), "device")
+    refused(call(slots=None), "slots")
+    refused(call(rows=(1 << 20) + 1), "rows")
+    refused(call(k=tensor(heads=4)), "heads")
+    refused(call(v=tensor(heads=16)), "heads")
+    refused(call(v=tensor(dtype=capi.F32)), "one dtype")
+    refused(call(rope=plan()), "positions")
+    refused(call(rope=plan(rotary_dimension=256), positions=ADDRESS), "rotary")
+    refused(call(q=tensor(), q_out=tensor()), "rope")
+    refused(call(q=tensor(), rope=plan(), positions=ADDRESS), "together")
+    refused(call(q=tensor(dtype=capi.BF16), q_out=tensor(dtype=capi.BF16), rope=plan(), positions=ADDRESS), "one dtype")
+    refused(call(q=tensor(), q_out=tensor(row_stride=0), rope=plan(), positions=ADDRESS), "overlap")
+
+
+def test_kv_read_refuses():
+    lib = capi.library()
+
+    def call(device=0, pages=cache(), slots=ADDRESS, rows=4, k=tensor(), v=tensor()):
+        return lib.hllm_rocm_kv_read(device, None, by(pages), slots, rows, by(k), by(v))
+
+    assert call(rows=0) == capi.OK
+    for changes, text in BAD_PAGES:
+        refused(call(pages=pages_or_none(changes)), text)
+    for changes, text in BAD_OUTPUTS:
+        bad = None if changes is None else tensor(**changes)
+        refused(call(k=bad), text)
+        refused(call(v=bad), text)
+    refused(call(slots=None), "slots")
+    refused(call(device=-1), "device")
+    refused(call(rows=(1 << 20) + 1), "rows")
+    refused(call(k=tensor(heads=4)), "heads")
+    refused(call(v=tensor(dtype=capi.F32)), "one dtype")
+    wide = cache(kv_heads=1024, head_dimension=256, head_stride=64 * 256, token_stride=256, page_stride=1024 * 64 * 256)
+    big = tensor(heads=1024, dim=256)
+    refused(call(pages=wide, rows=1 << 20, k=big, v=big), "too many rows")
+
+
+def test_kv_attention_refuses():
+    lib = capi.library()
+
+    def call(device=0, pages=cache(), **changes):
+        a = capi.KvAttentionArgs(4, ADDRESS, 10, 10, ADDRESS, 600, 0.1, tensor(heads=32), tensor(heads=32, data=2 * ADDRESS),
+                                 ADDRESS, 1 << 30)
+        for name, value in changes.items():
+            setattr(a, name, value)
+        return lib.hllm_rocm_kv_attention(device, None, by(pages), C.byref(a))
+
+    assert call(rows=0) == capi.OK
+    for changes, text in BAD_PAGES:
+        refused(call(pages=pages_or_none(changes)), text)
+    for changes, text in BAD_TENSORS[1:]:
+        refused(call(q=tensor(**{"heads": 32, **changes})), text)
+    for changes, text in BAD_OUTPUTS[1:]:
+        refused(call(out=tensor(**{"heads": 32, "data": 2 * ADDRESS, **changes})), text)
+    refused(lib.hllm_rocm_kv_attention(0, None, C.byref(cache()), None), "null")
+    refused(call(device=-1), "device")
+    refused(call(rows=(1 << 20) + 1), "rows")
+    refused(call(out=tensor(heads=32)), "must not be q")
+    refused(call(out=tensor(heads=32, data=2 * ADDRESS, dtype=capi.BF16)), "dtype")
+    refused(call(out=tensor(heads=16, data=2 * ADDRESS)), "heads")
+    refused(call(q=tensor(heads=12), out=tensor(heads=12, data=2 * ADDRESS)), "multiple")
+    for scale in (math.nan, math.inf):
+        refused(call(scale=scale), "scale")
+    refused(call(lengths=None), "lengths")
+    refused(call(page_table=None), "page_table")
+    refused(call(table_width=1 << 26), "page table")
+    refused(call(table_stride=1 << 41), "table_stride")
+    refused(call(workspace=None), "workspace")
+    refused(call(workspace=ADDRESS + 4), "workspace")
+    refused(call(workspace_bytes=16), "workspace")
+
+
+def test_kv_attention_workspace_needs_no_device():
+    lib, need = capi.library(), C.c_uint64(1)
+
+    def size(rows, heads, length, pages=cache()):
+        status = lib.hllm_rocm_kv_attention_workspace(by(pages), rows, heads, length, C.byref(need))
+        assert status in (capi.OK, capi.INVALID_REQUEST)
+        return need.value if status == capi.OK else None
+
+    assert size(0, 32, 4096) == 0
+    assert size(4, 32, 0) == 0 and size(1, 8, 20) == 0
+    assert size(1, 32, 1 << 17) > 0
+    # No more than a bounded number of parts, whatever the length's bound.
+    assert size(1, 32, 1 << 20) <= 2 * size(1, 32, 1 << 19)
+    assert size(3, 12, 100) is None and size(3, 0, 100) is None
+    refused(lib.hllm_rocm_kv_attention_workspace(None, 1, 8, 100, C.byref(need)), "null")
+    refused(lib.hllm_rocm_kv_attention_workspace(C.byref(cache()), 1, 8, 100, None), "null")
+
+
+@pytest.mark.parametrize("struct,cname", [(capi.Tensor, "hllm_rocm_tensor"), (capi.RopeConfig, "hllm_rocm_rope_config"),
+                                          (capi.RopePlan, "hllm_rocm_rope"), (capi.KvPages, "hllm_rocm_kv_pages"),
+                                          (capi.KvAttentionArgs, "hllm_rocm_kv_attention_args")])
+def test_layouts_match_the_header(struct, cname):
+    fields = [f for f, _ in struct._fields_]
+    body = "\n".join(f'  printf("%zu ", offsetof({cname}, {f}));' for f in fields)
+    source = f'#include <stddef.h>\n#include <stdio.h>\n#include "hllm_rocm.h"\nint main(void) {{\n{body}\n' \
+             f'  printf("%zu\\n", sizeof({cname}));\n  return 0;\n}}\n'
+    with tempfile.TemporaryDirectory() as d:
+        c_file, exe = os.path.join(d, "probe.c"), os.path.join(d, "probe")
+        with open(c_file, "w") as f:
+            f.write(source)
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c_file, "-o", exe], check=True)
+        got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [getattr(struct, f).offset for f in fields] + [C.sizeof(struct)]
