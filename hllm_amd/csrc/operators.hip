@@ -3,7 +3,9 @@
 #include "operators.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "abi.hpp"
 
@@ -11,9 +13,10 @@ namespace hllm_rocm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 
 typedef __bf16 bhalf;
+typedef bhalf bhalf4 __attribute__((ext_vector_type(4)));
 typedef bhalf bhalf8 __attribute__((ext_vector_type(8)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
@@ -45,6 +48,13 @@ __device__ inline void store8(_Float16* p, const float* x) {
   for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
   *reinterpret_cast<half8*>(p) = h;
 }
+__device__ inline void store4(_Float16* p, floatx4 x) {
+  *reinterpret_cast<half4*>(p) = half4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
+__device__ inline void store4(bhalf* p, floatx4 x) {
+  *reinterpret_cast<bhalf4*>(p) = bhalf4{(bhalf)x[0], (bhalf)x[1], (bhalf)x[2], (bhalf)x[3]};
+}
+__device__ inline void store4(float* p, floatx4 x) { *reinterpret_cast<floatx4*>(p) = x; }
 __device__ inline void store8(bhalf* p, const float* x) {
   bhalf8 h;
 #pragma unroll
@@ -265,10 +275,13 @@ __device__ inline floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// The largest of a value over the four lanes of a column (lanes 16 apart).
+// The largest of a value over the four lanes of a column (lanes 16 apart), with the row swaps
+// of the vector unit: shuffles through LDS cost 0.1 us a tile more.
 __device__ inline float column_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(half[0]), __uint_as_float(half[1]));
+  const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(row[0]), __uint_as_float(row[1]));
 }
 __device__ inline float column_sum(float v) {
   v += __shfl_xor(v, 16, 64);
@@ -290,47 +303,212 @@ __device__ inline void halves4(uint32_t w, half2v& lo, half2v& hi) {
   }
 }
 
+// Copies into LDS as lds_copy16, with an address a lane; and of one word a lane.
+__device__ inline void lds_copy16_at(const void* from, uint32_t lds_byte_offset) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds_byte_offset)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+__device__ inline void lds_copy4_at(const void* from, uint32_t lds_byte_offset) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds_byte_offset)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// A wave's tile of 32 positions in LDS: key and value rows and the 64 scales. A row's sixteen-byte
+// chunks are permuted (chunk k at k ^ swizzle) so that the eight rows whose chunks are read at once
+// lie in different banks.
+template <int D>
+struct Tile {
+  static constexpr int kScales = 64 * D, kBytes = kScales + 256, kBlock = kThreads / 64 * kBytes;
+  // Rows of keys (which = 0) and values, 64-byte rows with both of eight positions together.
+  static __device__ int row_at(int which, int row) {
+    if constexpr (D == 64) return (row >> 3) * 1024 + which * 512 + ((row & 7) ^ ((row >> 3) & 1)) * 64;
+    return which * 32 * D + row * D;
+  }
+  static __device__ int swizzle(int row) { return D == 64 ? row & 3 : (row & 3) + 4 * ((row >> 3) & 1); }
+};
+
+// Sum over the wave's lanes up to this one; lanes from `count` on do not matter.
+__device__ inline int wave_scan(int v, int lane, int count) {
+  for (int o = 1; o < 64 && o < count; o <<= 1) {
+    const int below = __shfl_up(v, o, 64);
+    if (lane >= o) v += below;
+  }
+  return v;
+}
+
+// The pairs (a row, a KV head, sixteen of its query heads) lie on a line, each as long as its steps of 128
+// positions (one tile a wave) and kPairCost more for starting it, and the line is cut into equal
+// shares: a workgroup may end one pair, take whole ones and begin another.
+__device__ inline int steps_of(int length) { return (length + 127) / 128; }
+__device__ inline int pair_units(int length) { return length < 0 ? 0 : steps_of(length) + kPairCost; }
+
+// Where vector v of a pair's part i lies in the workspace. A workgroup writes two parts at most: of a pair
+// that began before it and of one that goes on after it.
+__device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int v) {
+  return (uint64_t)(i == 0 ? 2 * first + 1 : 2 * (first + i)) * min(a.group, 16) + v;
+}
+
 template <typename T, int F, int D>
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kernel(AttendArgs a) {
+  using Layout = Tile<D>;
   constexpr int KK = D / 32;   // 32-wide chunks of the score contraction
   constexpr int DF = D / 16;   // 16-row fragments of the output; a lane's value bytes of a position
   constexpr int VW = DF / 4;   // ... in words
   constexpr int P = sizeof(T) == 4 ? 2 : 1;  // F16 parts of a query element and of a weight
-  __shared__ int32_t held[kAttendMostKeys / 8 + 1];
-  __shared__ float merge[4 * 4 * DF * 64];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ float states[4][3][16];
+  __shared__ half8 queries[P][KK][64];
 
   const Pages& c = a.pages;
-  const int KVH = c.kv_heads, shift = c.page_shift;
-  const int pairs = a.rows * KVH * a.head_groups;
-  const int split = blockIdx.x / pairs, pair = blockIdx.x - split * pairs;
-  const int row = pair / (KVH * a.head_groups), kvg = pair - row * KVH * a.head_groups;
-  const int kvh = kvg / a.head_groups, g0 = (kvg - kvh * a.head_groups) * 16;
-  const int stated = uniform_load(a.lengths + row);
-  if (stated < 0) return;
-  const int length = min(stated, a.limit);
-  const int per = attend_part(length, a.splits, a.unit);
-  const int begin = split * per;
-  if (begin >= length && split > 0) return;
-  const int end = min(length, begin + per);
-  const int parts = (length + per - 1) / per;
-
+  const int KVH = c.kv_heads, shift = c.page_shift, in_row = KVH * a.head_groups;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int quad = lane >> 4, col = lane & 15;
+  const int me = blockIdx.x;
+  const auto length_of = [&](int row) { return min(uniform_load(a.lengths + row), a.limit); };
+
+  // The share, units from .. to of the line, and its first pair. Without `shared` a workgroup
+  // takes one pair.
+  int row, kvg, start, from = 0, to, budget = INT_MAX, length, units;
+  if (a.shared) {
+    const int chunk = (a.rows + 63) / 64, lanes = (a.rows + chunk - 1) / chunk;  // rows of a lane, at most 16
+    int own = 0, own_length = 0;
+    for (int i = 0; i < chunk; ++i) {
+      const int r = lane * chunk + i;
+      if (r < a.rows) {
+        own_length = min(a.lengths[r], a.limit);
+        own += pair_units(own_length) * in_row;
+      }
+    }
+    int sum = wave_scan(own, lane, lanes);
+    const int total = __builtin_amdgcn_readlane(sum, lanes - 1);
+    budget = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    from = me * budget;
+    to = min(from + budget, total);
+    if (from >= to) return;
+    int at = __builtin_ctzll(__ballot(sum > from));
+    row = at * chunk;
+    start = __builtin_amdgcn_readlane(sum - own, at);
+    if (chunk > 1) {
+      own_length = min(a.lengths[min(row + lane, a.rows - 1)], a.limit);
+      own = lane < chunk && row + lane < a.rows ? pair_units(own_length) * in_row : 0;
+      sum = start + wave_scan(own, lane, chunk);
+      at = __builtin_ctzll(__ballot(sum > from));
+      row += at;
+      start = __builtin_amdgcn_readlane(sum - own, at);
+    }
+    length = __builtin_amdgcn_readlane(own_length, at);
+    units = pair_units(length);
+    kvg = (from - start) / units;
+    start += kvg * units;
+  } else {
+    row = me / in_row;
+    kvg = me - row * in_row;
+    start = 0;
+    length = length_of(row);
+    to = units = pair_units(length);
+    if (units == 0) return;
+  }
+  // The next pair of the share, if there is one: rows of negative lengths have none.
+  const auto next_pair = [&] {
+    start += units;
+    if (start >= to) return false;
+    if (++kvg < in_row) return true;
+    kvg = 0;
+    do {
+      length = length_of(++row);
+      units = pair_units(length);
+    } while (units == 0);
+    return true;
+  };
+
+  bool again = false;
+  for (bool more = true; more; more = next_pair()) {
+  // This share's steps of the pair, low .. high - 1, and the workgroups that have others.
+  const int steps = steps_of(length), first_unit = start + kPairCost;
+  const int low = max(from - first_unit, 0), high = min(steps, to - first_unit);
+  if (steps > 0 ? low >= high : start < from) continue;  // only the cost of starting it is this share's
+  const int first = first_unit / budget;
+  const int parts = a.shared && steps > 0 ? (first_unit + steps - 1) / budget - first + 1 : 1;
+  if (again) __syncthreads();  // the workgroup has read the last pair's sums
+  again = true;
+  const int kvh = kvg / a.head_groups, g0 = (kvg - kvh * a.head_groups) * 16;
+  const int begin = 128 * low, end = min(length, 128 * high);
+  if (again) __syncthreads();  // the workgroup has read the last pair's sums
+  again = true;
   const int vectors = min(16, a.group - g0);
 
-  // The part's page numbers, -1 for those that name no page.
-  const int first_page = begin >> shift, held_pages = ((end - 1) >> shift) - first_page + 1;
-  for (int i = threadIdx.x; i < held_pages; i += kThreads) {
-    const int id = a.table[(uint64_t)row * a.table_stride + first_page + i];
-    held[i] = id >= 0 && id < c.pages ? id : -1;
+  const int32_t* table = a.table + (uint64_t)row * a.table_stride;
+  const int mask = (1 << shift) - 1;
+  const uint32_t token = c.token_stride;
+  const uint8_t* keys = c.keys + (uint64_t)kvh * c.head_stride;
+  const uint8_t* values = c.values + (uint64_t)kvh * c.head_stride;
+  char* tile = smem + wave * Layout::kBytes;
+  const uint32_t tile_at = (uint32_t)(size_t)((__attribute__((address_space(3))) char*)smem) + wave * Layout::kBytes;
+
+  // One copy instruction takes 1 KiB: 16 / (D / 64) rows of 64 D.. bytes, so each lies in one group of
+  // eight positions, which is in one page; groups alternate between two sets of lane offsets.
+  uint32_t lane_at[2];
+  const uint8_t* lane_from[2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd) {
+    constexpr int kChunks = D / 16;
+    if constexpr (D == 64) {
+      const int r = ((lane >> 2) & 7) ^ odd, chunk = (lane & 3) ^ Layout::swizzle(r);
+      lane_from[odd] = (lane < 32 ? keys : values) + (uint32_t)r * token + chunk * 16;
+    } else {
+      const int r = lane / kChunks, chunk = lane % kChunks ^ Layout::swizzle(r + 8 * odd);
+      lane_at[odd] = (uint32_t)r * token + chunk * 16;
+    }
+  }
+  const float* lane_scales = lane < 32 ? c.key_scales : c.value_scales;
+  // The table's entries of a tile's four groups (of the last position's group behind the part).
+  int ids[4];
+  const auto load_ids = [&](int t) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) ids[g] = uniform_load(table + (min(t + 8 * g, end - 1) >> shift));
+  };
+  // Starts a tile's copies; returns a bit for each group whose page is not there.
+  const auto copy_tile = [&](int t) {
+    int missing = 0, pages[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const bool there = ids[g] >= 0 && ids[g] < c.pages;
+      missing |= there ? 0 : 1 << g;
+      pages[g] = there ? ids[g] : 0;
+      const uint64_t page_at = (uint64_t)(uint32_t)pages[g] * c.page_stride + (uint64_t)(uint32_t)((t + 8 * g) & mask) * token;
+      if constexpr (D == 64) {
+        lds_copy16_at(lane_from[g & 1] + page_at, tile_at + g * 1024);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          lds_copy16(keys + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + (g * (D / 128) + i) * 1024);
+          lds_copy16(values + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + 32 * D + (g * (D / 128) + i) * 1024);
+        }
+      }
+    }
+    const int group = (lane & 31) >> 3;
+    const int page = group & 2 ? (group & 1 ? pages[3] : pages[2]) : (group & 1 ? pages[1] : pages[0]);
+    lds_copy4_at(lane_scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + (lane & 31)) & mask)), tile_at + Layout::kScales);
+    return missing;
+  };
+
+  int t = begin + 32 * wave, missing = 0;
+  if (t < end) {
+    load_ids(t);
+    missing = copy_tile(t);
+    load_ids(min(t + 128, end - 1));
   }
 
-  // Q^T as the B operand: chunk kk = 2 hh + s holds elements 64 hh + 16 quad + 8 s + j, the order
+  // Q^T as the B operand, kept in LDS for the four waves: chunk kk = 2 hh + s holds elements 64 hh + 16 quad + 8 s + j, the order
   // of a key's sixteen bytes. Each vector is divided by the power of two of its
   // largest element, which puts F32 and BF16 ranges into F16's and goes back into its scores.
-  half8 qf[P][KK];
-  float factor;
+  float factor, factor_lo;
   {
     float x[KK][8];
     const T* src = at<const T>(a.q, row, kvh * a.group + g0 + min(col, vectors - 1), 16 * quad);
@@ -347,101 +525,125 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(AttendArgs a) {
     const uint32_t exponent = most >> 23;
     const bool usual = exponent >= 1 && exponent <= 253;
     const float down = usual ? __uint_as_float((254u - exponent) << 23) : 1.0f;
-    factor = a.scale * kLog2e * (usual ? __uint_as_float(exponent << 23) : 1.0f);
+    const float up = usual ? __uint_as_float(exponent << 23) : 1.0f;
+    factor = a.scale_hi * up;
+    factor_lo = a.scale_lo * up;
+    if (wave == 0) {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+      for (int kk = 0; kk < KK; ++kk) {
+        half8 part[P];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = x[kk][j] * down;
-        qf[0][kk][j] = (_Float16)y;
-        if constexpr (P == 2) qf[1][kk][j] = (_Float16)(y - (float)qf[0][kk][j]);
+        for (int j = 0; j < 8; ++j) {
+          const float y = x[kk][j] * down;
+          part[0][j] = (_Float16)y;
+          if constexpr (P == 2) part[1][j] = (_Float16)(y - (float)part[0][j]);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) queries[p][kk][lane] = part[p];
       }
+    }
   }
   __syncthreads();
 
+
   // The weights of a position are 2^(score - m) times its value scale; they enter the products
-  // divided by their running maximum r, and so do the sums o.
+  // divided by r, and so do the sums o. r is a weight that was the largest once: it follows m, and is
+  // raised when a weight is 2^12 times as large, so that o is seldom rescaled and F16 holds
+  // every weight to 2^-11 or to 2^-25 of the largest.
   floatx4 o[DF];
 #pragma unroll
   for (int f = 0; f < DF; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f, r = 0.0f;
 
-  const uint64_t head_at = (uint64_t)kvh * c.head_stride;
-  const uint8_t* keys = c.keys + head_at + 16 * quad;
-  const uint8_t* values = c.values + head_at + DF * col;
-  const int mask = (1 << shift) - 1;
-  const uint64_t token = c.token_stride;
-  for (int t = begin + 32 * wave; t < end; t += 128) {
-    // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are the eight
-    // positions 8 quad .. + 7, which are also its slots of the value products.
-    const int key_at = t + 8 * (col >> 2), own_at = t + 8 * quad;
-    const int key_page = held[min((key_at >> shift) - first_page, held_pages - 1)];
-    const int own_page = held[min((own_at >> shift) - first_page, held_pages - 1)];
-    const uint8_t* kp = keys + (uint64_t)max(key_page, 0) * c.page_stride + (uint64_t)((key_at & mask) + (col & 3)) * token;
-    const uint8_t* vp = values + (uint64_t)max(own_page, 0) * c.page_stride + (uint64_t)(own_at & mask) * token;
-    const uint64_t scale_at = (((uint64_t)max(own_page, 0) * KVH + kvh) << shift) + (own_at & mask);
-    uint4v kw[2][D / 64];
+  // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are the eight
+  // positions 8 quad .. + 7, which are also its slots of the value products.
+  const int key_row = 8 * (col >> 2) + (col & 3);
+  const int key_lane = Layout::row_at(0, key_row) + ((quad ^ Layout::swizzle(key_row)) * 16);
+  const int value_lane = Layout::row_at(1, 8 * quad) + ((DF * col / 16 ^ Layout::swizzle(8 * quad)) * 16) + DF * col % 16;
+  for (; t < end; t += 128) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int gone = missing;
+    const bool whole = gone == 0 && t + 32 <= end;
+    if (!whole) {
+      // Values of positions past the part and in pages that are not there, whatever they are.
+      const int own = lane >> 1;
+      if (t + own >= end || (gone >> (own >> 3)) & 1) {
+        char* line = tile + Layout::row_at(1, own) + (lane & 1) * (D / 2);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < D / 32; ++i) *reinterpret_cast<uint4v*>(line + 16 * i) = uint4v{0, 0, 0, 0};
+        reinterpret_cast<float*>(tile + Layout::kScales)[32 + own] = 0.0f;
+      }
+    }
+    floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int hh = 0; hh < D / 64; ++hh) kw[h][hh] = *reinterpret_cast<const uint4v*>(kp + 4 * h * token + 64 * hh);
+    for (int hh = 0; hh < D / 64; ++hh) {
+      const int at_hh = (key_lane ^ (hh & 1) * 64) + (hh >> 1) * 128;
+      uint4v kw[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) kw[h] = *reinterpret_cast<const uint4v*>(tile + at_hh + 4 * D * h);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        half8 k[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            half2v lo, hi;
+            halves4<F>(kw[h][2 * s + w], lo, hi);
+            k[h][4 * w] = lo[0];
+            k[h][4 * w + 1] = lo[1];
+            k[h][4 * w + 2] = hi[0];
+            k[h][4 * w + 3] = hi[1];
+          }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const half8 q = queries[p][2 * hh + s][lane];
+          s0 = mfma(k[0], q, s0);
+          s1 = mfma(k[1], q, s1);
+        }
+      }
+    }
+    // F32 tensors keep the scores' factors as sums of two floats and round a score once, after the
+    // maximum is taken away: a score of some tens rounded by itself moves its weight by 1e-6.
+    float sc[8], ks[8], by_lo[8], vs[8];
+    load8(reinterpret_cast<const float*>(tile + Layout::kScales) + 8 * quad, ks);
+    load8(reinterpret_cast<const float*>(tile + Layout::kScales) + 32 + 8 * quad, vs);
     uint32_t vw[8][VW];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (VW == 1) vw[j][0] = *reinterpret_cast<const uint32_t*>(vp + j * token);
+      const char* line = D == 64 ? tile + (value_lane ^ (j * 64 + (j & 3) * 16)) : tile + (value_lane ^ (j & 3) * 16) + j * D;
+      if constexpr (VW == 1) vw[j][0] = *reinterpret_cast<const uint32_t*>(line);
       if constexpr (VW == 2) {
-        const uint2v w = *reinterpret_cast<const uint2v*>(vp + j * token);
+        const uint2v w = *reinterpret_cast<const uint2v*>(line);
         vw[j][0] = w[0];
         vw[j][1] = w[1];
       }
       if constexpr (VW == 4) {
-        const uint4v w = *reinterpret_cast<const uint4v*>(vp + j * token);
+        const uint4v w = *reinterpret_cast<const uint4v*>(line);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vw[j][i] = w[i];
       }
     }
-    float ks[8], vs[8];
-    load8(c.key_scales + scale_at, ks);
-    load8(c.value_scales + scale_at, vs);
-
-    floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      half8 k[2];
+    for (int i = 0; i < 8; ++i) {
+      const float d = i < 4 ? s0[i & 3] : s1[i & 3];
+      const float by = ks[i] * factor;
+      sc[i] = d * by;
+      if constexpr (P == 2) by_lo[i] = fmaf(d, by, -sc[i]) + d * (fmaf(ks[i], factor, -by) + ks[i] * factor_lo);
+    }
+    if (!whole) {
+      const int valid = (gone >> quad) & 1 ? 0 : end - (t + 8 * quad);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          half2v lo, hi;
-          halves4<F>(kw[h][kk >> 1][2 * (kk & 1) + w], lo, hi);
-          k[h][4 * w] = lo[0];
-          k[h][4 * w + 1] = lo[1];
-          k[h][4 * w + 2] = hi[0];
-          k[h][4 * w + 3] = hi[1];
-        }
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        s0 = mfma(k[0], qf[p][kk], s0);
-        s1 = mfma(k[1], qf[p][kk], s1);
+      for (int i = 0; i < 8; ++i) {
+        sc[i] = i < valid ? sc[i] : -INFINITY;
+        if constexpr (P == 2) by_lo[i] = i < valid ? by_lo[i] : 0.0f;
       }
     }
-    float sc[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sc[i] = s0[i] * (ks[i] * factor);
-      sc[4 + i] = s1[i] * (ks[4 + i] * factor);
-    }
-    // Positions past the part and in pages that are not there: whatever their memory holds.
-    const int valid = own_page < 0 ? 0 : end - own_at;
-    if (__any(valid < 8)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i >= valid) {
-          sc[i] = -INFINITY;
-          vs[i] = 0.0f;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) vw[i][w] = 0;
-        }
+    // The tile is in registers: the next one's copies start.
+    if (t + 128 < end) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      missing = copy_tile(t + 128);
+      load_ids(min(t + 256, end - 1));
     }
     float most = sc[0];
 #pragma unroll
@@ -452,21 +654,29 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(AttendArgs a) {
     float weight[8], sum = 0.0f, largest = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float p = exp2_fast(sc[i] - base);
+      const float p = exp2_fast(P == 2 ? (sc[i] - base) + by_lo[i] : sc[i] - base);
       sum += p;
       weight[i] = p * vs[i];
       largest = fmaxf(largest, weight[i]);
     }
     l = l * decay + sum;
     m = m_new;
-    const float r_old = r * decay;
-    r = fmaxf(r_old, column_max(largest));
-    const float over = r > 0x1p-120f ? 1.0f / r : 0.0f;  // smaller sums are nothing
-    const float rescale = r_old * over;
+    r *= decay;
+    largest = column_max(largest);
+    if (__any(largest > 4096.0f * r)) {
+      const float raised = fmaxf(r, largest), rescale = raised > r ? r / raised : 1.0f;
+#pragma unroll
+      for (int f = 0; f < DF; ++f) o[f] *= rescale;
+      r = raised;
+    }
+    const float over = r > 0x1p-125f ? __builtin_amdgcn_rcpf(r) : 0.0f;  // smaller weights are nothing
     half8 pf[P];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float w = weight[i] * over;
+      float w = weight[i] * over;
+      // As a value of its own: rounded with the product in one step, the first part would differ
+      // from the one that the second part is the rest of.
+      if constexpr (P == 2) asm("" : "+v"(w));
       pf[0][i] = (_Float16)w;
       if constexpr (P == 2) pf[1][i] = (_Float16)(w - (float)pf[0][i]);
     }
@@ -489,109 +699,112 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(AttendArgs a) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        floatx4 acc = o[4 * w + i] * rescale;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int p = 0; p < P; ++p) acc = mfma(v[i], pf[p], acc);
-        o[4 * w + i] = acc;
-      }
+        for (int p = 0; p < P; ++p) o[4 * w + i] = mfma(v[i], pf[p], o[4 * w + i]);
     }
   }
 
-  // The four waves' states meet in LDS; wave i then sums and writes the elements of the
-  // accumulators' component i.
+  // The four waves' states meet in LDS, each wave's in its own tile.
   l = column_sum(l);
   if (quad == 0) {
     states[wave][0][col] = m;
     states[wave][1][col] = l;
     states[wave][2][col] = r;
   }
+  static_assert(Layout::kBytes >= 4 * DF * 64 * 4, "a wave's sums lie in its tile");
+  // A lane's component i of four fragments: four elements that follow one another.
 #pragma unroll
-  for (int f = 0; f < DF; ++f)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) merge[((wave * 4 + i) * DF + f) * 64 + lane] = o[f][i];
+    for (int k = 0; k < VW; ++k)
+      reinterpret_cast<floatx4*>(tile)[(i * VW + k) * 64 + lane] = floatx4{o[4 * k][i], o[4 * k + 1][i], o[4 * k + 2][i], o[4 * k + 3][i]};
   __syncthreads();
-  float top = -INFINITY;
+  T* out = at<T>(a.out, row, kvh * a.group + g0, 0);
+  if (a.cuts && low == 0 && threadIdx.x == 0) a.cuts[row * in_row + kvg] = int2{first, parts};
+  for (int e = threadIdx.x; e < vectors * (D / 4); e += kThreads) {
+    const int v = e / (D / 4), d = e % (D / 4) * 4;
+    float top = -INFINITY, total = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, states[w][0][col]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, share[4];
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, states[w][0][v]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float decay = exp2_fast(states[w][0][col] - base);
-    total += states[w][1][col] * decay;
-    share[w] = states[w][2][col] * decay;
-  }
-  if (col >= vectors) return;
-  const float over = total == 0.0f ? 0.0f : 1.0f / total;
-  float y[DF];
-#pragma unroll
-  for (int f = 0; f < DF; ++f) {
-    float s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) s += merge[((w * 4 + wave) * DF + f) * 64 + lane] * share[w];
-    y[f] = s * over;
-  }
-  const int head = kvh * a.group + g0 + col, d = 4 * DF * quad + DF * wave;
-  if (parts > 1) {
-    const uint64_t part = ((uint64_t)row * a.q_heads + head) * a.splits + split;
-    float* to = a.part + part * D + d;
-#pragma unroll
-    for (int f = 0; f < DF; f += 4) *reinterpret_cast<floatx4*>(to + f) = floatx4{y[f], y[f + 1], y[f + 2], y[f + 3]};
-    if (quad == 0 && wave == 0) {
-      a.stats[2 * part] = top;
-      a.stats[2 * part + 1] = total;
+    for (int w = 0; w < 4; ++w) {
+      const float decay = exp2_fast(states[w][0][v] - base);
+      total += states[w][1][v] * decay;
+      y += reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[(d / DF % 4 * VW + d % DF / 4) * 64 + d / (4 * DF) * 16 + v] *
+           (states[w][2][v] * decay);
     }
-  } else {
-    T* to = at<T>(a.out, row, head, d);
-    if constexpr (DF >= 8) {
-#pragma unroll
-      for (int f = 0; f < DF; f += 8) store8(to + f, y + f);
+    y *= total == 0.0f ? 0.0f : 1.0f / total;
+    if (parts == 1) {
+      store4(out + v * a.out.head + d, y);
     } else {
-#pragma unroll
-      for (int f = 0; f < DF; ++f) to[f] = (T)y[f];
+      const uint64_t part = part_at(a, first, me - first, v);
+      *reinterpret_cast<floatx4*>(a.part + part * D + d) = y;
+      if (d == 0) *reinterpret_cast<float2*>(a.stats + 2 * part) = float2{top, total};
     }
+  }
   }
 }
 
-// Joins a row's parts, one workgroup for a query head: each part's output weighted with its
-// share of the softmax sum.
+__device__ inline int2 uniform_cut(const int2* p) {
+  return int2{uniform_load(&p->x), uniform_load(&p->y)};
+}
+
+// Joins the parts of the pairs that were cut, one wave for a query head: each part's output weighted
+// with its share of the softmax sum. A part's vector takes D / 4 lanes, so a wave reads up to four parts at
+// once, and eight times as many before it uses them: the kernel is a few memory round trips long.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
-  constexpr int L = D / 4, kSlots = kThreads / L;  // lanes of a part's vector; parts at a time
-  __shared__ float sums[kSlots][D];
-  __shared__ float totals[kSlots];
-  const int row = blockIdx.x / a.q_heads, head = blockIdx.x - row * a.q_heads;
-  const int length = min(uniform_load(a.lengths + row), a.limit);
-  if (length <= 0) return;
-  const int per = attend_part(length, a.splits, a.unit), parts = (length + per - 1) / per;
-  if (parts <= 1) return;
-  const uint64_t first = (uint64_t)blockIdx.x * a.splits;
-  const float* stats = a.stats + 2 * first;
-  float top = -INFINITY;
-  for (int s = threadIdx.x & 63; s < parts; s += 64) top = fmaxf(top, stats[2 * s]);
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const float base = top == -INFINITY ? 0.0f : top;
-  const int slot = threadIdx.x / L, d = threadIdx.x % L * 4;
-  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  float total = 0.0f;
-#pragma unroll 4
-  for (int s = slot; s < parts; s += kSlots) {
-    const float share = exp2_fast(stats[2 * s] - base) * stats[2 * s + 1];
-    total += share;
-    sum += *reinterpret_cast<const floatx4*>(a.part + (first + s) * D + d) * share;
-  }
-  *reinterpret_cast<floatx4*>(&sums[slot][d]) = sum;
-  if (d == 0) totals[slot] = total;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  float y = 0.0f, all = 0.0f;
+  constexpr int kLanes = D / 4, kSlots = 64 / kLanes, kDeep = 8;
+  const int vector = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (vector >= a.rows * a.q_heads) return;
+  const int row = vector / a.q_heads, head = vector - row * a.q_heads, kvh = head / a.group, g = head - kvh * a.group;
+  const int length = uniform_load(a.lengths + row);
+  const int2 cut = uniform_cut(a.cuts + (row * a.pages.kv_heads + kvh) * a.head_groups + g / 16);
+  const int first = cut.x, parts = cut.y;
+  if (min(length, a.limit) <= 0 || parts <= 1) return;  // a row without positions has no cut there
+  const int v = g % 16, slot = lane / kLanes, d = lane % kLanes * 4;
+  const auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.stats + 2 * part_at(a, first, min(i, parts - 1), v)); };
+  floatx4 y = {0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, total = 0.0f;
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    // Statistics and the first outputs of 64 parts are loaded together.
+    const int n = min(64, parts - i0);
+    const float2 own = stat(i0 + lane);
+    float most = lane < n ? own.x : -INFINITY;
+    for (int j0 = 0; j0 < n; j0 += kSlots * kDeep) {
+      floatx4 x[kDeep];
 #pragma unroll
-  for (int s = 0; s < kSlots; ++s) {
-    y += sums[s][threadIdx.x];
-    all += totals[s];
+      for (int j = 0; j < kDeep; ++j)
+        x[j] = *reinterpret_cast<const floatx4*>(a.part + part_at(a, first, i0 + min(j0 + j * kSlots + slot, n - 1), v) * D + d);
+      if (j0 == 0) {
+        for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+        most = fmaxf(most, top);
+        const float decay = top == -INFINITY ? 0.0f : exp2_fast(top - most);
+        total *= decay;
+        y *= decay;
+        top = most;
+      }
+      const float weight = lane < n && own.x != -INFINITY ? exp2_fast(own.x - top) * own.y : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        const int i = j0 + j * kSlots + slot;
+        const float w = __shfl(weight, min(i, 63), 64);
+        if (i < n) {
+          total += w;
+          y += x[j] * w;
+        }
+      }
+    }
   }
-  *at<T>(a.out, row, head, threadIdx.x) = (T)(all == 0.0f ? 0.0f : y / all);
+  for (int o = kLanes; o < 64; o <<= 1) {
+    total += __shfl_xor(total, o, 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], o, 64);
+  }
+  if (slot == 0) store4(at<T>(a.out, row, head, d), total == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : y / total);
 }
 
 template <typename T, int F>
@@ -627,9 +840,15 @@ void kv_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
 
 template <typename T, int F, int D>
 void attend(hipStream_t stream, const AttendArgs& a) {
-  const unsigned blocks = (unsigned)((uint64_t)a.rows * a.pages.kv_heads * a.head_groups * a.splits);
-  kv_attention_kernel<T, F, D><<<blocks, kThreads, 0, stream>>>(a);
-  if (a.splits > 1) kv_join_kernel<T, D><<<(unsigned)(a.rows * a.q_heads), kThreads, 0, stream>>>(a);
+  constexpr int kLds = Tile<D>::kBlock;
+  static const bool configured = [] {
+    HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&kv_attention_kernel<T, F, D>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    return true;
+  }();
+  (void)configured;
+  kv_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);
+  if (a.cuts) kv_join_kernel<T, D><<<(unsigned)(a.rows * a.q_heads + 3) / 4, kThreads, 0, stream>>>(a);
 }
 template <typename T, int F>
 void attend_dim(hipStream_t stream, int head_dim, const AttendArgs& a) {
@@ -734,7 +953,7 @@ Pages pages_of(const hllm_rocm_kv_pages* p) {
   if (!p->keys || !p->values || !p->key_scales || !p->value_scales) refuse("a cache's memory is null");
   if (((uintptr_t)p->keys | (uintptr_t)p->values | (uintptr_t)p->key_scales | (uintptr_t)p->value_scales) % 16)
     refuse("a cache's memory must be 16-byte aligned");
-  if (p->page_stride > (1ull << 40) || p->token_stride > (1ull << 40) || p->head_stride > (1ull << 40))
+  if (p->page_stride >= (1ull << 32) || p->token_stride > (1ull << 28) || p->head_stride > (1ull << 40))
     refuse("a cache's stride is too large");
   if ((p->pages > 1 && p->page_stride % 16) || p->token_stride % 16 || (p->kv_heads > 1 && p->head_stride % 16))
     refuse("a cache's strides must be multiples of 16 bytes");
@@ -746,7 +965,7 @@ Pages pages_of(const hllm_rocm_kv_pages* p) {
   int shift = 0;
   while ((1u << shift) < p->page_tokens) ++shift;
   return {static_cast<uint8_t*>(p->keys), static_cast<uint8_t*>(p->values), p->key_scales, p->value_scales,
-          p->pages > 1 ? p->page_stride : 0, p->token_stride, head, (int32_t)p->pages, shift, (int32_t)p->kv_heads};
+          p->pages > 1 ? (uint32_t)p->page_stride : 0u, (uint32_t)p->token_stride, head, (int32_t)p->pages, shift, (int32_t)p->kv_heads};
 }
 
 void check_rope(const hllm_rocm_rope* rope, uint64_t head_dim) {
@@ -828,8 +1047,9 @@ void plan_rope(const hllm_rocm_rope_config& c, hllm_rocm_rope& out) {
     last = std::min((long double)n - 1, std::ceil(pair(slow)));
     r.magnitude = (float)positive(c.magnitude, 0.1 * std::log(c.factor) + 1.0, "magnitude");
   }
+  const long double step = -2.0L * std::log((long double)c.theta) / n;
   for (uint32_t i = 0; i < n / 2; ++i) {
-    long double f = std::pow((long double)c.theta, -2.0L * i / n);
+    long double f = std::exp(step * i);
     if (c.scaling == HLLM_ROPE_LINEAR) f /= factor;
     if (c.scaling == HLLM_ROPE_LLAMA3) {
       const long double keep = std::clamp((length * f / turn - low) / (high - low), 0.0L, 1.0L);
@@ -957,12 +1177,11 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
 
 namespace {
 
-// The split of a call and the floats of its workspace.
+// How a call's work is cut and what its workspace holds: each pair's cut, then outputs and statistics of
+// two parts of each workgroup.
 struct AttendPlan {
-  uint64_t head_groups = 1;
-  AttendSplit split{1, 1};
-  uint64_t parts = 0;  // [rows][query_heads][splits], 0 when rows are not split
-  uint64_t bytes = 0;
+  uint64_t head_groups = 1, blocks = 0, cuts = 0, parts = 0, bytes = 0;
+  bool shared = false;
 };
 
 AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64_t query_heads, uint64_t limit) {
@@ -970,14 +1189,20 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
     refuse("query heads are a multiple of the cache's heads, at most 1024");
   AttendPlan p;
   if (rows == 0) return p;
-  p.head_groups = (query_heads / pages.kv_heads + 15) / 16;
-  const uint64_t pairs = rows * pages.kv_heads * p.head_groups;
-  p.split = attend_split(pairs, limit);
-  if (pairs * p.split.splits > kMostBlocks || rows * query_heads > kMostBlocks) refuse("too many rows for these heads and lengths");
-  if (p.split.splits > 1) {
-    p.parts = rows * query_heads * p.split.splits;
-    p.bytes = p.parts * (pages.head_dimension + 2) * sizeof(float);
+  const uint64_t group = query_heads / pages.kv_heads;
+  p.head_groups = (group + 15) / 16;
+  const uint64_t pairs = rows * pages.kv_heads * p.head_groups, cost = kPairCost + (limit + 127) / 128;
+  if (pairs > kMostBlocks) refuse("too many rows for these heads");
+  p.shared = limit > 128 * kWholeSteps && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
+
+  if (!p.shared) {
+    p.blocks = pairs;
+    return p;
   }
+  p.blocks = std::min<uint64_t>(attend_blocks((int)pages.head_dimension), pairs * cost);
+  p.cuts = (pairs + 1) / 2 * 2;  // whole sixteen bytes
+  p.parts = 2 * p.blocks * std::min<uint64_t>(group, 16);
+  p.bytes = p.cuts * sizeof(int2) + p.parts * (pages.head_dimension + 2) * sizeof(float);
   return p;
 }
 
@@ -1028,11 +1253,15 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     a.group = a.q_heads / a.pages.kv_heads;
     a.head_groups = (int32_t)plan.head_groups;
     a.limit = (int32_t)limit;
-    a.splits = plan.split.splits;
-    a.unit = plan.split.unit;
-    a.scale = args->scale;
-    a.part = static_cast<float*>(args->workspace);
-    a.stats = a.part + plan.parts * D;
+    a.blocks = (int32_t)plan.blocks;
+    a.shared = plan.shared;
+    a.scale_hi = (float)(args->scale * kLog2e);
+    a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);
+    if (plan.bytes > 0) {
+      a.cuts = static_cast<int2*>(args->workspace);
+      a.part = reinterpret_cast<float*>(a.cuts + plan.cuts);
+      a.stats = a.part + plan.parts * D;
+    }
     OnDevice on(device);
     launch_kv_attention(static_cast<hipStream_t>(stream), args->q.dtype, (int)pages->format, (int)D, a);
     HIP_CHECK(hipGetLastError());

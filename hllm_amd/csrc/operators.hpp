@@ -2,6 +2,7 @@
 // entry points; every launch goes to `stream` on the current device.
 #pragma once
 
+#include <cstdlib>
 #include "common.hpp"
 
 namespace hllm_rocm {
@@ -18,7 +19,8 @@ struct Pages {
   uint8_t* values;
   float* key_scales;
   float* value_scales;
-  uint64_t page_stride, token_stride, head_stride;  // bytes
+  uint32_t page_stride, token_stride;  // bytes
+  uint64_t head_stride;
   int32_t pages, page_shift, kv_heads;
 };
 
@@ -56,33 +58,25 @@ struct AttendArgs {
   int32_t rows, q_heads, group;  // group: query heads of one KV head
   int32_t head_groups;           // sixteens of a KV head's query heads
   int32_t limit;                 // positions of a row that count at most
-  int32_t splits, unit;          // attend_split
-  float scale;
-  float* part;                   // [rows][q_heads][splits][D]: splits' outputs, each normalised
-  float* stats;                  // [rows][q_heads][splits][2]: their score maximum (base 2) and sum
+  int32_t blocks;                // workgroups
+  int32_t shared;                // the rows' work is cut into the workgroups' shares (else a pair each)
+  float scale_hi, scale_lo;      // the scores' scale times log2 e as a sum of two floats
+  int2* cuts;                    // [pairs]: the first workgroup and the number of its parts (null: no pair is cut)
+  float* part;                   // [blocks][2][min(group, 16)][D]: parts' outputs, each normalised
+  float* stats;                  // [blocks][2][min(group, 16)][2]: their score maximum (base 2) and sum
 };
 void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
 
-// Positions that one workgroup holds page numbers for.
-constexpr int kAttendMostKeys = 8192;
-// How a call splits its rows: at most `splits` parts of a row, of at least `unit` positions.
-struct AttendSplit {
-  int splits, unit;
-};
-// `pairs`: rows x KV heads x sixteens of query heads.
-inline AttendSplit attend_split(uint64_t pairs, uint64_t limit) {
-  constexpr uint64_t kTarget = 2048, kUnit = 128;
-  const uint64_t wanted = (kTarget + pairs - 1) / pairs, most = (limit + kUnit - 1) / kUnit;
-  const uint64_t least = (limit + kAttendMostKeys - 1) / kAttendMostKeys;
-  uint64_t splits = wanted < most ? wanted : most;
-  if (splits < least) splits = least;
-  if (splits < 1) splits = 1;
-  return {(int)splits, (int)kUnit};
-}
-// Positions of each part of a row of `length`: a multiple of 32.
-__host__ __device__ inline int attend_part(int length, int splits, int unit) {
-  const int per = (int)(((int64_t)length + splits - 1) / splits);
-  return ((per > unit ? per : unit) + 31) & ~31;
+// Steps (of 128 positions) that starting a pair is counted as; rows of up to kWholeSteps are not cut.
+constexpr int kPairCost = 1, kWholeSteps = 4;
+// Rows whose lengths every workgroup sums to find its share: sixteen a lane.
+constexpr uint64_t kMostSharedRows = 1024;
+// Workgroups on a CU, of which there are 256: a wave has its tile in LDS and about a hundred registers
+// and D / 2.
+template <int D>
+constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
+inline uint64_t attend_blocks(int head_dim) {
+  return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : kAttendBlocks<256>);
 }
 
 }  // namespace hllm_rocm

@@ -147,12 +147,13 @@ def _numbers(x: torch.Tensor, name: str, device: torch.device, shape) -> int:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # torch.cuda.current_stream(device).cuda_stream without the object around it: 0.1 us, not 1.9.
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _output(out, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like)  # 1.6 us; torch.empty with a shape, dtype and device 3.6
     if not isinstance(out, torch.Tensor) or out.dtype != like.dtype:
         raise ValueError(f"{name} must have the input's dtype")
     return out
@@ -217,7 +218,7 @@ def kv_read(pages: KvPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     if (k_out is None) != (v_out is None):
         raise ValueError("k_out and v_out come together")
     if k_out is None:
-        k_out, v_out = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        k_out, v_out = pages.key_scales.new_empty((2, *shape), dtype=dtype)
     a, b = _rows(k_out, "k_out", device, shape), _rows(v_out, "v_out", device, shape)
     capi.check(capi.library().hllm_rocm_kv_read(device.index, _stream(device), C.byref(pages.c), at, shape[0],
                                                 C.byref(a), C.byref(b)))
@@ -250,7 +251,7 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
         raise ValueError("max_length is negative")
     if workspace is None:
         need = kv_attention_workspace(pages, shape[0], shape[1], min(max_length, page_table.shape[1] * pages.page_tokens))
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        workspace = pages.key_scales.new_empty(need, dtype=torch.uint8) if need else None
     elif workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous uint8 on {device}")
     args = capi.KvAttentionArgs(shape[0], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), n, max_length,

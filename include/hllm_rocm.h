@@ -428,7 +428,7 @@ hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_r
 typedef enum { HLLM_KV_E4M3 = 0, HLLM_KV_INT8 = 1 } hllm_kv_format;
 
 /* A paged cache in device memory: codes at page * page_stride + position * token_stride + head *
- * head_stride (bytes, multiples of 16; either of positions and heads inside the other; vectors
+ * head_stride (bytes, multiples of 16, token_stride at most 2^28; either of positions and heads inside the other; vectors
  * may not overlap) and scales [pages][kv_heads][page_tokens], for keys and values alike. A slot
  * is page * page_tokens + position in the page. All four pointers are 16-byte aligned. */
 typedef struct {

@@ -126,9 +126,9 @@ def fill(cache, kind, table, lengths, seed=1, spread=0.0):
             cache[name[:-1] + "_scales"].permute(0, 2, 1)[ids, at % page] = scale[here]
 
 
-def attended(q, cache, table, lengths, scale, max_length=1 << 31):
+def attended(q, cache, table, lengths, scale, max_length=1 << 31, exact_dots=False):
     """(outputs in 64 bits, the bound of the kernel's error, element by element); rows of negative
-    lengths are NaN.
+    lengths are NaN. `exact_dots`: q . k has no rounding (small whole numbers).
 
     A weight w_i = p_i s_i enters the products with half a step of F16 (2^-11; two F16 parts of
     F32 tensors: 2^-22) or, below F16's normal range, 2^-25 of the largest weight; p is off by what its
@@ -169,6 +169,8 @@ def attended(q, cache, table, lengths, scale, max_length=1 << 31):
         lost = (qd.abs().amax(-1, keepdim=True) * k.abs().sum(1)[:, None, :]) * abs(scale) * 2.0 ** -25
         rounding = 2.0 ** -22 if two else 2.0 ** -11
         e = lost + size * ((dim + 4) * 2.0 ** -24 + (2.0 ** -22 if two else 0.0))
+        if exact_dots:
+            e = torch.zeros_like(e)
         e = e + 4 * 2.0 ** -24 * (score - score.amax(-1, keepdim=True)).abs() + 4 * 2.0 ** -24 * score.abs().amax(-1, keepdim=True)
         e = e.amax(-1, keepdim=True) + 2.0 ** -22
         total = 2 * e + rounding + (len(at) / 32 + 64) * 2.0 ** -24

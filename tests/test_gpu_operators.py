@@ -257,7 +257,8 @@ def test_kv_attention_at_tile_edges(ops, kind, dtype, q_heads, heads, dim, page,
 
 @pytest.mark.parametrize("kind,dtype,dim", [("e4m3", torch.float16, 128), ("int8", torch.bfloat16, 256), ("e4m3", torch.float32, 64),
                                             ("int8", torch.float16, 64), ("e4m3", torch.bfloat16, 256), ("int8", torch.float32, 128)])
-@pytest.mark.parametrize("lengths", [[1], [100], [5000], [9000, 3, 0, 1025], [16411], [129] * 70, [2048, -1, 40] * 9])
+@pytest.mark.parametrize("lengths", [[1], [100], [5000], [9000, 3, 0, 1025], [16411], [129] * 70, [2048, -1, 40] * 9,
+                                     [600] * 3 + [0, -1] * 70 + [513, 1], [700, 20] * 280])
 def test_kv_attention_split_and_joined(ops, kind, dtype, dim, lengths):
     attend_case(ops, kind, dtype, lengths, 8, 2, dim, 16)
 
@@ -274,6 +275,30 @@ def test_kv_attention_of_peaked_scores_and_uneven_values(ops, dim, dtype):
 @pytest.mark.parametrize("dtype,q_scale", [(torch.bfloat16, 1e30), (torch.float32, 1e-30), (torch.float16, 1000.0), (torch.float32, 0.0)])
 def test_kv_attention_of_large_and_small_queries(ops, dtype, q_scale):
     attend_case(ops, "e4m3", dtype, [70, 400], 8, 2, 128, 64, q_scale=q_scale, scale=0.05 / max(q_scale, 1e-30))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_kv_attention_weights_to_their_last_bits(ops, dim, dtype):
+    """Whole numbers whose products are exact, so that only the weights' roundings are left: in F32
+    tensors a weight is right to 2^-22, in both of its parts."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    lengths, heads, page = [7, 40, 300, 1100], 2, 32
+    table, count = paged(lengths, page)
+    cache = forms.make_pages("int8", count, heads, page, dim)
+    cache["keys"].copy_(torch.randint(-3, 4, cache["keys"].shape, generator=g, device="cuda"))
+    cache["key_scales"].fill_(2.0 ** -4)
+    q = torch.randint(-2, 3, (4, 16, dim), generator=g, device="cuda").to(dtype)
+    out = ops.kv_attention(q, ops.KvPages(**cache), table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 1100)
+    expect, off = forms.attended(q, cache, table, lengths, dim ** -0.5, exact_dots=True)
+    near(out, expect, off)
+
+
+def test_kv_attention_of_more_rows_than_share_work(ops):
+    """Past 1024 rows each pair has a workgroup of its own."""
+    lengths = ([3, 0, 70, -1, 600] * 220)[:1090]
+    attend_case(ops, "e4m3", torch.float16, lengths, 4, 1, 64, 16)
 
 
 def test_kv_attention_leaves_out_dropped_pages(ops):
