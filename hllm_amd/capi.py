@@ -190,15 +190,14 @@ def library() -> C.CDLL:
     L.hllm_rocm_device_allocator_metrics.argtypes = [C.c_int32, C.POINTER(AllocatorMetrics)]
     L.hllm_rocm_device_reset_peak.argtypes = [C.c_int32]
     L.hllm_rocm_device_query.argtypes = [C.c_int32, C.POINTER(DeviceInfo)]
-    tensor, i32 = C.POINTER(Tensor), C.c_int32
-    L.hllm_rocm_rope_plan.argtypes = [C.POINTER(RopeConfig), C.POINTER(RopePlan)]
-    L.hllm_rocm_rope_apply.argtypes = [i32, vp, C.POINTER(RopePlan), vp, u64, u32, tensor, tensor,
-                                       tensor, tensor]
-    L.hllm_rocm_kv_append.argtypes = [i32, vp, C.POINTER(KvPages), vp, u64, tensor, tensor,
-                                      C.POINTER(RopePlan), vp, tensor, tensor]
-    L.hllm_rocm_kv_read.argtypes = [i32, vp, C.POINTER(KvPages), vp, u64, tensor, tensor]
-    L.hllm_rocm_kv_attention.argtypes = [i32, vp, C.POINTER(KvPages), C.POINTER(KvAttentionArgs)]
-    L.hllm_rocm_kv_attention_workspace.argtypes = [C.POINTER(KvPages), u64, u32, u64, C.POINTER(u64)]
+    # The operators' structures are taken by address: of a ctypes structure or of bytes laid out like it.
+    i32 = C.c_int32
+    L.hllm_rocm_rope_plan.argtypes = [vp, vp]
+    L.hllm_rocm_rope_apply.argtypes = [i32, vp, vp, vp, u64, u32, vp, vp, vp, vp]
+    L.hllm_rocm_kv_append.argtypes = [i32, vp, vp, vp, u64, vp, vp, vp, vp, vp, vp]
+    L.hllm_rocm_kv_read.argtypes = [i32, vp, vp, vp, u64, vp, vp]
+    L.hllm_rocm_kv_attention.argtypes = [i32, vp, vp, vp]
+    L.hllm_rocm_kv_attention_workspace.argtypes = [vp, u64, u32, u64, vp]
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is C.c_int or (fn.restype is None and name != "hllm_rocm_stage_destroy"):

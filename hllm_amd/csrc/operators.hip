@@ -133,7 +133,8 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
 // for all heads of the block, and no table is read. In half layout with a rotary
 // dimension of whole sixteens a thread holds both elements of its pairs (eight of either half);
 // interleaved pairs lie beside each other; other half layouts exchange through LDS (kExchange). So
-// every pair is read before it is written and a tensor can be rotated in place.
+// every pair is read before it is written and a tensor can be rotated in place. Bound by memory:
+// 4.1 to 4.5 TB/s of 16-bit rows and 5.5 of F32 rows at 42 and 84 MB (a copy reaches 4.8).
 //
 // F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
 // share its largest value by shuffles.
@@ -153,8 +154,12 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   const bool active = in_block < a.heads_per_block && head < a.q_heads + a.k_heads + a.v_heads;
   const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + a.k_heads;
   const int h = is_q ? head : is_v ? head - a.q_heads - a.k_heads : head - a.q_heads;
-  const bool paired = !kExchange && !a.interleaved && !is_v && 16 * u < R;
-  const int d0 = paired ? 8 * u : 16 * u, d1 = paired ? half + 8 * u : 16 * u + 8;
+  // The lane's two eights: of the pairs' halves, or of the halves of the elements that are not paired over
+  // halves (from `rest` on), so that a head's lanes read whole lines.
+  const bool over_halves = !kExchange && !a.interleaved && !is_v, paired = over_halves && 16 * u < R;
+  const int rest = over_halves ? R : 0, before = rest / 16;
+  const int d0 = kExchange ? 16 * u : paired ? 8 * u : rest + 8 * (u - before);
+  const int d1 = kExchange ? d0 + 8 : paired ? half + 8 * u : d0 + (16 * a.lanes - rest) / 2;
   float x[16];
   if (active) {
     const Strided& in = is_q ? a.q : is_v ? a.v : a.k;
@@ -194,8 +199,9 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
     } else if (a.interleaved) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (16 * u + 2 * i >= R) continue;
-        const float2 v = cs[8 * u + i];
+        const int d = i < 4 ? d0 + 2 * i : d1 + 2 * (i - 4);
+        if (d >= R) continue;
+        const float2 v = cs[d / 2];
         const float x0 = x[2 * i], x1 = x[2 * i + 1];
         x[2 * i] = x0 * v.x - x1 * v.y;
         x[2 * i + 1] = x1 * v.x + x0 * v.y;
@@ -236,36 +242,45 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
 
 // ---------------------------------------------------------------- reading back
 
-// A thread reads sixteen codes of a key and of the value beside it and writes them: nothing
-// but memory traffic.
+// A thread reads the codes of sixteen bytes of output of a key, and of the value beside it, and writes
+// them: a wave's accesses are whole lines (sixteen codes a thread, so F32 stores of 64 bytes a
+// lane: 3.5 TB/s). Nothing but memory traffic.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
-  constexpr int L = D / 16;
+  constexpr int kCodes = 16 / sizeof(T), L = D / kCodes;
   const Pages& c = a.pages;
   const uint32_t per_row = (uint32_t)c.kv_heads * L;
   const uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
   const uint64_t row = unit / per_row;
   if (row >= (uint64_t)a.rows) return;
-  const int in_row = (int)(unit - row * per_row), h = in_row / L, d = in_row % L * 16;
+  const int in_row = (int)(unit - row * per_row), h = in_row / L, d = in_row % L * kCodes;
   const int slot = a.slots[row];
   if (slot < 0 || (slot >> c.page_shift) >= c.pages) return;
   const int page = slot >> c.page_shift, offset = slot & ((1 << c.page_shift) - 1);
   const uint64_t from = (uint64_t)page * c.page_stride + (uint64_t)offset * c.token_stride + (uint64_t)h * c.head_stride + d;
   const uint64_t scale_at = (((uint64_t)page * c.kv_heads + h) << c.page_shift) + offset;
-  const uint4v codes[2] = {*reinterpret_cast<const uint4v*>(c.keys + from), *reinterpret_cast<const uint4v*>(c.values + from)};
+  uint32_t codes[2][kCodes / 4];
+#pragma unroll
+  for (int j = 0; j < kCodes / 4; ++j) {
+    codes[0][j] = reinterpret_cast<const uint32_t*>(c.keys + from)[j];
+    codes[1][j] = reinterpret_cast<const uint32_t*>(c.values + from)[j];
+  }
   const float scale[2] = {c.key_scales[scale_at], c.value_scales[scale_at]};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float x[16];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const floatx4 v = decode4<F>(codes[which][j]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i] * scale[which];
-    }
     T* to = at<T>(which ? a.v : a.k, (int)row, h, d);
-    store8(to, x);
-    store8(to + 8, x + 8);
+    if constexpr (kCodes == 8) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const floatx4 v = decode4<F>(codes[which][j]) * scale[which];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i];
+      }
+      store8(to, x);
+    } else {
+      store4(to, decode4<F>(codes[which][0]) * scale[which]);
+    }
   }
 }
 
@@ -831,7 +846,7 @@ void rotate_to(hipStream_t stream, int format, int rows, const RotateArgs& a) {
 
 template <typename T, int F>
 void kv_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
-  const uint64_t units = (uint64_t)a.rows * a.pages.kv_heads * (head_dim / 16);
+  const uint64_t units = (uint64_t)a.rows * a.pages.kv_heads * (head_dim * sizeof(T) / 16);
   const unsigned blocks = (unsigned)((units + kThreads - 1) / kThreads);
   if (head_dim == 64) kv_read_kernel<T, F, 64><<<blocks, kThreads, 0, stream>>>(a);
   if (head_dim == 128) kv_read_kernel<T, F, 128><<<blocks, kThreads, 0, stream>>>(a);
@@ -1166,7 +1181,7 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
     a.v = tensor(v_out, "v_out", rows, pages->head_dimension, true);
     if (k_out->heads != pages->kv_heads || v_out->heads != pages->kv_heads) refuse("k_out and v_out must have the cache's heads");
     if (k_out->dtype != v_out->dtype) refuse("k_out and v_out must have one dtype");
-    if (rows * pages->kv_heads * (pages->head_dimension / 16) > kMostBlocks * kThreads) refuse("too many rows for these heads");
+    if (rows * pages->kv_heads * (pages->head_dimension / 4) > kMostBlocks * kThreads) refuse("too many rows for these heads");
     OnDevice on(device);
     launch_kv_read(static_cast<hipStream_t>(stream), k_out->dtype, (int)pages->format, (int)pages->head_dimension, a);
     HIP_CHECK(hipGetLastError());

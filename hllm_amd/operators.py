@@ -17,6 +17,7 @@ looked at on the host. Wrong tensors raise ValueError, what the library refuses 
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -25,6 +26,9 @@ from . import capi
 _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _FORMATS = {torch.float8_e4m3fn: capi.KV_E4M3, torch.int8: capi.KV_INT8}
 _CODES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+# capi.Tensor and capi.KvAttentionArgs as bytes: a quarter of the time of filling a ctypes structure.
+TENSOR = struct.Struct("@PIIQQ")
+ATTENTION_ARGS = struct.Struct("@QPQQPQf4xPIIQQPIIQQPQ")
 _SCALINGS = {
     "linear": (capi.ROPE_LINEAR, ("factor",), ()),
     "llama3": (capi.ROPE_LLAMA3, ("factor", "original_max_position_embeddings", "low_freq_factor",
@@ -66,7 +70,8 @@ class Rope:
             raise ValueError(f"rope_type 'default' takes no parameters: {sorted(given)}")
         self.rotary_dim = rotary_dim
         self.plan = capi.RopePlan()
-        capi.check(capi.library().hllm_rocm_rope_plan(C.byref(c), C.byref(self.plan)))
+        self.address = C.addressof(self.plan)
+        capi.check(capi.library().hllm_rocm_rope_plan(C.byref(c), self.address))
 
 
 class KvPages:
@@ -99,9 +104,8 @@ class KvPages:
         self.c = capi.KvPages(_FORMATS[keys.dtype], self.pages, self.page_tokens, self.kv_heads, self.head_dim,
                               keys.stride(0), keys.stride(2), keys.stride(1), keys.data_ptr(), values.data_ptr(),
                               key_scales.data_ptr(), value_scales.data_ptr())
-        # The library looks the description over here too, so that a wrong one shows at once.
-        need = C.c_uint64()
-        capi.check(capi.library().hllm_rocm_kv_attention_workspace(C.byref(self.c), 0, self.kv_heads, 0, C.byref(need)))
+        self.address = C.addressof(self.c)
+        kv_attention_workspace(self, 0, self.kv_heads, 0)  # the library refuses a wrong description here
 
     @classmethod
     def empty(cls, format: str, pages: int, kv_heads: int, page_tokens: int, head_dim: int, device="cuda"):
@@ -123,26 +127,32 @@ def _on_device(x: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be a tensor in device memory")
 
 
-def _rows(x: torch.Tensor, name: str, device: torch.device, shape=None) -> capi.Tensor:
-    """The C description of a tensor [rows, heads, head_dim]."""
+def _fields(x: torch.Tensor, name: str, device: torch.device, rows: int, dim: int, heads: int | None = None):
+    """A tensor [rows, heads, dim] as the fields of capi.Tensor."""
     if not isinstance(x, torch.Tensor) or x.device != device:
         raise ValueError(f"{name} must be a tensor on {device}")
-    if x.dtype not in _DTYPES or x.dim() != 3:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or x.dim() != 3:
         raise ValueError(f"{name} must be [rows, heads, head_dim] of float32, float16 or bfloat16")
-    if shape is not None and x.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}: it is {list(x.shape)}")
-    s = x.stride()
-    if s[2] != 1:
+    n, own, width = x.shape
+    if n != rows or width != dim or (heads is not None and own != heads):
+        raise ValueError(f"{name} must be [{rows}, {'heads' if heads is None else heads}, {dim}]: it is {list(x.shape)}")
+    row, head, last = x.stride()
+    if last != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return capi.Tensor(x.data_ptr(), _DTYPES[x.dtype], x.shape[1], s[0], s[1])
+    return x.data_ptr(), dtype, own, row, head
 
 
-def _numbers(x: torch.Tensor, name: str, device: torch.device, shape) -> int:
-    """The address of contiguous int32 numbers."""
+def _rows(x: torch.Tensor, name: str, device: torch.device, rows: int, dim: int, heads: int | None = None) -> bytes:
+    return TENSOR.pack(*_fields(x, name, device, rows, dim, heads))
+
+
+def _numbers(x: torch.Tensor, name: str, device: torch.device, rows: int) -> int:
+    """The address of `rows` contiguous int32 numbers."""
     if not isinstance(x, torch.Tensor) or x.device != device or x.dtype != torch.int32:
         raise ValueError(f"{name} must be int32 on {device}")
-    if x.shape != shape or not x.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {list(shape)}")
+    if x.dim() != 1 or x.shape[0] != rows or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous [{rows}]")
     return x.data_ptr()
 
 
@@ -164,20 +174,22 @@ def rope(plan: Rope, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor |
     """q and k [rows, heads, head_dim] rotated at ``positions`` [rows] (int32): (q_out, k_out), or
     q_out alone without k. An output may be its input."""
     _on_device(q, "q")
-    device, shape = q.device, q.shape
-    a = _rows(q, "q", device)
+    if q.dim() != 3:
+        raise ValueError("q must be [rows, heads, head_dim]")
+    device = q.device
+    rows, heads, dim = q.shape
+    a = _rows(q, "q", device, rows, dim)
     q_out = _output(q_out, q, "q_out")
-    b = _rows(q_out, "q_out", device, shape)
-    at = _numbers(positions, "positions", device, shape[:1])
+    b = _rows(q_out, "q_out", device, rows, dim, heads)
+    at = _numbers(positions, "positions", device, rows)
     c = d = None
     if k is not None:
-        c = C.byref(_rows(k, "k", device, (shape[0], *k.shape[1:2], shape[2])))
+        c = _rows(k, "k", device, rows, dim)
         k_out = _output(k_out, k, "k_out")
-        d = C.byref(_rows(k_out, "k_out", device, k.shape))
+        d = _rows(k_out, "k_out", device, rows, dim, k.shape[1])
     elif k_out is not None:
         raise ValueError("k_out without k")
-    capi.check(capi.library().hllm_rocm_rope_apply(device.index, _stream(device), C.byref(plan.plan), at, shape[0],
-                                                   shape[2], C.byref(a), C.byref(b), c, d))
+    capi.check(capi.library().hllm_rocm_rope_apply(device.index, _stream(device), plan.address, at, rows, dim, a, b, c, d))
     return q_out if k is None else (q_out, k_out)
 
 
@@ -187,21 +199,22 @@ def kv_append(pages: KvPages, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
     """Quantises k and v [rows, kv_heads, head_dim] into the cache at ``slots`` [rows] (int32, -1: a
     padding row). With ``rope``, k is rotated at ``positions`` [rows] first, and q as by
     ``rope``: returns q_out then, else None. Rows of a call name different slots."""
-    device, shape = pages.device, k.shape
-    a = _rows(k, "k", device, (*shape[:1], pages.kv_heads, pages.head_dim))
-    b = _rows(v, "v", device, shape)
-    to = _numbers(slots, "slots", device, shape[:1])
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("k must be [rows, kv_heads, head_dim]")
+    device, rows, dim = pages.device, k.shape[0], pages.head_dim
+    a = _rows(k, "k", device, rows, dim, pages.kv_heads)
+    b = _rows(v, "v", device, rows, dim, pages.kv_heads)
+    to = _numbers(slots, "slots", device, rows)
     plan = at = c = d = None
     if rope is not None:
-        plan, at = C.byref(rope.plan), _numbers(positions, "positions", device, shape[:1])
+        plan, at = rope.address, _numbers(positions, "positions", device, rows)
     if q is not None:
-        c = C.byref(_rows(q, "q", device, (shape[0], *q.shape[1:2], pages.head_dim)))
+        c = _rows(q, "q", device, rows, dim)
         q_out = _output(q_out, q, "q_out")
-        d = C.byref(_rows(q_out, "q_out", device, q.shape))
+        d = _rows(q_out, "q_out", device, rows, dim, q.shape[1])
     elif q_out is not None:
         raise ValueError("q_out without q")
-    capi.check(capi.library().hllm_rocm_kv_append(device.index, _stream(device), C.byref(pages.c), to, shape[0],
-                                                  C.byref(a), C.byref(b), plan, at, c, d))
+    capi.check(capi.library().hllm_rocm_kv_append(device.index, _stream(device), pages.address, to, rows, a, b, plan, at, c, d))
     return q_out
 
 
@@ -213,15 +226,14 @@ def kv_read(pages: KvPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     device = pages.device
     if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
         raise ValueError("slots must be int32 [rows]")
-    shape = (slots.shape[0], pages.kv_heads, pages.head_dim)
-    at = _numbers(slots, "slots", device, shape[:1])
+    rows, heads, dim = slots.shape[0], pages.kv_heads, pages.head_dim
+    at = _numbers(slots, "slots", device, rows)
     if (k_out is None) != (v_out is None):
         raise ValueError("k_out and v_out come together")
     if k_out is None:
-        k_out, v_out = pages.key_scales.new_empty((2, *shape), dtype=dtype)
-    a, b = _rows(k_out, "k_out", device, shape), _rows(v_out, "v_out", device, shape)
-    capi.check(capi.library().hllm_rocm_kv_read(device.index, _stream(device), C.byref(pages.c), at, shape[0],
-                                                C.byref(a), C.byref(b)))
+        k_out, v_out = pages.key_scales.new_empty((2, rows, heads, dim), dtype=dtype)
+    a, b = _rows(k_out, "k_out", device, rows, dim, heads), _rows(v_out, "v_out", device, rows, dim, heads)
+    capi.check(capi.library().hllm_rocm_kv_read(device.index, _stream(device), pages.address, at, rows, a, b))
     return k_out, v_out
 
 
@@ -237,33 +249,36 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
     device = pages.device
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [rows, heads, head_dim]")
-    shape = q.shape
-    a = _rows(q, "q", device, (*shape[:2], pages.head_dim))
+    rows, heads, dim = q.shape
+    a = _fields(q, "q", device, rows, pages.head_dim)
     out = _output(out, q, "out")
-    b = _rows(out, "out", device, shape)
-    n = _numbers(lengths, "lengths", device, shape[:1])
+    b = _fields(out, "out", device, rows, dim, heads)
+    n = _numbers(lengths, "lengths", device, rows)
     if not isinstance(page_table, torch.Tensor) or page_table.device != device or page_table.dtype != torch.int32 \
-            or page_table.dim() != 2 or page_table.shape[0] != shape[0]:
+            or page_table.dim() != 2 or page_table.shape[0] != rows:
         raise ValueError(f"page_table must be int32 [rows, width] on {device}")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    width = page_table.shape[1]
+    stride, last = page_table.stride()
+    if width > 1 and last != 1:
         raise ValueError("a row of page_table must be contiguous")
     if max_length < 0:
         raise ValueError("max_length is negative")
+    max_length = min(max_length, width * pages.page_tokens)
     if workspace is None:
-        need = kv_attention_workspace(pages, shape[0], shape[1], min(max_length, page_table.shape[1] * pages.page_tokens))
-        workspace = pages.key_scales.new_empty(need, dtype=torch.uint8) if need else None
+        need = kv_attention_workspace(pages, rows, heads, max_length)
+        if need:
+            workspace = pages.key_scales.new_empty(need, dtype=torch.uint8)
     elif workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous uint8 on {device}")
-    args = capi.KvAttentionArgs(shape[0], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), n, max_length,
-                                pages.head_dim ** -0.5 if scale is None else scale, a, b,
-                                None if workspace is None else workspace.data_ptr(),
-                                0 if workspace is None else workspace.numel())
-    capi.check(capi.library().hllm_rocm_kv_attention(device.index, _stream(device), C.byref(pages.c), C.byref(args)))
+    at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    args = ATTENTION_ARGS.pack(rows, page_table.data_ptr(), width, stride, n, max_length,
+                               pages.head_dim ** -0.5 if scale is None else scale, *a, *b, at, size)
+    capi.check(capi.library().hllm_rocm_kv_attention(device.index, _stream(device), pages.address, args))
     return out
 
 
 def kv_attention_workspace(pages: KvPages, rows: int, q_heads: int, max_length: int) -> int:
     """Bytes of workspace that ``kv_attention`` needs for these sizes (0: none)."""
     need = C.c_uint64()
-    capi.check(capi.library().hllm_rocm_kv_attention_workspace(C.byref(pages.c), rows, q_heads, max_length, C.byref(need)))
+    capi.check(capi.library().hllm_rocm_kv_attention_workspace(pages.address, rows, q_heads, max_length, C.byref(need)))
     return need.value

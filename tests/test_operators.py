@@ -280,3 +280,17 @@ def test_layouts_match_the_header(struct, cname):
         subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c_file, "-o", exe], check=True)
         got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [getattr(struct, f).offset for f in fields] + [C.sizeof(struct)]
+
+
+def test_packed_bytes_have_the_structures_layouts():
+    from hllm_amd import operators
+
+    def values(struct):
+        return [v for f, _ in struct._fields_ for v in (values(getattr(struct, f)) if isinstance(getattr(struct, f), C.Structure)
+                                                        else [getattr(struct, f) or 0])]
+
+    t = capi.Tensor(ADDRESS, 2, 7, 1 << 33, 1 << 34)
+    assert operators.TENSOR.pack(*values(t)) == bytes(t)
+    a = capi.KvAttentionArgs(3, ADDRESS, 5, 1 << 35, 2 * ADDRESS, 1 << 36, 0.5, t, capi.Tensor(ADDRESS + 16, 1, 9, 8, 4), 0, 1 << 37)
+    assert operators.ATTENTION_ARGS.pack(*values(a)) == bytes(a)
+    assert operators.ATTENTION_ARGS.size == C.sizeof(capi.KvAttentionArgs)
