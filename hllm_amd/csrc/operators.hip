@@ -1206,15 +1206,21 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   if (rows == 0) return p;
   const uint64_t group = query_heads / pages.kv_heads;
   p.head_groups = (group + 15) / 16;
-  const uint64_t pairs = rows * pages.kv_heads * p.head_groups, cost = kPairCost + (limit + 127) / 128;
+  const uint64_t pairs = rows * pages.kv_heads * p.head_groups, steps = (limit + 127) / 128, cost = kPairCost + steps;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
-  p.shared = limit > 128 * kWholeSteps && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
-
+  // A workgroup for each pair where rows are short or pairs many: no row has more steps than 8 and 8 for each
+  // pair a workgroup of the card. Shares cost 3 to 5 us more (each workgroup sums all rows' steps; the join), and
+  // spare waiting for the longest row. Head dimension 128, 8 KV heads, us with a pair each / with shares:
+  // 64 rows to 1000 positions 16.8 / 21.6, to 2048 23.0 / 21.9; 16 rows to 2048 18.9 / 13.8; 256 rows
+  // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61.
+  const uint64_t fit = attend_blocks((int)pages.head_dimension);
+  const bool whole = steps * fit <= 8 * (fit + pairs);
+  p.shared = !whole && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
   if (!p.shared) {
     p.blocks = pairs;
     return p;
   }
-  p.blocks = std::min<uint64_t>(attend_blocks((int)pages.head_dimension), pairs * cost);
+  p.blocks = std::min<uint64_t>(fit, pairs * cost);
   p.cuts = (pairs + 1) / 2 * 2;  // whole sixteen bytes
   p.parts = 2 * p.blocks * std::min<uint64_t>(group, 16);
   p.bytes = p.cuts * sizeof(int2) + p.parts * (pages.head_dimension + 2) * sizeof(float);

@@ -216,7 +216,7 @@ def test_kv_attention_refuses():
     lib = capi.library()
 
     def call(device=0, pages=cache(), **changes):
-        a = capi.KvAttentionArgs(4, ADDRESS, 10, 10, ADDRESS, 600, 0.1, tensor(heads=32), tensor(heads=32, data=2 * ADDRESS),
+        a = capi.KvAttentionArgs(4, ADDRESS, 100, 100, ADDRESS, 6000, 0.1, tensor(heads=32), tensor(heads=32, data=2 * ADDRESS),
                                  ADDRESS, 1 << 30)
         for name, value in changes.items():
             setattr(a, name, value)
