@@ -318,18 +318,29 @@ __device__ inline void halves4(uint32_t w, half2v& lo, half2v& hi) {
   }
 }
 
-// Copies into LDS as lds_copy16, with an address a lane; and of one word a lane.
-__device__ inline void lds_copy16_at(const void* from, uint32_t lds_byte_offset) {
+// Copies into LDS as lds_copy16, of cache lines that are not kept: a step reads a layer's cache once
+// (5.4 -> 6.1 TB/s at 3 x 200000 positions, the read probe 6.3; caches that would fit the 256 MB
+// last level and are read again at once lose: 64 rows of 200 to 1000 positions 16.5 -> 18.0 us).
+__device__ inline void lds_stream16(const void* sbase, uint32_t voffset, uint32_t lds_byte_offset) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds_byte_offset)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voffset), "s"(sbase),
+               "s"(lds_byte_offset)
                : "memory", "m0");
 #pragma clang diagnostic pop
 }
-__device__ inline void lds_copy4_at(const void* from, uint32_t lds_byte_offset) {
+// ... with an address a lane; and of one word a lane.
+__device__ inline void lds_stream16_at(const void* from, uint32_t lds_byte_offset) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds_byte_offset)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(lds_byte_offset)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+__device__ inline void lds_stream4_at(const void* from, uint32_t lds_byte_offset) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off nt" ::"v"(from), "s"(lds_byte_offset)
                : "memory", "m0");
 #pragma clang diagnostic pop
 }
@@ -498,18 +509,18 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       pages[g] = there ? ids[g] : 0;
       const uint64_t page_at = (uint64_t)(uint32_t)pages[g] * c.page_stride + (uint64_t)(uint32_t)((t + 8 * g) & mask) * token;
       if constexpr (D == 64) {
-        lds_copy16_at(lane_from[g & 1] + page_at, tile_at + g * 1024);
+        lds_stream16_at(lane_from[g & 1] + page_at, tile_at + g * 1024);
       } else {
 #pragma unroll
         for (int i = 0; i < D / 128; ++i) {
-          lds_copy16(keys + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + (g * (D / 128) + i) * 1024);
-          lds_copy16(values + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + 32 * D + (g * (D / 128) + i) * 1024);
+          lds_stream16(keys + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + (g * (D / 128) + i) * 1024);
+          lds_stream16(values + page_at + (uint64_t)(4 * i) * token, lane_at[g & 1], tile_at + 32 * D + (g * (D / 128) + i) * 1024);
         }
       }
     }
     const int group = (lane & 31) >> 3;
     const int page = group & 2 ? (group & 1 ? pages[3] : pages[2]) : (group & 1 ? pages[1] : pages[0]);
-    lds_copy4_at(lane_scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + (lane & 31)) & mask)), tile_at + Layout::kScales);
+    lds_stream4_at(lane_scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + (lane & 31)) & mask)), tile_at + Layout::kScales);
     return missing;
   };
 
@@ -1208,13 +1219,13 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   p.head_groups = (group + 15) / 16;
   const uint64_t pairs = rows * pages.kv_heads * p.head_groups, steps = (limit + 127) / 128, cost = kPairCost + steps;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
-  // A workgroup for each pair where rows are short or pairs many: no row has more steps than 8 and 8 for each
+  // A workgroup for each pair where rows are short or pairs many: no row has more steps than 5 and 9 for each
   // pair a workgroup of the card. Shares cost 3 to 5 us more (each workgroup sums all rows' steps; the join), and
   // spare waiting for the longest row. Head dimension 128, 8 KV heads, us with a pair each / with shares:
   // 64 rows to 1000 positions 16.8 / 21.6, to 2048 23.0 / 21.9; 16 rows to 2048 18.9 / 13.8; 256 rows
-  // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61.
+  // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61. 7 F32 rows to 903, head dimension 64: 12.3 / 10.5.
   const uint64_t fit = attend_blocks((int)pages.head_dimension);
-  const bool whole = steps * fit <= 8 * (fit + pairs);
+  const bool whole = steps * fit <= 5 * fit + 9 * pairs;
   p.shared = !whole && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
   if (!p.shared) {
     p.blocks = pairs;
