@@ -3,6 +3,7 @@
 #include "operators.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -547,9 +548,10 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
     }
     most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
-    // 2^e <= largest < 2^(e+1), for e from -126 to 126; other vectors (zero, not finite) as they are.
-    const uint32_t exponent = most >> 23;
-    const bool usual = exponent >= 1 && exponent <= 253;
+    // 2^e <= largest < 2^(e+1), e at most 126 (the largest numbers are left below 4); vectors that are
+    // zero, below the normal range or not finite as they are.
+    const uint32_t exponent = min(most >> 23, 253u);
+    const bool usual = exponent >= 1 && most < 0x7f800000u;
     const float down = usual ? __uint_as_float((254u - exponent) << 23) : 1.0f;
     const float up = usual ? __uint_as_float(exponent << 23) : 1.0f;
     factor = a.scale_hi * up;
@@ -867,12 +869,15 @@ void kv_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
 template <typename T, int F, int D>
 void attend(hipStream_t stream, const AttendArgs& a) {
   constexpr int kLds = Tile<D>::kBlock;
-  static const bool configured = [] {
+  // More than 64 KiB of LDS is asked for once on each device.
+  static std::atomic<uint64_t> asked{0};
+  int device = 0;
+  HIP_CHECK(hipGetDevice(&device));
+  if (!(asked.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
     HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&kv_attention_kernel<T, F, D>),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-    return true;
-  }();
-  (void)configured;
+    asked.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+  }
   kv_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);
   if (a.cuts) kv_join_kernel<T, D><<<(unsigned)(a.rows * a.q_heads + 3) / 4, kThreads, 0, stream>>>(a);
 }
@@ -1224,7 +1229,7 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   // spare waiting for the longest row. Head dimension 128, 8 KV heads, us with a pair each / with shares:
   // 64 rows to 1000 positions 16.8 / 21.6, to 2048 23.0 / 21.9; 16 rows to 2048 18.9 / 13.8; 256 rows
   // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61. 7 F32 rows to 903, head dimension 64: 12.3 / 10.5.
-  const uint64_t fit = attend_blocks((int)pages.head_dimension);
+  const uint64_t fit = attend_blocks((int)pages.head_dimension, false);
   const bool whole = steps * fit <= 5 * fit + 9 * pairs;
   p.shared = !whole && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
   if (!p.shared) {
@@ -1238,7 +1243,10 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   return p;
 }
 
-uint64_t clamp_length(uint64_t max_length) { return std::min<uint64_t>(max_length, 0x7fffffffull); }
+// Positions of one row: sums of a length and a tile's stay below 2^31.
+constexpr uint64_t kMostPositions = 1u << 30;
+
+uint64_t clamp_length(uint64_t max_length) { return std::min(max_length, kMostPositions); }
 
 }  // namespace
 
@@ -1270,7 +1278,7 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     if (args->q.data == args->out.data) refuse("out must not be q");
     if (!std::isfinite(args->scale)) refuse("scale is not finite");
     if (!args->lengths) refuse("lengths is null");
-    if (args->table_width > 0x7fffffffull / pages->page_tokens) refuse("a page table's row holds at most 2^31 - 1 positions");
+    if (args->table_width > kMostPositions / pages->page_tokens) refuse("a page table's row holds at most 2^30 positions");
     const uint64_t limit = std::min(clamp_length(args->max_length), args->table_width * pages->page_tokens);
     if (limit > 0 && !args->page_table) refuse("page_table is null");
     if (args->table_stride > (1ull << 40)) refuse("table_stride is too large");
@@ -1285,7 +1293,9 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     a.group = a.q_heads / a.pages.kv_heads;
     a.head_groups = (int32_t)plan.head_groups;
     a.limit = (int32_t)limit;
-    a.blocks = (int32_t)plan.blocks;
+    // F32 queries take twice the LDS.
+    const bool f32 = args->q.dtype == HLLM_DTYPE_F32;
+    a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks((int)D, f32)) : plan.blocks);
     a.shared = plan.shared;
     a.scale_hi = (float)(args->scale * kLog2e);
     a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);

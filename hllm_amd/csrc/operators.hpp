@@ -72,12 +72,12 @@ void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int hea
 constexpr int kPairCost = 1;
 // Rows whose lengths every workgroup sums to find its share: sixteen a lane.
 constexpr uint64_t kMostSharedRows = 1024;
-// Workgroups on a CU, of which there are 256: a wave has its tile in LDS and about a hundred registers
-// and D / 2.
+// Workgroups that the card's 256 CUs hold at once, by LDS (a wave's tile) and registers (about a hundred and
+// D / 2); F32 queries of 256 elements leave room for one on a CU.
 template <int D>
 constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
-inline uint64_t attend_blocks(int head_dim) {
-  return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : kAttendBlocks<256>);
+inline uint64_t attend_blocks(int head_dim, bool f32) {
+  return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : f32 ? 1 : kAttendBlocks<256>);
 }
 
 }  // namespace hllm_rocm

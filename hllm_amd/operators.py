@@ -5,8 +5,8 @@ attended over by one new token a row (``kv_attention``).
 Thin calls of the C ABI (include/hllm_rocm.h, which states what each operator computes): they
 check types, shapes and devices, make the outputs that are not given, and enqueue on the current
 stream of the tensors' device. What a tensor's memory holds (slots, page tables, lengths) is not
-looked at on the host. Wrong tensors raise ValueError, what the library refuses raises
-``capi.StageError``.
+looked at on the host, and no gradients are recorded. Wrong tensors raise ValueError, what the
+library refuses raises ``capi.StageError``.
 
     plan = Rope(128, theta=1e6, scaling={"rope_type": "yarn", "factor": 4.0,
                                          "original_max_position_embeddings": 32768})
@@ -83,7 +83,8 @@ class KvPages:
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor,
                  value_scales: torch.Tensor):
-        _on_device(keys, "keys")
+        for name, x in (("keys", keys), ("values", values), ("key_scales", key_scales), ("value_scales", value_scales)):
+            _on_device(x, name)
         if keys.dtype not in _FORMATS or keys.dim() != 4:
             raise ValueError("keys must be [pages, kv_heads, page_tokens, head_dim] of float8_e4m3fn or int8")
         if values.shape != keys.shape or values.dtype != keys.dtype or values.stride() != keys.stride():

@@ -349,7 +349,7 @@ hllm_status hllm_rocm_stage_profile_records(hllm_rocm_stage* stage, char* buffer
  * be captured into a graph. `rows` = 0 enqueues nothing. Positions, slots, page tables and
  * lengths are read by the device when the kernels run, so a captured call takes what they
  * hold at each replay. Calls may run at once on several streams; what they write must not
- * overlap. */
+ * overlap, and neither may two outputs of one call. */
 
 /* One tensor [rows][heads][head_dimension]: the last dimension is contiguous, strides are in
  * elements. `data` is 16-byte aligned and so is every head's vector (strides that are
@@ -428,8 +428,8 @@ hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_r
 typedef enum { HLLM_KV_E4M3 = 0, HLLM_KV_INT8 = 1 } hllm_kv_format;
 
 /* A paged cache in device memory: codes at page * page_stride + position * token_stride + head *
- * head_stride (bytes, multiples of 16, token_stride at most 2^28; either of positions and heads inside the other; vectors
- * may not overlap) and scales [pages][kv_heads][page_tokens], for keys and values alike. A slot
+ * head_stride (bytes, multiples of 16; page_stride below 2^32, token_stride at most 2^28; either of
+ * positions and heads inside the other; vectors may not overlap) and scales [pages][kv_heads][page_tokens], for keys and values alike. A slot
  * is page * page_tokens + position in the page. All four pointers are 16-byte aligned. */
 typedef struct {
   uint32_t format;          /* hllm_kv_format */
@@ -478,7 +478,7 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
 typedef struct {
   uint64_t rows;
   const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */
-  uint64_t table_width;       /* table_width * page_tokens < 2^31 */
+  uint64_t table_width;       /* table_width * page_tokens at most 2^30 */
   uint64_t table_stride;
   const int32_t* lengths;     /* [rows] */
   uint64_t max_length;        /* the host's bound of the lengths: work is split for it */

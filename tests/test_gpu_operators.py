@@ -277,6 +277,18 @@ def test_kv_attention_of_large_and_small_queries(ops, dtype, q_scale):
     attend_case(ops, "e4m3", dtype, [70, 400], 8, 2, 128, 64, q_scale=q_scale, scale=0.05 / max(q_scale, 1e-30))
 
 
+def test_kv_attention_of_the_largest_queries(ops):
+    q, pages, table, n, most, _ = attend_case(ops, "int8", torch.bfloat16, [70, 400], 8, 2, 64, 64)
+    top = torch.finfo(torch.bfloat16).max
+    cache = {x: getattr(pages, x) for x in ("keys", "values", "key_scales", "value_scales")}
+    for dtype in (torch.bfloat16, torch.float32):
+        large = (q.sign() * top).to(dtype)
+        out = ops.kv_attention(large, pages, table, n, most, scale=1e-39)
+        expect, off = forms.attended(large, cache, table, n.tolist(), 1e-39)
+        # 1e-39 is below F32's normal range: held to 2^-149.
+        near(out, expect, off + 2.0 ** -149 * top * 64 * 4 * expect.abs().max())
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_kv_attention_weights_to_their_last_bits(ops, dim, dtype):

@@ -122,7 +122,7 @@ BAD_PAGES = [(None, "null"), (dict(format=2), "format"), (dict(head_dimension=96
              (dict(pages=0), "slots"), (dict(pages=1 << 25), "slots"), (dict(keys=None), "null"), (dict(value_scales=None), "null"),
              (dict(values=ADDRESS + 4), "aligned"), (dict(key_scales=ADDRESS + 4), "aligned"), (dict(token_stride=136), "16 bytes"),
              (dict(page_stride=8 * 64 * 128 - 16), "overlap"), (dict(token_stride=64), "overlap"), (dict(head_stride=128), "overlap"),
-             (dict(page_stride=1 << 41), "too large")]
+             (dict(page_stride=1 << 32), "too large"), (dict(token_stride=(1 << 28) + 16), "too large")]
 
 
 def pages_or_none(changes):
@@ -240,7 +240,8 @@ def test_kv_attention_refuses():
         refused(call(scale=scale), "scale")
     refused(call(lengths=None), "lengths")
     refused(call(page_table=None), "page_table")
-    refused(call(table_width=1 << 26), "page table")
+    for width in (1 << 26, (1 << 24) + 1):
+        refused(call(table_width=width), "page table")
     refused(call(table_stride=1 << 41), "table_stride")
     refused(call(workspace=None), "workspace")
     refused(call(workspace=ADDRESS + 4), "workspace")
