@@ -144,12 +144,9 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   __shared__ float2 cs[128];
   __shared__ float xs[kExchange ? kThreads * 17 : 1];
   const int row = blockIdx.x, t = threadIdx.x;
-  int slot = 0;
-  if constexpr (F >= 0) {
-    slot = uniform_load(a.slots + row);
-    if (slot < 0 || (slot >> a.pages.page_shift) >= a.pages.pages) return;
-  }
   const int R = a.rotary, half = R / 2;
+  // The slot, the position and the elements are loaded together; a padding row's go unused.
+  const int slot = F >= 0 ? uniform_load(a.slots + row) : 0, position = R > 0 ? uniform_load(a.positions + row) : 0;
   const int in_block = t / a.lanes, u = t - in_block * a.lanes;
   const int head = blockIdx.y * a.heads_per_block + in_block;
   const bool active = in_block < a.heads_per_block && head < a.q_heads + a.k_heads + a.v_heads;
@@ -167,8 +164,9 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
     load8(at<const T>(in, row, h, d0), x);
     load8(at<const T>(in, row, h, d1), x + 8);
   }
+  if (F >= 0 && (slot < 0 || (slot >> a.pages.page_shift) >= a.pages.pages)) return;
   if (t < half) {
-    const float2 v = turn(uniform_load(a.positions + row), a.turns[t]);
+    const float2 v = turn(position, a.turns[t]);
     cs[t] = float2{v.x * a.magnitude, v.y * a.magnitude};
   }
   if constexpr (kExchange) {
