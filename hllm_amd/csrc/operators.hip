@@ -460,8 +460,6 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   if (steps > 0 ? low >= high : start < from) continue;  // only the cost of starting it is this share's
   const int first = first_unit / budget;
   const int parts = a.shared && steps > 0 ? (first_unit + steps - 1) / budget - first + 1 : 1;
-  if (again) __syncthreads();  // the workgroup has read the last pair's sums
-  again = true;
   const int kvh = kvg / a.head_groups, g0 = (kvg - kvh * a.head_groups) * 16;
   const int begin = 128 * low, end = min(length, 128 * high);
   if (again) __syncthreads();  // the workgroup has read the last pair's sums
@@ -476,8 +474,9 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   char* tile = smem + wave * Layout::kBytes;
   const uint32_t tile_at = (uint32_t)(size_t)((__attribute__((address_space(3))) char*)smem) + wave * Layout::kBytes;
 
-  // One copy instruction takes 1 KiB: 16 / (D / 64) rows of 64 D.. bytes, so each lies in one group of
-  // eight positions, which is in one page; groups alternate between two sets of lane offsets.
+  // One copy instruction takes 1 KiB, sixteen bytes a lane, all of one group of eight positions, which lies
+  // in one page: the group's keys and values (D = 64), its keys (128) or half of them (256). The
+  // chunks' order differs between even and odd groups.
   uint32_t lane_at[2];
   const uint8_t* lane_from[2];
 #pragma unroll
@@ -570,7 +569,6 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
     }
   }
   __syncthreads();
-
 
   // The weights of a position are 2^(score - m) times its value scale; they enter the products
   // divided by r, and so do the sums o. r is a weight that was the largest once: it follows m, and is
@@ -966,6 +964,11 @@ void check_in_place(const hllm_rocm_tensor* in, const hllm_rocm_tensor* out, uin
     refuse("an output in its input's memory must have its strides");
 }
 
+// Two outputs, or an output and another tensor's input, that start at one address.
+void check_apart(const void* a, const char* name_a, const void* b, const char* name_b) {
+  if (a == b) refuse(std::string(name_a) + " and " + name_b + " are one memory");
+}
+
 void check_rows(uint64_t rows) {
   if (rows > kMostRows) refuse("at most 1048576 rows a call");
 }
@@ -1020,6 +1023,10 @@ class OnDevice {
   explicit OnDevice(int32_t device) {
     HIP_CHECK(hipGetDevice(&before_));
     if (before_ != device) {
+      // Asked first: the error of a failed hipSetDevice would be reported by the next launch.
+      int devices = 0;
+      HIP_CHECK(hipGetDeviceCount(&devices));
+      if (device >= devices) refuse("there is no device " + std::to_string(device));
       HIP_CHECK(hipSetDevice(device));
       changed_ = true;
     }
@@ -1137,6 +1144,11 @@ hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_r
     }
     a.lanes = (int32_t)head_dimension / 16;
     take_rope(rope, positions, a);
+    if (k) {
+      check_apart(q_out->data, "q_out", k_out->data, "k_out");
+      check_apart(q_out->data, "q_out", k->data, "k");
+      check_apart(k_out->data, "k_out", q->data, "q");
+    }
     OnDevice on(device);
     launch_rotate(static_cast<hipStream_t>(stream), q->dtype, -1, (int)rows, a);
     HIP_CHECK(hipGetLastError());
@@ -1174,6 +1186,11 @@ hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv
     }
     a.lanes = (int32_t)D / 16;
     if (rope) take_rope(rope, positions, a);
+    check_apart(pages->keys, "the cache's keys", pages->values, "values");
+    if (q) {
+      check_apart(q_out->data, "q_out", k->data, "k");
+      check_apart(q_out->data, "q_out", v->data, "v");
+    }
     OnDevice on(device);
     launch_rotate(static_cast<hipStream_t>(stream), k->dtype, (int)pages->format, (int)rows, a);
     HIP_CHECK(hipGetLastError());
@@ -1196,6 +1213,7 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
     if (k_out->heads != pages->kv_heads || v_out->heads != pages->kv_heads) refuse("k_out and v_out must have the cache's heads");
     if (k_out->dtype != v_out->dtype) refuse("k_out and v_out must have one dtype");
     if (rows * pages->kv_heads * (pages->head_dimension / 4) > kMostBlocks * kThreads) refuse("too many rows for these heads");
+    check_apart(k_out->data, "k_out", v_out->data, "v_out");
     OnDevice on(device);
     launch_kv_read(static_cast<hipStream_t>(stream), k_out->dtype, (int)pages->format, (int)pages->head_dimension, a);
     HIP_CHECK(hipGetLastError());
@@ -1229,14 +1247,15 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61. 7 F32 rows to 903, head dimension 64: 12.3 / 10.5.
   const uint64_t fit = attend_blocks((int)pages.head_dimension, false);
   const bool whole = steps * fit <= 5 * fit + 9 * pairs;
-  p.shared = !whole && rows <= kMostSharedRows && pairs <= (1u << 30) / cost;
-  if (!p.shared) {
-    p.blocks = pairs;
-    return p;
-  }
-  p.blocks = std::min<uint64_t>(fit, pairs * cost);
+  p.blocks = pairs;
+  if (whole || rows > kMostSharedRows) return p;
+  // The line of all pairs is counted in 31 bits. Where it could be longer the pairs stay whole, but the
+  // workspace is that of shares: a bound of the lengths is never given less than a smaller bound.
+  p.shared = pairs <= (1u << 30) / cost;
+  const uint64_t sharing = std::min<uint64_t>(fit, pairs * cost);
+  if (p.shared) p.blocks = sharing;
   p.cuts = (pairs + 1) / 2 * 2;  // whole sixteen bytes
-  p.parts = 2 * p.blocks * std::min<uint64_t>(group, 16);
+  p.parts = 2 * sharing * std::min<uint64_t>(group, 16);
   p.bytes = p.cuts * sizeof(int2) + p.parts * (pages.head_dimension + 2) * sizeof(float);
   return p;
 }
@@ -1274,7 +1293,7 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     a.out = tensor(&args->out, "out", rows, D, true);
     if (args->q.dtype != args->out.dtype || args->q.heads != args->out.heads) refuse("out must have q's dtype and heads");
     if (args->q.data == args->out.data) refuse("out must not be q");
-    if (!std::isfinite(args->scale)) refuse("scale is not finite");
+    if (!std::isfinite((float)(args->scale * kLog2e))) refuse("scale is not finite");  // as the kernels take it, with log2 e
     if (!args->lengths) refuse("lengths is null");
     if (args->table_width > kMostPositions / pages->page_tokens) refuse("a page table's row holds at most 2^30 positions");
     const uint64_t limit = std::min(clamp_length(args->max_length), args->table_width * pages->page_tokens);
@@ -1297,7 +1316,7 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     a.shared = plan.shared;
     a.scale_hi = (float)(args->scale * kLog2e);
     a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);
-    if (plan.bytes > 0) {
+    if (plan.shared) {
       a.cuts = static_cast<int2*>(args->workspace);
       a.part = reinterpret_cast<float*>(a.cuts + plan.cuts);
       a.stats = a.part + plan.parts * D;

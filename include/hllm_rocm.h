@@ -349,7 +349,7 @@ hllm_status hllm_rocm_stage_profile_records(hllm_rocm_stage* stage, char* buffer
  * be captured into a graph. `rows` = 0 enqueues nothing. Positions, slots, page tables and
  * lengths are read by the device when the kernels run, so a captured call takes what they
  * hold at each replay. Calls may run at once on several streams; what they write must not
- * overlap, and neither may two outputs of one call. */
+ * overlap, and neither may two outputs of one call (refused where they start at one address). */
 
 /* One tensor [rows][heads][head_dimension]: the last dimension is contiguous, strides are in
  * elements. `data` is 16-byte aligned and so is every head's vector (strides that are
@@ -429,8 +429,9 @@ typedef enum { HLLM_KV_E4M3 = 0, HLLM_KV_INT8 = 1 } hllm_kv_format;
 
 /* A paged cache in device memory: codes at page * page_stride + position * token_stride + head *
  * head_stride (bytes, multiples of 16; page_stride below 2^32, token_stride at most 2^28; either of
- * positions and heads inside the other; vectors may not overlap) and scales [pages][kv_heads][page_tokens], for keys and values alike. A slot
- * is page * page_tokens + position in the page. All four pointers are 16-byte aligned. */
+ * positions and heads inside the other; vectors may not overlap) and scales [pages][kv_heads]
+ * [page_tokens], for keys and values alike. A slot is page * page_tokens + position in the page. All
+ * four pointers are 16-byte aligned. */
 typedef struct {
   uint32_t format;          /* hllm_kv_format */
   uint32_t pages;           /* pages * page_tokens < 2^31 */
@@ -492,8 +493,8 @@ typedef struct {
 
 hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
                                    const hllm_rocm_kv_attention_args* args);
-/* The workspace that a call with `rows` rows of `query_heads` heads and this max_length needs
- * (0: none, and `workspace` may be NULL). Needs no device. */
+/* The workspace that does for a call with `rows` rows of `query_heads` heads and this max_length or a
+ * smaller one (0: none, and `workspace` may be NULL). Needs no device. */
 hllm_status hllm_rocm_kv_attention_workspace(const hllm_rocm_kv_pages* pages, uint64_t rows,
                                              uint32_t query_heads, uint64_t max_length,
                                              uint64_t* bytes);

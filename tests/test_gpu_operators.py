@@ -1,10 +1,12 @@
 """The operators on device memory against plain 64-bit forms (tests/operator_forms.py, which
 derives every bound), at the sizes, layouts and masks where they can go wrong."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
+from hllm_amd import capi
 from tests import operator_forms as forms
 from tests.operator_forms import HALF_STEP, LLAMA3, YARN
 
@@ -567,3 +569,15 @@ def test_tensors_are_checked(ops):
         with pytest.raises(capi.StageError) as e:
             call()
         assert e.value.status == capi.INVALID_REQUEST
+
+
+def test_a_device_that_is_not_there_is_refused(ops):
+    """... and leaves no error behind for the next call."""
+    plan, at = ops.Rope(64), torch.arange(3, dtype=torch.int32, device="cuda")
+    q = draw(3, 4, 64, torch.float16, 1)
+    t = capi.Tensor(q.data_ptr(), capi.F16, 4, 256, 64)
+    turned = ops.rope(plan, at, q)
+    status = capi.library().hllm_rocm_rope_apply(torch.cuda.device_count(), None, plan.address, at.data_ptr(), 3, 64, C.byref(t),
+                                                 C.byref(t), None, None)
+    assert status == capi.INVALID_REQUEST
+    assert torch.equal(ops.rope(plan, at, q), turned)

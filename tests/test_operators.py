@@ -295,3 +295,42 @@ def test_packed_bytes_have_the_structures_layouts():
     a = capi.KvAttentionArgs(3, ADDRESS, 5, 1 << 35, 2 * ADDRESS, 1 << 36, 0.5, t, capi.Tensor(ADDRESS + 16, 1, 9, 8, 4), 0, 1 << 37)
     assert operators.ATTENTION_ARGS.pack(*values(a)) == bytes(a)
     assert operators.ATTENTION_ARGS.size == C.sizeof(capi.KvAttentionArgs)
+
+
+def test_outputs_in_other_tensors_memory_are_refused():
+    lib, other = capi.library(), tensor(data=2 * ADDRESS)
+    third, fourth = tensor(data=3 * ADDRESS), tensor(data=4 * ADDRESS)
+
+    def rope(q, q_out, k, k_out):
+        return lib.hllm_rocm_rope_apply(0, None, by(plan()), ADDRESS, 4, 128, by(q), by(q_out), by(k), by(k_out))
+
+    refused(rope(tensor(), other, third, other), "one memory")
+    refused(rope(tensor(), other, other, third), "one memory")
+    refused(rope(tensor(), other, third, tensor()), "one memory")
+    apart = cache(values=2 * ADDRESS)
+
+    def append(pages, k, v, q, q_out):
+        return lib.hllm_rocm_kv_append(0, None, by(pages), ADDRESS, 4, by(k), by(v), by(plan()), ADDRESS, by(q), by(q_out))
+
+    refused(append(apart, other, third, fourth, other), "one memory")
+    refused(append(apart, other, third, fourth, third), "one memory")
+    refused(append(cache(), other, third, fourth, fourth), "one memory")
+    refused(lib.hllm_rocm_kv_read(0, None, by(apart), ADDRESS, 4, by(other), by(other)), "one memory")
+
+
+def test_a_scale_that_overflows_with_its_factor_is_refused():
+    a = capi.KvAttentionArgs(4, ADDRESS, 100, 100, ADDRESS, 6000, 3.4e38, tensor(), tensor(data=2 * ADDRESS), ADDRESS, 1 << 30)
+    refused(capi.library().hllm_rocm_kv_attention(0, None, C.byref(cache()), C.byref(a)), "scale")
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads", [(1, 32, 8), (64, 32, 8), (300, 64, 64), (1024, 1024, 1024), (1025, 8, 8)])
+def test_a_larger_bound_is_given_no_less_workspace(rows, heads, kv_heads):
+    """A call's bound is the smaller of max_length and its table's positions, so a workspace sized for any
+    larger max_length has to do."""
+    lib, need, last = capi.library(), C.c_uint64(0), 0
+    pages = cache(kv_heads=kv_heads, page_stride=kv_heads * 64 * 128)
+    for length in (0, 1, 100, 640, 641, 2000, 5000, 1 << 15, 1 << 18, 1 << 21, 1 << 26, 1 << 30, 1 << 40, (1 << 64) - 1):
+        assert lib.hllm_rocm_kv_attention_workspace(by(pages), rows, heads, length, C.byref(need)) == capi.OK
+        assert need.value >= last
+        last = need.value
+    assert rows > 1024 or last > 0
