@@ -135,10 +135,12 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
 // dimension of whole sixteens a thread holds both elements of its pairs (eight of either half);
 // interleaved pairs lie beside each other; other half layouts exchange through LDS (kExchange). So
 // every pair is read before it is written and a tensor can be rotated in place. Bound by memory:
-// 4.1 to 4.5 TB/s of 16-bit rows and 5.5 of F32 rows at 42 and 84 MB (a copy reaches 4.8).
+// 4.1 to 4.5 TB/s of 16-bit rows and 5.5 of F32 rows at 42 and 84 MB read and as much written (a copy of
+// 4 GiB reaches 4.8); interleaved 16-bit pairs 3.5 to 4.0, the exchange through LDS 3.0 to 3.7.
 //
 // F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
-// share its largest value by shuffles.
+// share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
+// heads of 256: 12.6 us, 4.3 TB/s; 64 rows 4.2 us, one chain of loads, sines, the largest value and the stores.
 template <typename T, int F, bool kExchange>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   __shared__ float2 cs[128];
@@ -242,8 +244,9 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
 // ---------------------------------------------------------------- reading back
 
 // A thread reads the codes of sixteen bytes of output of a key, and of the value beside it, and writes
-// them: a wave's accesses are whole lines (sixteen codes a thread, so F32 stores of 64 bytes a
-// lane: 3.5 TB/s). Nothing but memory traffic.
+// them: a wave's accesses are whole lines (with sixteen codes a thread F32 stores were 64 bytes a
+// lane apart: 3.5 TB/s). Nothing but memory traffic: 30000 positions of 8 heads of 128 to F16 32.6 us,
+// 5.7 TB/s; F32 5.2 to 6.1.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
   constexpr int kCodes = 16 / sizeof(T), L = D / kCodes;
@@ -379,6 +382,20 @@ __device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int v)
   return (uint64_t)(i == 0 ? 2 * first + 1 : 2 * (first + i)) * min(a.group, 16) + v;
 }
 
+// A pair's scores S = K Q^T (positions x query heads) and sums O^T = V^T P are products on the matrix
+// units: 16 query heads fill the columns of a 16 x 16 x 32 tile, so that groups of 1 to 16 heads read
+// each position once and cost the same. Codes are exact in F16; a key's scale enters its score and a
+// value's scale its weight, so no element is multiplied by a scale. The softmax (base 2) keeps its running
+// maximum and sum in F32 and the tile's weights go from the score product to the value product in
+// registers: with position 8 q + 4 h + i in row 4 q + i of score fragment h, a lane's scores are its
+// operand of the value product.
+//
+// Bound by the cache's bytes where it is long: 6.1 TB/s at 3 x 200000 positions (a streaming read 6.3). A
+// wave copies its next tile of 32 positions straight into LDS while it works on the last one, which is in registers by
+// then: one tile a wave, so that 3 workgroups (D = 128) fit a CU. Two tiles a wave and half the workgroups took
+// 31 us where this takes 26 (3 rows of 12000 to 30000 positions), tiles through registers 30. At
+// some hundred positions a row it is bound by the chain of a workgroup's start (length, page numbers, first tile:
+// 2.7 us) and the last round's imbalance: 64 rows to 2048 positions, 66 MB, 18.6 us.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kernel(AttendArgs a) {
   using Layout = Tile<D>;
@@ -778,7 +795,9 @@ __device__ inline int2 uniform_cut(const int2* p) {
 
 // Joins the parts of the pairs that were cut, one wave for a query head: each part's output weighted
 // with its share of the softmax sum. A part's vector takes D / 4 lanes, so a wave reads up to four parts at
-// once, and eight times as many before it uses them: the kernel is a few memory round trips long.
+// once, and eight times as many before it uses them: the kernel is a few memory round trips long (64 rows
+// of 32 heads 4.0 us, 3 rows of up to 30 parts a pair 5.3). A workgroup that joined the parts itself when it was the last
+// to arrive took 3 to 8 us longer: its stores and counts have to reach the other dies' caches.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kSlots = 64 / kLanes, kDeep = 8;
