@@ -267,6 +267,8 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
         raise ValueError("a row of page_table must be contiguous")
     if max_length < 0:
         raise ValueError("max_length is negative")
+    if scale is not None and not abs(scale) < 2e38:
+        raise ValueError("scale is not finite")  # in F32, with log2 e
     max_length = min(max_length, width * pages.page_tokens)
     if workspace is None:
         need = kv_attention_workspace(pages, rows, heads, max_length)

@@ -581,3 +581,10 @@ def test_a_device_that_is_not_there_is_refused(ops):
                                                  C.byref(t), None, None)
     assert status == capi.INVALID_REQUEST
     assert torch.equal(ops.rope(plan, at, q), turned)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39, -3e38])
+def test_scales_that_f32_does_not_hold_are_refused(ops, scale):
+    q, pages, table, n, most, _ = attend_case(ops, "e4m3", torch.float16, [20, 50], 4, 2, 64, 16)
+    with pytest.raises(ValueError):
+        ops.kv_attention(q, pages, table, n, most, scale=scale)
