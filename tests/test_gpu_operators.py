@@ -588,3 +588,41 @@ def test_scales_that_f32_does_not_hold_are_refused(ops, scale):
     q, pages, table, n, most, _ = attend_case(ops, "e4m3", torch.float16, [20, 50], 4, 2, 64, 16)
     with pytest.raises(ValueError):
         ops.kv_attention(q, pages, table, n, most, scale=scale)
+
+
+def test_the_most_rows_of_a_call(ops):
+    """1048576 rows at once equal the same rows in a call of their own."""
+    rows, dim, page = 1 << 20, 64, 8
+    pages = ops.KvPages.empty("int8", rows // page, 1, page, dim)
+    generator = torch.Generator("cuda").manual_seed(5)
+    q, k, v = (torch.randn(rows, 1, dim, generator=generator, device="cuda").half() for _ in range(3))
+    slots = torch.randperm(rows, generator=generator, device="cuda", dtype=torch.int32)
+    at = torch.arange(rows, dtype=torch.int32, device="cuda") * 2047 - (1 << 30)
+    plan = ops.Rope(dim)
+    turned = ops.kv_append(pages, slots, k, v, q=q, rope=plan, positions=at)
+    assert torch.equal(ops.rope(plan, at, q), turned)
+    keys, values = ops.kv_read(pages, slots)
+    table = torch.arange(rows, dtype=torch.int32, device="cuda")[:, None] % (rows // page)
+    n = torch.arange(rows, dtype=torch.int32, device="cuda") % (page + 1)
+    out = ops.kv_attention(turned, pages, table, n, page)
+    other = ops.KvPages.empty("int8", rows // page, 1, page, dim)
+    for part in (slice(0, 700), slice(rows // 2 - 5, rows // 2 + 300), slice(rows - 513, rows)):
+        one = ops.kv_append(other, slots[part], k[part], v[part], q=q[part], rope=plan, positions=at[part])
+        assert torch.equal(one, turned[part])
+        for x, y in zip(ops.kv_read(other, slots[part]), (keys, values)):
+            assert torch.equal(x, y[part])
+        assert torch.equal(ops.kv_attention(turned[part], pages, table[part], n[part], page), out[part])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_that_name_one_slot_read_alike(ops, kind):
+    """Equal rows written to one slot leave that row there; a slot may be read any number of times."""
+    pages = ops.KvPages.empty(kind, 4, 3, 16, 128)
+    k, v = (draw(1, 3, 128, torch.float16, s).expand(40, 3, 128) for s in (1, 2))
+    slots = torch.full((40,), 21, dtype=torch.int32, device="cuda")
+    ops.kv_append(pages, slots, k, v)
+    alone = ops.KvPages.empty(kind, 4, 3, 16, 128)
+    ops.kv_append(alone, slots[:1], k[:1], v[:1])
+    for x, y in zip(ops.kv_read(pages, slots), ops.kv_read(alone, slots[:1])):
+        assert torch.equal(x, y.expand(40, 3, 128))
+    assert torch.equal(pages.keys.view(torch.int8), alone.keys.view(torch.int8))
