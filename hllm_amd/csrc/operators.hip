@@ -830,7 +830,9 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
         y *= decay;
         top = most;
       }
-      const float weight = lane < n && own.x != -INFINITY ? exp2_fast(own.x - top) * own.y : 0.0f;
+      // A part holds nothing where its sum is 0. The maximum does not tell: NaN scores leave it at -inf and
+      // the sum NaN, which goes on to the output.
+      const float weight = lane < n && own.y != 0.0f ? exp2_fast(own.x - top) * own.y : 0.0f;
 #pragma unroll
       for (int j = 0; j < kDeep; ++j) {
         const int i = j0 + j * kSlots + slot;

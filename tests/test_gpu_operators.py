@@ -626,3 +626,45 @@ def test_rows_that_name_one_slot_read_alike(ops, kind):
     for x, y in zip(ops.kv_read(pages, slots), ops.kv_read(alone, slots[:1])):
         assert torch.equal(x, y.expand(40, 3, 128))
     assert torch.equal(pages.keys.view(torch.int8), alone.keys.view(torch.int8))
+
+
+# ------------------------------------------------------------------ rows whose work is cut
+
+
+def cut(ops, pages, lengths, q_heads, most):
+    """Whether a call with these rows cuts pairs (a call that does not has no workspace)."""
+    return ops.kv_attention_workspace(pages, len(lengths), q_heads, most) > 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_stays_nan_where_work_is_cut(ops, kind, dtype, dim):
+    """A NaN in a query, in every key scale of a row and head, or in those of some positions makes that
+    head's (or group's) output NaN and no other, at bounds of the lengths that cut a row and that do not."""
+    lengths, page = [5000, 40, 3000], 64
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim)
+    pages = ops.KvPages(**cache)
+    q = draw(3, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
+
+    def check(q, bad):
+        for most in (5000, 2048, 300):
+            out = ops.kv_attention(q, pages, table, n, most)
+            assert torch.equal(torch.isnan(out).all(-1), bad) and torch.equal(torch.isnan(out).any(-1), bad), most
+
+    bad = torch.zeros(3, 8, dtype=torch.bool, device="cuda")
+    check(q, bad)
+    wrong = q.clone()
+    wrong[0, 3, 9] = math.nan
+    wrong[1, 7, 0] = math.nan
+    wrong[2] = math.nan
+    bad[0, 3] = bad[1, 7] = bad[2] = True
+    check(wrong, bad)
+    cache["key_scales"][table[0].long(), 1] = math.nan
+    cache["key_scales"][table[2, 2].long(), 0, 5:9] = math.nan
+    bad[:] = False
+    bad[0, 4:] = bad[2, :4] = True
+    check(q, bad)
