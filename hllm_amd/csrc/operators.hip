@@ -595,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
 #pragma unroll
   for (int f = 0; f < DF; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f, r = 0.0f;
+  bool any = false;  // whether the wave has had a position
 
   // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are the eight
   // positions 8 quad .. + 7, which are also its slots of the value products.
@@ -605,6 +606,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int gone = missing;
     const bool whole = gone == 0 && t + 32 <= end;
+    any |= gone != 15;  // groups behind the end count as the last one's page
     if (!whole) {
       // Values of positions past the part and in pages that are not there, whatever they are.
       const int own = lane >> 1;
@@ -670,7 +672,8 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       const float d = i < 4 ? s0[i & 3] : s1[i & 3];
       const float by = ks[i] * factor;
       sc[i] = d * by;
-      if constexpr (P == 2) by_lo[i] = fmaf(d, by, -sc[i]) + d * (fmaf(ks[i], factor, -by) + ks[i] * factor_lo);
+      if constexpr (P == 2)
+        by_lo[i] = sc[i] == -INFINITY ? 0.0f : fmaf(d, by, -sc[i]) + d * (fmaf(ks[i], factor, -by) + ks[i] * factor_lo);
     }
     if (!whole) {
       const int valid = (gone >> quad) & 1 ? 0 : end - (t + 8 * quad);
@@ -748,6 +751,8 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
 
   // The four waves' states meet in LDS, each wave's in its own tile.
   l = column_sum(l);
+  // Only scores of -inf (an infinite query's): a sum that is not 0 beside that maximum tells them from no positions.
+  if (any && l == 0.0f) l = 1.0f;
   if (quad == 0) {
     states[wave][0][col] = m;
     states[wave][1][col] = l;
@@ -765,9 +770,12 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   if (a.cuts && low == 0 && threadIdx.x == 0) a.cuts[row * in_row + kvg] = int2{first, parts};
   for (int e = threadIdx.x; e < vectors * (D / 4); e += kThreads) {
     const int v = e / (D / 4), d = e % (D / 4) * 4;
-    float top = -INFINITY, total = 0.0f;
+    float top = -INFINITY, total = 0.0f, held = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, states[w][0][v]);
+    for (int w = 0; w < 4; ++w) {
+      top = fmaxf(top, states[w][0][v]);
+      held += states[w][1][v];
+    }
     const float base = top == -INFINITY ? 0.0f : top;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -778,9 +786,11 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
            (states[w][2][v] * decay);
     }
     y *= total == 0.0f ? 0.0f : 1.0f / total;
+    const bool undefined = total == 0.0f && held != 0.0f;  // no softmax of scores that are all -inf
     if (parts == 1) {
-      store4(out + v * a.out.head + d, y);
+      store4(out + v * a.out.head + d, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
     } else {
+      if (undefined) total = 1.0f;  // NaN in the join, unless another part has finite scores
       const uint64_t part = part_at(a, first, me - first, v);
       *reinterpret_cast<floatx4*>(a.part + part * D + d) = y;
       if (d == 0) *reinterpret_cast<float2*>(a.stats + 2 * part) = float2{top, total};

@@ -474,8 +474,8 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
  * A row's length counts at most max_length and table_width * page_tokens positions; a length
  * of 0 gives zeros and a negative one marks a padding row, which is left as it was. Positions in
  * pages outside [0, pages) take no part, as if they were masked (a dropped page is -1); a row
- * with no other position gives zeros. What lies in a page behind a row's length is not used,
- * NaN or not. */
+ * with no other position gives zeros. NaN scores, and scores that are all -inf (an infinite query),
+ * give NaN. What lies in a page behind a row's length is not used, NaN or not. */
 typedef struct {
   uint64_t rows;
   const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */

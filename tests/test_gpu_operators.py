@@ -668,3 +668,49 @@ def test_nan_stays_nan_where_work_is_cut(ops, kind, dtype, dim):
     bad[:] = False
     bad[0, 4:] = bad[2, :4] = True
     check(q, bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("infinity", [math.inf, -math.inf])
+def test_infinite_queries_give_nan(ops, dtype, infinity):
+    """Scores that are all infinite, of either sign, have no softmax: NaN, whether a row is cut or not; rows
+    without positions stay zeros."""
+    lengths, page = [5000, 40, 0, 700], 32
+    table, count = paged(lengths, page)
+    table[3] = -1
+    cache = forms.make_pages("int8", count, 2, page, 128)
+    cache["keys"][..., 9] = 5
+    pages = ops.KvPages(**cache)
+    q = draw(4, 8, 128, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
+    for most in (5000, 300):
+        clean = ops.kv_attention(q, pages, table, n, most)
+        assert not torch.isnan(clean).any()
+        wrong = q.clone()
+        wrong[:, 2, 9] = infinity
+        out = ops.kv_attention(wrong, pages, table, n, most)
+        assert torch.isnan(out[:2, 2]).all() and (out[2:] == 0).all()
+        out[:, 2] = clean[:, 2] = 0
+        assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_minus_infinity_weigh_nothing(ops, dtype):
+    """... beside finite ones, in the same tile or in other parts of a cut row: as if their pages were dropped."""
+    lengths, page = [5000, 40, 700], 32
+    table, count = paged(lengths, page)
+    cache = forms.make_pages("int8", count, 2, page, 128)
+    q = draw(3, 8, 128, dtype, 1).abs() + 0.25
+    gone = table.clone()
+    gone[0, 20:90] = gone[0, 101] = gone[1, 0] = gone[2, ::2] = -1
+    there = torch.unique(gone[gone >= 0]).long()
+    lost = torch.ones(count, dtype=torch.bool, device="cuda")
+    lost[there] = False
+    cache["keys"][lost] = -3
+    cache["key_scales"][lost] = math.inf
+    pages = ops.KvPages(**cache)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
+    for most in (5000, 300):
+        assert torch.equal(ops.kv_attention(q, pages, table, n, most), ops.kv_attention(q, pages, gone, n, most))
