@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       const float p = exp2_fast(P == 2 ? (sc[i] - base) + by_lo[i] : sc[i] - base);
       sum += p;
       weight[i] = p * vs[i];
-      largest = fmaxf(largest, weight[i]);
+      largest = fmaxf(largest, fabsf(weight[i]));  // a caller's own scales may be negative
     }
     l = l * decay + sum;
     m = m_new;

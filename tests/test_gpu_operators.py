@@ -714,3 +714,24 @@ def test_scores_of_minus_infinity_weigh_nothing(ops, dtype):
     assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
     for most in (5000, 300):
         assert torch.equal(ops.kv_attention(q, pages, table, n, most), ops.kv_attention(q, pages, gone, n, most))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_value_scales_of_either_sign(ops, dtype, dim):
+    """Negated value scales with negated codes are the same values: the same bits come out."""
+    lengths, page = [5000, 40, 1, 700], 32
+    table, count = paged(lengths, page)
+    cache = forms.make_pages("int8", count, 2, page, dim)
+    other = {name: x.clone() for name, x in cache.items()}
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    flip = torch.rand(cache["value_scales"].shape, generator=g, device="cuda") < 0.5
+    flip[table[1].long()] = True  # a row of negative scales alone
+    other["value_scales"][flip] *= -1
+    other["values"] = torch.where(flip[..., None], -other["values"], other["values"])
+    q = draw(4, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for most in (5000, 300):
+        expect = ops.kv_attention(q, ops.KvPages(**cache), table, n, most)
+        assert torch.equal(ops.kv_attention(q, ops.KvPages(**other), table, n, most), expect)
