@@ -777,15 +777,20 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       held += states[w][1][v];
     }
     const float base = top == -INFINITY ? 0.0f : top;
+    float decay[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      decay[w] = exp2_fast(states[w][0][v] - base);
+      total += states[w][1][v] * decay[w];
+    }
+    // Divided by the total before r's share of a value scale enters: a mean of large values is finite, their sum may not be.
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float decay = exp2_fast(states[w][0][v] - base);
-      total += states[w][1][v] * decay;
-      y += reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[(d / DF % 4 * VW + d % DF / 4) * 64 + d / (4 * DF) * 16 + v] *
-           (states[w][2][v] * decay);
+      const floatx4 x = reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[(d / DF % 4 * VW + d % DF / 4) * 64 + d / (4 * DF) * 16 + v];
+      y += x * inverse * (states[w][2][v] * decay[w]);
     }
-    y *= total == 0.0f ? 0.0f : 1.0f / total;
     const bool undefined = total == 0.0f && held != 0.0f;  // no softmax of scores that are all -inf
     if (parts == 1) {
       store4(out + v * a.out.head + d, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
@@ -822,11 +827,12 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
   const auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.stats + 2 * part_at(a, first, min(i, parts - 1), v)); };
   floatx4 y = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, total = 0.0f;
+  bool held = false;
   for (int i0 = 0; i0 < parts; i0 += 64) {
     // Statistics and the first outputs of 64 parts are loaded together.
     const int n = min(64, parts - i0);
     const float2 own = stat(i0 + lane);
-    float most = lane < n ? own.x : -INFINITY;
+    float most = lane < n ? own.x : -INFINITY, weight = 0.0f;
     for (int j0 = 0; j0 < n; j0 += kSlots * kDeep) {
       floatx4 x[kDeep];
 #pragma unroll
@@ -835,31 +841,34 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
       if (j0 == 0) {
         for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
         most = fmaxf(most, top);
-        const float decay = top == -INFINITY ? 0.0f : exp2_fast(top - most);
-        total *= decay;
-        y *= decay;
+        // A part holds nothing where its sum is 0. The maximum does not tell: NaN scores leave it at -inf and
+        // the sum NaN, which goes on to the output.
+        const float base = most == -INFINITY ? 0.0f : most, before = total * exp2_fast(top - base);
         top = most;
+        weight = lane < n ? exp2_fast(own.x - base) * own.y : 0.0f;
+        held |= __any(lane < n && own.y != 0.0f);
+        // y is kept divided by the total: means of large values are finite, their sums may not be.
+        total = weight;
+        for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+        total += before;
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        weight *= inverse;
+        y *= before * inverse;
       }
-      // A part holds nothing where its sum is 0. The maximum does not tell: NaN scores leave it at -inf and
-      // the sum NaN, which goes on to the output.
-      const float weight = lane < n && own.y != 0.0f ? exp2_fast(own.x - top) * own.y : 0.0f;
 #pragma unroll
       for (int j = 0; j < kDeep; ++j) {
         const int i = j0 + j * kSlots + slot;
         const float w = __shfl(weight, min(i, 63), 64);
-        if (i < n) {
-          total += w;
-          y += x[j] * w;
-        }
+        if (i < n) y += x[j] * w;
       }
     }
   }
   for (int o = kLanes; o < 64; o <<= 1) {
-    total += __shfl_xor(total, o, 64);
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], o, 64);
   }
-  if (slot == 0) store4(at<T>(a.out, row, head, d), total == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : y / total);
+  const bool undefined = total == 0.0f && held;
+  if (slot == 0) store4(at<T>(a.out, row, head, d), undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
 }
 
 template <typename T, int F>

@@ -735,3 +735,48 @@ def test_value_scales_of_either_sign(ops, dtype, dim):
     for most in (5000, 300):
         expect = ops.kv_attention(q, ops.KvPages(**cache), table, n, most)
         assert torch.equal(ops.kv_attention(q, ops.KvPages(**other), table, n, most), expect)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_near_the_largest_number(ops, dtype, dim):
+    """Means of values up to 2.5e38 are finite, though sums of two of them are not."""
+    lengths, page = [5000, 300, 2, 9000], 32
+    table, count = paged(lengths, page)
+    cache = forms.make_pages("int8", count, 2, page, dim)
+    cache["values"].copy_(cache["values"].abs().clamp_min(60))
+    cache["value_scales"].copy_((0.5 + 20 * cache["value_scales"]).clamp_max(1.0) * 2e36)
+    q = draw(4, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    pages = ops.KvPages(**cache)
+    assert cut(ops, pages, lengths, 8, 9000)
+    for most in (9000, 300):
+        expect, off = forms.attended(q, cache, table, lengths, dim ** -0.5, most)
+        assert expect.max() > 1e38
+        near(ops.kv_attention(q, pages, table, n, most), expect, off)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_pairs_of_more_than_64_parts(ops, dtype, dim):
+    """A pair that most workgroups share, whose first two thirds hold nothing, nothing finite or NaN."""
+    lengths, page = [150000], 64
+    table, count = paged(lengths, page)
+    cache = forms.make_pages("int8", count, 1, page, dim, stale=True)
+    forms.fill(cache, "int8", table, lengths)
+    q = draw(1, 4, dim, dtype, 1).abs() + 0.25
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    gone = table.clone()
+    gone[0, :1600] = -1
+    pages = ops.KvPages(**cache)
+    expect, off = forms.attended(q, cache, table, lengths, dim ** -0.5)
+    near(ops.kv_attention(q, pages, table, n, 150000), expect, off)
+    expect, off = forms.attended(q, cache, gone, lengths, dim ** -0.5)
+    dropped = ops.kv_attention(q, pages, gone, n, 150000)
+    near(dropped, expect, off)
+    lost = table[0, :1600].long()
+    cache["keys"][lost] = -3
+    cache["key_scales"][lost] = math.inf
+    assert torch.equal(ops.kv_attention(q, pages, table, n, 150000), dropped)
+    cache["key_scales"][lost[7], 0, 5] = math.nan
+    assert torch.isnan(ops.kv_attention(q, pages, table, n, 150000)).all()
