@@ -780,3 +780,24 @@ def test_pairs_of_more_than_64_parts(ops, dtype, dim):
     assert torch.equal(ops.kv_attention(q, pages, table, n, 150000), dropped)
     cache["key_scales"][lost[7], 0, 5] = math.nan
     assert torch.isnan(ops.kv_attention(q, pages, table, n, 150000)).all()
+
+
+@pytest.mark.parametrize("kind,dtype,dim", [("e4m3", torch.float16, 128), ("int8", torch.bfloat16, 256), ("e4m3", torch.float32, 64),
+                                            ("int8", torch.float32, 256)])
+@pytest.mark.parametrize("lengths", [
+    [10000] + [0, -1, 5, 40] * 16, [3, 0] * 32 + [8191], [-1] * 129 + [6000], [130, 1] * 40 + [12000, -1, 7000] + [0] * 47,
+    [9000] + [20, -1, 0, 129, 3] * 139 + [-1, 2500, 1, 0], [-1, 64] * 511 + [10000, 9], [0] * 500 + [16000] + [1] * 523])
+def test_shares_of_many_rows(ops, kind, dtype, dim, lengths):
+    """65 to 1024 rows, several to a lane of the scan that finds a share's first row, of which one or two are long."""
+    q, pages, *_ = attend_case(ops, kind, dtype, lengths, 2, 1, dim, 16)
+    assert cut(ops, pages, lengths, 2, max(lengths))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128), (torch.float32, 128), (torch.float16, 256),
+                                       (torch.float32, 256)])
+@pytest.mark.parametrize("q_heads,heads", [(20, 1), (32, 1), (40, 2), (17, 1), (64, 1)])
+def test_cut_groups_of_more_than_sixteen_heads(ops, kind, dtype, dim, q_heads, heads):
+    for lengths in ([5000], [129, 20000, -1, 0, 6400]):
+        q, pages, *_ = attend_case(ops, kind, dtype, lengths, q_heads, heads, dim, 32)
+        assert cut(ops, pages, lengths, q_heads, max(lengths))
