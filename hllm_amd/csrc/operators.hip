@@ -1227,9 +1227,18 @@ hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv
     a.lanes = (int32_t)D / 16;
     if (rope) take_rope(rope, positions, a);
     check_apart(pages->keys, "the cache's keys", pages->values, "values");
+    check_apart(pages->keys, "the cache's keys", pages->key_scales, "key_scales");
+    check_apart(pages->keys, "the cache's keys", pages->value_scales, "value_scales");
+    check_apart(pages->values, "the cache's values", pages->key_scales, "key_scales");
+    check_apart(pages->values, "the cache's values", pages->value_scales, "value_scales");
+    check_apart(pages->key_scales, "the cache's key_scales", pages->value_scales, "value_scales");
     if (q) {
       check_apart(q_out->data, "q_out", k->data, "k");
       check_apart(q_out->data, "q_out", v->data, "v");
+      check_apart(q_out->data, "q_out", pages->keys, "the cache's keys");
+      check_apart(q_out->data, "q_out", pages->values, "the cache's values");
+      check_apart(q_out->data, "q_out", pages->key_scales, "the cache's key_scales");
+      check_apart(q_out->data, "q_out", pages->value_scales, "the cache's value_scales");
     }
     OnDevice on(device);
     launch_rotate(static_cast<hipStream_t>(stream), k->dtype, (int)pages->format, (int)rows, a);
@@ -1342,6 +1351,10 @@ hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm
     const AttendPlan plan = plan_attention(*pages, rows, args->q.heads, limit);
     if (plan.bytes > 0 && (!args->workspace || args->workspace_bytes < plan.bytes || (uintptr_t)args->workspace % 16))
       refuse("the workspace is null, not 16-byte aligned or below " + std::to_string(plan.bytes) + " bytes");
+    if (plan.bytes > 0) {
+      check_apart(args->workspace, "the workspace", args->out.data, "out");
+      check_apart(args->workspace, "the workspace", args->q.data, "q");
+    }
     a.table = args->page_table;
     a.table_stride = args->table_stride;
     a.lengths = args->lengths;

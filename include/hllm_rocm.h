@@ -349,7 +349,8 @@ hllm_status hllm_rocm_stage_profile_records(hllm_rocm_stage* stage, char* buffer
  * be captured into a graph. `rows` = 0 enqueues nothing. Positions, slots, page tables and
  * lengths are read by the device when the kernels run, so a captured call takes what they
  * hold at each replay. Calls may run at once on several streams; what they write must not
- * overlap, and neither may two outputs of one call (refused where they start at one address). */
+ * overlap, and neither may two outputs of one call, a cache's four buffers and a workspace among
+ * them (refused where they start at one address). */
 
 /* One tensor [rows][heads][head_dimension]: the last dimension is contiguous, strides are in
  * elements. `data` is 16-byte aligned and so is every head's vector (strides that are

@@ -334,3 +334,24 @@ def test_a_larger_bound_is_given_no_less_workspace(rows, heads, kv_heads):
         assert need.value >= last
         last = need.value
     assert rows > 1024 or last > 0
+
+
+def test_cache_buffers_and_a_workspace_in_one_memory_are_refused():
+    lib = capi.library()
+    k, v, q, q_out = (tensor(data=i * ADDRESS) for i in (5, 6, 7, 8))
+    buffers = ("keys", "values", "key_scales", "value_scales")
+    apart = {name: (i + 1) * ADDRESS for i, name in enumerate(buffers)}
+
+    def append(pages, out=None):
+        return lib.hllm_rocm_kv_append(0, None, by(pages), ADDRESS, 4, by(k), by(v), by(plan()), ADDRESS, by(q if out else None), by(out))
+
+    for i, name in enumerate(buffers):
+        for other in buffers[:i]:
+            one = cache(**{**apart, name: apart[other]})
+            refused(append(one), f"{other} and {name} are one memory")
+            refused(append(one, q_out), f"{other} and {name} are one memory")
+        refused(append(cache(**apart), tensor(data=apart[name])), f"q_out and the cache's {name} are one memory")
+    for place in (7, 8):
+        a = capi.KvAttentionArgs(4, ADDRESS, 100, 100, ADDRESS, 6000, 0.1, tensor(heads=32, data=7 * ADDRESS),
+                                 tensor(heads=32, data=8 * ADDRESS), place * ADDRESS, 1 << 30)
+        refused(lib.hllm_rocm_kv_attention(0, None, C.byref(cache(**apart)), C.byref(a)), "one memory")
