@@ -871,13 +871,19 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
   if (slot == 0) store4(at<T>(a.out, row, head, d), undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
 }
 
+// Threads for a row's heads of `lanes` lanes in one workgroup of rotate_kernel, and its workgroups.
+int rotate_threads(const RotateArgs& a) { return std::min(kThreads, ((a.q_heads + a.k_heads + a.v_heads) * a.lanes + 63) / 64 * 64); }
+int rotate_blocks(const RotateArgs& a) {
+  const int heads = a.q_heads + a.k_heads + a.v_heads, per_block = rotate_threads(a) / a.lanes;
+  return (heads + per_block - 1) / per_block;
+}
+
 template <typename T, int F>
 void rotate(hipStream_t stream, int rows, const RotateArgs& a) {
-  const int heads = a.q_heads + a.k_heads + a.v_heads;
-  const int threads = std::min(kThreads, (heads * a.lanes + 63) / 64 * 64);
+  const int threads = rotate_threads(a);
   RotateArgs b = a;
   b.heads_per_block = threads / a.lanes;
-  const dim3 grid(rows, (heads + b.heads_per_block - 1) / b.heads_per_block);
+  const dim3 grid(rows, rotate_blocks(a));
   // The block's first rotary / 2 threads compute the cosines.
   const int block = std::max(threads, (a.rotary / 2 + 63) / 64 * 64);
   if (!a.interleaved && a.rotary % 16)
@@ -961,7 +967,7 @@ void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int hea
 
 namespace {
 
-// Rows of one call: grids stay below 2^32 threads.
+// Rows of one call, and workgroups of kThreads threads of one launch: below 2^32 threads over all of a grid's dimensions.
 constexpr uint64_t kMostRows = 1u << 20;
 constexpr uint64_t kMostBlocks = (1u << 24) - 1;
 
@@ -1011,6 +1017,10 @@ void check_apart(const void* a, const char* name_a, const void* b, const char* n
 
 void check_rows(uint64_t rows) {
   if (rows > kMostRows) refuse("at most 1048576 rows a call");
+}
+
+void check_rotate_grid(uint64_t rows, const RotateArgs& a) {
+  if (rows * rotate_blocks(a) > kMostBlocks) refuse("too many rows for these heads");
 }
 
 Pages pages_of(const hllm_rocm_kv_pages* p) {
@@ -1183,6 +1193,7 @@ hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_r
       a.k_heads = (int32_t)k->heads;
     }
     a.lanes = (int32_t)head_dimension / 16;
+    check_rotate_grid(rows, a);
     take_rope(rope, positions, a);
     if (k) {
       check_apart(q_out->data, "q_out", k_out->data, "k_out");
@@ -1225,6 +1236,7 @@ hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv
       a.q_heads = (int32_t)q->heads;
     }
     a.lanes = (int32_t)D / 16;
+    check_rotate_grid(rows, a);
     if (rope) take_rope(rope, positions, a);
     check_apart(pages->keys, "the cache's keys", pages->values, "values");
     check_apart(pages->keys, "the cache's keys", pages->key_scales, "key_scales");

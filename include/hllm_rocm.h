@@ -346,9 +346,10 @@ hllm_status hllm_rocm_stage_profile_records(hllm_rocm_stage* stage, char* buffer
  * its default stream). A call checks its arguments on the host (HLLM_INVALID_REQUEST, nothing
  * enqueued), enqueues its kernels on `stream` and returns without waiting; it allocates
  * nothing, keeps nothing between calls, leaves the thread's current device as it was and may
- * be captured into a graph. `rows` = 0 enqueues nothing. Positions, slots, page tables and
- * lengths are read by the device when the kernels run, so a captured call takes what they
- * hold at each replay. Calls may run at once on several streams; what they write must not
+ * be captured into a graph. `rows` = 0 enqueues nothing; a call takes at most 2^20 rows, and of
+ * very many heads no more than launches of less than 2^32 threads do. Positions, slots, page
+ * tables and lengths are read by the device when the kernels run, so a captured call takes what
+ * they hold at each replay. Calls may run at once on several streams; what they write must not
  * overlap, and neither may two outputs of one call, a cache's four buffers and a workspace among
  * them (refused where they start at one address). */
 

@@ -355,3 +355,20 @@ def test_cache_buffers_and_a_workspace_in_one_memory_are_refused():
         a = capi.KvAttentionArgs(4, ADDRESS, 100, 100, ADDRESS, 6000, 0.1, tensor(heads=32, data=7 * ADDRESS),
                                  tensor(heads=32, data=8 * ADDRESS), place * ADDRESS, 1 << 30)
         refused(lib.hllm_rocm_kv_attention(0, None, C.byref(cache(**apart)), C.byref(a)), "one memory")
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """2^32 threads of sixteen elements: reached by many heads below the most rows."""
+    lib = capi.library()
+    q, q_out = tensor(heads=1024, dim=256), tensor(heads=1024, dim=256, data=2 * ADDRESS)
+    k, k_out = tensor(heads=1024, dim=256, data=3 * ADDRESS), tensor(heads=1024, dim=256, data=4 * ADDRESS)
+
+    def rope(rows, *tensors):
+        return lib.hllm_rocm_rope_apply(0, None, by(plan()), ADDRESS, rows, 256, *(by(x) for x in (tensors + (None, None))[:4]))
+
+    refused(rope(1 << 20, q, q_out), "too many rows")
+    refused(rope(1 << 18, q, q_out), "too many rows")  # 64 workgroups a row: 2^24
+    refused(rope(1 << 17, q, q_out, k, k_out), "too many rows")
+    wide = cache(kv_heads=1024, head_dimension=256, head_stride=64 * 256, token_stride=256, page_stride=1024 * 64 * 256,
+                 keys=5 * ADDRESS, values=6 * ADDRESS, key_scales=7 * ADDRESS, value_scales=8 * ADDRESS)
+    refused(lib.hllm_rocm_kv_append(0, None, by(wide), ADDRESS, 1 << 17, by(q), by(k), None, None, None, None), "too many rows")
