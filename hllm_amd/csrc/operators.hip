@@ -1132,6 +1132,7 @@ void plan_rope(const hllm_rocm_rope_config& c, hllm_rocm_rope& out) {
     first = std::max(0.0L, std::floor(pair(fast)));
     last = std::min((long double)n - 1, std::ceil(pair(slow)));
     r.magnitude = (float)positive(c.magnitude, 0.1 * std::log(c.factor) + 1.0, "magnitude");
+    if (!(r.magnitude > 0.0f) || !std::isfinite(r.magnitude)) refuse("magnitude is no F32 number");
   }
   const long double step = -2.0L * std::log((long double)c.theta) / n;
   for (uint32_t i = 0; i < n / 2; ++i) {

@@ -395,7 +395,7 @@ typedef struct {
   double high_frequency_factor;  /* LLAMA3: > low_frequency_factor */
   double beta_fast;              /* YARN: > beta_slow; 0 = 32 */
   double beta_slow;              /* YARN: > 0; 0 = 1 */
-  double magnitude;              /* YARN: >= 0 */
+  double magnitude;              /* YARN: >= 0, and so in F32 */
 } hllm_rocm_rope_config;
 
 /* A rotation's plan, host memory filled by hllm_rocm_rope_plan and kept by the caller: each

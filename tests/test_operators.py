@@ -372,3 +372,10 @@ def test_launches_of_too_many_threads_are_refused():
     wide = cache(kv_heads=1024, head_dimension=256, head_stride=64 * 256, token_stride=256, page_stride=1024 * 64 * 256,
                  keys=5 * ADDRESS, values=6 * ADDRESS, key_scales=7 * ADDRESS, value_scales=8 * ADDRESS)
     refused(lib.hllm_rocm_kv_append(0, None, by(wide), ADDRESS, 1 << 17, by(q), by(k), None, None, None, None), "too many rows")
+
+
+@pytest.mark.parametrize("magnitude", [3.5e38, 1e300, 1e-46])
+def test_a_magnitude_that_f32_does_not_hold_is_refused(magnitude):
+    lib, plan = capi.library(), capi.RopePlan(rotary_dimension=5)
+    refused(lib.hllm_rocm_rope_plan(C.byref(config(scaling=capi.ROPE_YARN, magnitude=magnitude)), C.byref(plan)), "magnitude")
+    assert plan.rotary_dimension == 5
