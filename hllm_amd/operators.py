@@ -25,6 +25,7 @@ from . import capi
 
 _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _FORMATS = {torch.float8_e4m3fn: capi.KV_E4M3, torch.int8: capi.KV_INT8}
+_MOST = (1 << 32) - 1  # past every size that the library takes, and past every length that counts
 _CODES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 # capi.Tensor and capi.KvAttentionArgs as bytes: a quarter of the time of filling a ctypes structure.
 TENSOR = struct.Struct("@PIIQQ")
@@ -48,6 +49,8 @@ class Rope:
 
     def __init__(self, rotary_dim: int, theta: float = 10000.0, interleaved: bool = False,
                  scaling: dict | None = None):
+        if not 0 <= rotary_dim < 1 << 32:  # ctypes would take it modulo 2^32
+            raise ValueError("the rotary dimension is even, 2 to 256")
         c = capi.RopeConfig(rotary_dimension=rotary_dim, theta=theta,
                             layout=capi.ROPE_INTERLEAVED if interleaved else capi.ROPE_HALF)
         given = dict(scaling or {})
@@ -271,7 +274,7 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
         raise ValueError("scale is not finite")  # in F32, with log2 e
     max_length = min(max_length, width * pages.page_tokens)
     if workspace is None:
-        need = kv_attention_workspace(pages, rows, heads, max_length)
+        need = _workspace_bytes(pages, rows, heads, max_length)
         if need:
             workspace = pages.key_scales.new_empty(need, dtype=torch.uint8)
     elif workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
@@ -285,6 +288,12 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
 
 def kv_attention_workspace(pages: KvPages, rows: int, q_heads: int, max_length: int) -> int:
     """Bytes of workspace that ``kv_attention`` needs for these sizes (0: none)."""
+    if min(rows, q_heads, max_length) < 0:
+        raise ValueError("rows, q_heads and max_length are not negative")
+    return _workspace_bytes(pages, min(rows, _MOST), min(q_heads, _MOST), min(max_length, _MOST))
+
+
+def _workspace_bytes(pages: KvPages, rows: int, q_heads: int, max_length: int) -> int:
     need = C.c_uint64()
     capi.check(capi.library().hllm_rocm_kv_attention_workspace(pages.address, rows, q_heads, max_length, C.byref(need)))
     return need.value

@@ -379,3 +379,25 @@ def test_a_magnitude_that_f32_does_not_hold_is_refused(magnitude):
     lib, plan = capi.library(), capi.RopePlan(rotary_dimension=5)
     refused(lib.hllm_rocm_rope_plan(C.byref(config(scaling=capi.ROPE_YARN, magnitude=magnitude)), C.byref(plan)), "magnitude")
     assert plan.rotary_dimension == 5
+
+
+def test_numbers_past_the_c_types_do_not_wrap():
+    from types import SimpleNamespace
+
+    from hllm_amd import operators
+
+    for rotary in (-2, (1 << 32) + 64, 1 << 64):
+        with pytest.raises(ValueError):
+            operators.Rope(rotary)
+    c = cache()
+    pages = SimpleNamespace(address=C.addressof(c))
+    need = operators.kv_attention_workspace(pages, 4, 32, 1 << 30)
+    assert need > 0
+    for length in ((1 << 32) - 1, 1 << 32, 1 << 64, (1 << 64) + 5):
+        assert operators.kv_attention_workspace(pages, 4, 32, length) == need
+    for sizes in ((-1, 32, 100), (4, -32, 100), (4, 32, -1), ((1 << 64) - 4, -8, -8)):
+        with pytest.raises(ValueError):
+            operators.kv_attention_workspace(pages, *sizes)
+    for sizes in (((1 << 64) + 4, 32, 100), (4, (1 << 32) + 32, 100)):
+        with pytest.raises(capi.StageError):
+            operators.kv_attention_workspace(pages, *sizes)
