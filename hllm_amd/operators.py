@@ -277,7 +277,8 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
         need = _workspace_bytes(pages, rows, heads, max_length)
         if need:
             workspace = pages.key_scales.new_empty(need, dtype=torch.uint8)
-    elif workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    elif not isinstance(workspace, torch.Tensor) or workspace.device != device or workspace.dtype != torch.uint8 \
+            or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous uint8 on {device}")
     at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     args = ATTENTION_ARGS.pack(rows, page_table.data_ptr(), width, stride, n, max_length,

@@ -801,3 +801,16 @@ def test_cut_groups_of_more_than_sixteen_heads(ops, kind, dtype, dim, q_heads, h
     for lengths in ([5000], [129, 20000, -1, 0, 6400]):
         q, pages, *_ = attend_case(ops, kind, dtype, lengths, q_heads, heads, dim, 32)
         assert cut(ops, pages, lengths, q_heads, max(lengths))
+
+
+def test_workspaces_are_checked(ops):
+    q, pages, table, n, most, out = attend_case(ops, "e4m3", torch.float16, [5000, 50], 8, 2, 128, 64)
+    need = ops.kv_attention_workspace(pages, 2, 8, most)
+    good = torch.empty(need + 64, dtype=torch.uint8, device="cuda")
+    for wrong in (need, good.data_ptr(), b"", good.cpu(), good.view(torch.int8), good[::2]):
+        with pytest.raises(ValueError):
+            ops.kv_attention(q, pages, table, n, most, workspace=wrong)
+    for wrong in (good[:need - 1], good[8:], good[:0]):
+        with pytest.raises(capi.StageError):
+            ops.kv_attention(q, pages, table, n, most, workspace=wrong)
+    assert torch.equal(ops.kv_attention(q, pages, table, n, most, workspace=good[16:]), out)
