@@ -771,8 +771,10 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   for (int e = threadIdx.x; e < vectors * (D / 4); e += kThreads) {
     const int v = e / (D / 4), d = e % (D / 4) * 4;
     float top = -INFINITY, total = 0.0f, held = 0.0f;
+    floatx4 x[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
+      x[w] = reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[(d / DF % 4 * VW + d % DF / 4) * 64 + d / (4 * DF) * 16 + v];
       top = fmaxf(top, states[w][0][v]);
       held += states[w][1][v];
     }
@@ -787,10 +789,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
     const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const floatx4 x = reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[(d / DF % 4 * VW + d % DF / 4) * 64 + d / (4 * DF) * 16 + v];
-      y += x * inverse * (states[w][2][v] * decay[w]);
-    }
+    for (int w = 0; w < 4; ++w) y += x[w] * inverse * (states[w][2][v] * decay[w]);
     const bool undefined = total == 0.0f && held != 0.0f;  // no softmax of scores that are all -inf
     if (parts == 1) {
       store4(out + v * a.out.head + d, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
@@ -804,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   }
 }
 
+__device__ inline float first_lane(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 __device__ inline int2 uniform_cut(const int2* p) {
   return int2{uniform_load(&p->x), uniform_load(&p->y)};
 }
@@ -839,8 +839,9 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
       for (int j = 0; j < kDeep; ++j)
         x[j] = *reinterpret_cast<const floatx4*>(a.part + part_at(a, first, i0 + min(j0 + j * kSlots + slot, n - 1), v) * D + d);
       if (j0 == 0) {
-        for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-        most = fmaxf(most, top);
+        // The first lanes hold the parts: as many steps as those take, and the result from lane 0.
+        for (int o = 1; o < n; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+        most = fmaxf(first_lane(most), top);
         // A part holds nothing where its sum is 0. The maximum does not tell: NaN scores leave it at -inf and
         // the sum NaN, which goes on to the output.
         const float base = most == -INFINITY ? 0.0f : most, before = total * exp2_fast(top - base);
@@ -849,8 +850,8 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
         held |= __any(lane < n && own.y != 0.0f);
         // y is kept divided by the total: means of large values are finite, their sums may not be.
         total = weight;
-        for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-        total += before;
+        for (int o = 1; o < n; o <<= 1) total += __shfl_xor(total, o, 64);
+        total = first_lane(total) + before;
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
         weight *= inverse;
         y *= before * inverse;
@@ -867,7 +868,7 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], o, 64);
   }
-  const bool undefined = total == 0.0f && held;
+  const bool undefined = total == 0.0f && held;  // no softmax of scores that are all -inf
   if (slot == 0) store4(at<T>(a.out, row, head, d), undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
 }
 
