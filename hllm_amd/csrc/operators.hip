@@ -114,9 +114,10 @@ __device__ inline floatx4 decode4(uint32_t w) {
 // ---------------------------------------------------------------- rotary positions
 
 // cos and sin of position x turns, `turns` a 64-bit binary fraction of a turn: the fraction of the
-// product is its low 64 bits, of which the upper 32 are kept (2^-32 turn is 1.5e-9). Reduced to
+// product is its low 64 bits, of which the upper 32 are kept (2^-32 turn is 1.5e-9 radians). Reduced to
 // the nearest quarter turn, |x| <= pi / 4, where the Taylor series to x^9 and x^8 are off by at
-// most 2e-9 and 3e-8.
+// most 2e-9 and 3e-8; with the roundings of x (three of 2^-24, 1.5e-7) and of the sums sine and cosine are
+// right to 5e-7.
 __device__ inline float2 turn(int32_t position, uint64_t turns) {
   const uint32_t lo = (uint32_t)turns, hi = (uint32_t)(turns >> 32), p = (uint32_t)position;
   const uint32_t angle = __umulhi(p, lo) + p * hi - (position < 0 ? lo : 0u);
@@ -134,13 +135,14 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
 // for all heads of the block, and no table is read. In half layout with a rotary
 // dimension of whole sixteens a thread holds both elements of its pairs (eight of either half);
 // interleaved pairs lie beside each other; other half layouts exchange through LDS (kExchange). So
-// every pair is read before it is written and a tensor can be rotated in place. Bound by memory:
-// 4.1 to 4.5 TB/s of 16-bit rows and 5.5 of F32 rows at 42 and 84 MB read and as much written (a copy of
-// 4 GiB reaches 4.8); interleaved 16-bit pairs 3.5 to 4.0, the exchange through LDS 3.0 to 3.7.
+// every pair is read before it is written and a tensor can be rotated in place. Bound by memory (a copy of
+// 4 GiB reaches 4.8 TB/s): 8192 rows of 40 heads of 128 take 41 us in BF16 and 63 in F32, 4.1 and 5.4
+// TB/s; interleaved pairs 44 and 64. The exchange sends every element through LDS as a word, turned or
+// not: 24 of the 128 rotated 50 and 80 us, 3.4 and 4.2 TB/s.
 //
 // F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
 // share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
-// heads of 256: 12.6 us, 4.3 TB/s; 64 rows 4.2 us, one chain of loads, sines, the largest value and the stores.
+// heads of 256: 12.7 us, 4.3 TB/s; 64 rows 4.1 us, one chain of loads, sines, the largest value and the stores.
 template <typename T, int F, bool kExchange>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   __shared__ float2 cs[128];
@@ -320,9 +322,11 @@ __device__ inline void halves4(uint32_t w, half2v& lo, half2v& hi) {
   }
 }
 
-// Copies into LDS as lds_copy16, of cache lines that are not kept: a step reads a layer's cache once
-// (5.4 -> 6.1 TB/s at 3 x 200000 positions, the read probe 6.3; caches that would fit the 256 MB
-// last level and are read again at once lose: 64 rows of 200 to 1000 positions 16.5 -> 18.0 us).
+// Copies into LDS as lds_copy16, of cache lines that are not kept: a step reads a layer's cache once. With nt /
+// without, us, BF16, 8 KV heads of 128, caches not read just before: 3 x 200000 positions 204 / 229 (the first 6.2 TB/s, the
+// read probe 6.3), 64 rows to 8192 43.4 / 49.5, 64 rows of 200 to 1000 18.5 / 20.4; one cache of 67 MB read again and again
+// 17.3 / 17.1. Groups of more than sixteen query heads read a KV head twice, and lose the second reading's hits where
+// the cache is small: groups of 20 over 2 KV heads 17.2 / 16.1 at 17 MB, 30.6 / 29.7 at 50 MB, 112 / 115 at 317 MB.
 __device__ inline void lds_stream16(const void* sbase, uint32_t voffset, uint32_t lds_byte_offset) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -395,7 +399,9 @@ __device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int v)
 // then: one tile a wave, so that 3 workgroups (D = 128) fit a CU. Two tiles a wave and half the workgroups took
 // 31 us where this takes 26 (3 rows of 12000 to 30000 positions), tiles through registers 30. At
 // some hundred positions a row it is bound by the chain of a workgroup's start (length, page numbers, first tile:
-// 2.7 us) and the last round's imbalance: 64 rows to 2048 positions, 66 MB, 18.6 us.
+// 2.7 us) and the last round's imbalance: 64 rows to 2048 positions, 66 MB, 18.9 us. F32 tensors take twice
+// as many products and LDS for twice the queries: 64 rows to 8192 33, 48, 99 us with the join at head dimensions 64, 128,
+// 256, where BF16 takes 29, 43, 76.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kernel(AttendArgs a) {
   using Layout = Tile<D>;
@@ -590,7 +596,9 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   // The weights of a position are 2^(score - m) times its value scale; they enter the products
   // divided by r, and so do the sums o. r is a weight that was the largest once: it follows m, and is
   // raised when a weight is 2^12 times as large, so that o is seldom rescaled and F16 holds
-  // every weight to 2^-11 or to 2^-25 of the largest.
+  // every weight to 2^-11 or to 2^-25 of the largest. One F16 part for 16-bit tensors, whose outputs are
+  // rounded as coarsely: 64 rows to 2048 in F16 are off by 2.4e-4 against 2.1e-4 for the plain form with F32 weights; two parts
+  // took 23.3 -> 24.0 us there, 58.2 -> 59.8 for 256 rows, 30.0 -> 30.5 for 3 long ones.
   floatx4 o[DF];
 #pragma unroll
   for (int f = 0; f < DF; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -811,7 +819,7 @@ __device__ inline int2 uniform_cut(const int2* p) {
 // Joins the parts of the pairs that were cut, one wave for a query head: each part's output weighted
 // with its share of the softmax sum. A part's vector takes D / 4 lanes, so a wave reads up to four parts at
 // once, and eight times as many before it uses them: the kernel is a few memory round trips long (64 rows
-// of 32 heads 4.0 us, 3 rows of up to 30 parts a pair 5.3). A workgroup that joined the parts itself when it was the last
+// of 32 heads 4.0 us, 3 rows of up to 30 parts a pair 4.9). A workgroup that joined the parts itself when it was the last
 // to arrive took 3 to 8 us longer: its stores and counts have to reach the other dies' caches.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
@@ -1305,9 +1313,16 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
   // A workgroup for each pair where rows are short or pairs many: no row has more steps than 5 and 9 for each
   // pair a workgroup of the card. Shares cost 3 to 5 us more (each workgroup sums all rows' steps; the join), and
-  // spare waiting for the longest row. Head dimension 128, 8 KV heads, us with a pair each / with shares:
-  // 64 rows to 1000 positions 16.8 / 21.6, to 2048 23.0 / 21.9; 16 rows to 2048 18.9 / 13.8; 256 rows
-  // 61.0 / 67.0. 128 rows to 8192, head dimension 256: 123 / 61. 7 F32 rows to 903, head dimension 64: 12.3 / 10.5.
+  // spare waiting for the longest row. Us with a pair each / with shares on either side of the line, BF16, 8 KV heads, groups of
+  // 4, lengths log-uniform from 32:
+  //   128: 16 rows to 768 11.8 / 11.8, to 1152 15.3 / 12.8; 64 rows to 1408 20.4 / 20.8, to 1920 24.7 / 22.8;
+  //        256 rows to 1792 53.9 / 54.7, to 2688 71.9 / 70.3, to 3712 92.5 / 85.9, to 5120 117 / 102
+  //   64:  16 rows to 768 9.4 / 10.1, to 1024 11.2 / 10.2; 64 rows to 1152 12.9 / 14.0, to 1664 16.7 / 15.8
+  //   256: 16 rows to 896 18.0 / 16.1; 64 rows to 1280 29.4 / 31.8, to 1792 35.6 / 33.7, to 2432 44.2 / 37.6
+  //   F32, 128: 64 rows to 1408 23.1 / 23.5, to 1920 28.4 / 26.0; F32, 256: 64 rows to 896 36.6 / 36.4, to 1792 53.0 / 46.4
+  // So the crossing lies at the line for some tens of rows, and below it by a third for hundreds (the line loses up to 13%
+  // there) and for F32 heads of 256. Rows that are padding count as pairs, for the host does not know them: 16
+  // rows to 8000 take 21.8, with 48 padding rows 22.0, with 900, where pairs stay whole, 73.
   const uint64_t fit = attend_blocks((int)pages.head_dimension, false);
   const bool whole = steps * fit <= 5 * fit + 9 * pairs;
   p.blocks = pairs;

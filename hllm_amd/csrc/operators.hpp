@@ -67,10 +67,12 @@ struct AttendArgs {
 };
 void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
 
-// Steps (of 128 positions) that starting a pair is counted as: with 1, 2, 3, 4 the shares of 128
-// rows to 8192 positions take 54.8, 56.7, 58.3, 59.7 us.
+// Steps (of 128 positions) that starting a pair is counted as. With 1, 2, 3, 4: 128 rows to 8192 positions of head dimension
+// 256 52.8, 52.7, 53.7, 55.2 us; 32 rows to 4096 of 64 14.6, 15.0, 16.0, 16.1; 64 rows to 8192 of 128 43.5, 43.9, 44.1,
+// 44.9; 16 rows to 2048 of 128 13.6, 13.2, 13.4, 14.2.
 constexpr int kPairCost = 1;
-// Rows whose lengths every workgroup sums to find its share: sixteen a lane.
+// Rows whose lengths every workgroup sums to find its share: sixteen a lane. Past them every pair is whole: a row of 32000
+// positions takes 79 us among 1024 rows of 40, 296 among 1025; rows log-uniform to 8192 539 and 541.
 constexpr uint64_t kMostSharedRows = 1024;
 // Workgroups that the card's 256 CUs hold at once, by LDS (a wave's tile) and registers (about a hundred and
 // D / 2); F32 queries of 256 elements leave room for one on a CU.
