@@ -20,6 +20,7 @@ F32, F16, BF16 = 0, 1, 2
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_UNSCALED, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
 KV_E4M3, KV_INT8 = 0, 1
+KV4_E2M1, KV4_INT4 = 0, 1
 ITEM_SAMPLE, ITEM_TOKEN_FROM_DEVICE, ITEM_LOGPROBS = 1, 2, 4
 STATUS_NAMES = {0: "OK", 1: "INVALID_REQUEST", 2: "INCOMPATIBLE_WORKER", 3: "RESOURCE_EXHAUSTED",
                 4: "DEADLINE_EXCEEDED", 5: "CANCELLED", 6: "INTERNAL"}
@@ -37,7 +38,8 @@ EXPORTS = ("hllm_rocm_last_error", "hllm_rocm_abi_version", "hllm_rocm_stage_cre
            "hllm_rocm_sample_logits_noalloc", "hllm_rocm_device_allocator_metrics",
            "hllm_rocm_device_reset_peak", "hllm_rocm_device_query", "hllm_rocm_measure_mfma_rate",
            "hllm_rocm_rope_plan", "hllm_rocm_rope_apply", "hllm_rocm_kv_append", "hllm_rocm_kv_read",
-           "hllm_rocm_kv_attention", "hllm_rocm_kv_attention_workspace")
+           "hllm_rocm_kv_attention", "hllm_rocm_kv_attention_workspace", "hllm_rocm_kv_attention_by_head",
+           "hllm_rocm_kv4_append", "hllm_rocm_kv4_read", "hllm_rocm_kv4_attention", "hllm_rocm_kv4_attention_workspace")
 NOALLOC_MAX_VOCABULARY = 262144
 
 
@@ -127,6 +129,9 @@ class KvPages(C.Structure):
                 ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p)]
 
 
+Kv4Pages = type("Kv4Pages", (C.Structure,), {"_fields_": KvPages._fields_})  # the same layout
+
+
 class KvAttentionArgs(C.Structure):
     _fields_ = [("rows", C.c_uint64), ("page_table", C.c_void_p), ("table_width", C.c_uint64),
                 ("table_stride", C.c_uint64), ("lengths", C.c_void_p), ("max_length", C.c_uint64),
@@ -197,7 +202,12 @@ def library() -> C.CDLL:
     L.hllm_rocm_kv_append.argtypes = [i32, vp, vp, vp, u64, vp, vp, vp, vp, vp, vp]
     L.hllm_rocm_kv_read.argtypes = [i32, vp, vp, vp, u64, vp, vp]
     L.hllm_rocm_kv_attention.argtypes = [i32, vp, vp, vp]
+    L.hllm_rocm_kv_attention_by_head.argtypes = [i32, vp, vp, vp, u64]
     L.hllm_rocm_kv_attention_workspace.argtypes = [vp, u64, u32, u64, vp]
+    L.hllm_rocm_kv4_append.argtypes = L.hllm_rocm_kv_append.argtypes
+    L.hllm_rocm_kv4_read.argtypes = L.hllm_rocm_kv_read.argtypes
+    L.hllm_rocm_kv4_attention.argtypes = L.hllm_rocm_kv_attention_by_head.argtypes
+    L.hllm_rocm_kv4_attention_workspace.argtypes = L.hllm_rocm_kv_attention_workspace.argtypes
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is C.c_int or (fn.restype is None and name != "hllm_rocm_stage_destroy"):

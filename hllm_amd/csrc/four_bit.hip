@@ -1,0 +1,534 @@
+// Kernels over the 4-bit paged cache: its vectors read back, and one new token's attention over it. (Rows are written by
+// the rotation's kernel.)
+#include <algorithm>
+#include <atomic>
+
+#include "operators_device.hpp"
+
+namespace hllm_rocm {
+namespace {
+
+// ---------------------------------------------------------------- codes
+
+// Eight codes of a word as F16, which holds every code exactly: E2M1 in order, INT4 with code i beside i + 4.
+template <int F>
+__device__ inline half8 halves8(uint32_t w) {
+  half2v x[4];
+  if constexpr (F == kE2m1) {
+    x[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0);
+    x[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1);
+    x[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2);
+    x[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3);
+  } else {
+    x[0] = low_halves(w);
+    x[1] = high_halves(w);
+    x[2] = low_halves(w >> 8);
+    x[3] = high_halves(w >> 8);
+  }
+  return half8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+}
+
+// ---------------------------------------------------------------- reading back
+
+// A thread reads the codes of sixteen bytes of output of a key, and of the value beside it, and writes them. A value's
+// codes lie G bytes apart (two elements of each group beside each other), in a line that the wave reads whole.
+template <typename T, int F, int D>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
+  constexpr int kCodes = 16 / sizeof(T), L = D / kCodes, G = D / 32;
+  const Pages& c = a.pages;
+  const uint32_t per_row = (uint32_t)c.kv_heads * L;
+  const uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+  const uint64_t row = unit / per_row;
+  if (row >= (uint64_t)a.rows) return;
+  const int in_row = (int)(unit - row * per_row), h = in_row / L, d = in_row % L * kCodes, g = d / 32;
+  const int slot = a.slots[row];
+  if (slot < 0 || (slot >> c.page_shift) >= c.pages) return;
+  const int page = slot >> c.page_shift, offset = slot & ((1 << c.page_shift) - 1);
+  const uint64_t from = (uint64_t)page * c.page_stride + (uint64_t)offset * c.token_stride + (uint64_t)h * c.head_stride;
+  const uint64_t scale_at = ((((uint64_t)page * c.kv_heads + h) << c.page_shift) + offset) * G + g;
+  uint32_t codes[2] = {0, 0};
+  if constexpr (kCodes == 8)
+    codes[0] = *reinterpret_cast<const uint32_t*>(c.keys + from + d / 2);
+  else
+    codes[0] = *reinterpret_cast<const uint16_t*>(c.keys + from + d / 2);
+#pragma unroll
+  for (int i = 0; i < kCodes / 2; ++i) codes[1] |= (uint32_t)c.values[from + G * (d % 32 / 2 + i) + g] << (8 * i);
+  float scale[2];
+  if constexpr (F == kE2m1) {
+    scale[0] = scale_of<F>(static_cast<const uint8_t*>(c.key_scales)[scale_at]);
+    scale[1] = scale_of<F>(static_cast<const uint8_t*>(c.value_scales)[scale_at]);
+  } else {
+    scale[0] = scale_of<F>(static_cast<const uint16_t*>(c.key_scales)[scale_at]);
+    scale[1] = scale_of<F>(static_cast<const uint16_t*>(c.value_scales)[scale_at]);
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    T* to = at<T>(which ? a.v : a.k, (int)row, h, d);
+    float x[8];
+    values8<F>(codes[which], x);
+    if constexpr (kCodes == 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= scale[which];
+      store8(to, x);
+    } else {
+      store4(to, floatx4{x[0], x[1], x[2], x[3]} * scale[which]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+
+// A wave's tile of N positions in LDS: the codes of keys and of values, then their scales as F32 numbers, each group's N
+// scales together, and each position's largest value scale. A position lies in slot `slot` and a row's
+// sixteen-byte chunks are permuted (chunk k at k ^ swizzle), so that the rows that are read at once, of four eights of
+// positions, lie in different banks, keys and values alike.
+template <int D>
+struct Tile4 {
+  static constexpr int N = kAttend4Tile<D>, kRow = D / 2, kChunks = kRow / 16, G = D / 32;
+  static constexpr int kCodes = N * kRow, kScales = 2 * kCodes, kLargest = kScales + 2 * G * N * 4;
+  static constexpr int kBytes = (std::max(kLargest + N * 4, 64 * D) + 255) / 256 * 256, kBlock = kThreads / 64 * kBytes;
+  static constexpr int kGroups = N / 8;   // eights of positions, each in one page
+  static constexpr int kCopies = kCodes / 1024;
+  static constexpr int kHalf = 4 * kRow;  // from a slot of the first thirty-two positions to that of the next
+  static __device__ int slot(int eight, int offset) {
+    return offset * kGroups + (D == 64 ? eight ^ (offset >> 1 & 1) << 2 : eight);
+  }
+  static __device__ int swizzle(int eight, int offset) {
+    return D == 64 ? offset & 1 : D == 128 ? offset & 3 : (offset & 3) | (eight >> 1) << 2;
+  }
+  // Byte `b` of the row of one of the first thirty-two positions, or of the one `half` = kHalf s bytes on.
+  static __device__ int at(int eight, int offset, int b, int half) {
+    const int first = slot(eight, offset) * kRow + ((b / 16 ^ swizzle(eight, offset)) * 16) + b % 16;
+    return D == 64 ? first ^ half : first + half;
+  }
+};
+
+// As kv_attention_kernel (operators.hip): a pair's scores S = K Q^T and sums O^T = V^T P are products on the matrix units,
+// with the softmax's running maximum and sum in F32. What differs comes from the scales that 32 elements of a
+// vector share. A 16 x 16 x 32 product takes one group of sixteen keys, and its sums are multiplied by the keys' scales of that group
+// in F32; a value's scales enter the weights, which are made for each group by itself. So codes enter the
+// products exactly (as F16 numbers), and no element is multiplied by its scale. A key's codes lie in order: a
+// lane's word is eight elements of one group. A value's codes lie so that a lane's bytes of a position are two elements of each
+// group: the sixteen rows of an output fragment have one group.
+template <typename T, int F, int D>
+__global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_kernel(AttendArgs a) {
+  using Layout = Tile4<D>;
+  constexpr int N = Layout::N, G = Layout::G, H = N / 32, kStep = 4 * N;
+  constexpr int W = (G + 3) / 4;             // words of a lane's value bytes of a position
+  constexpr int SB = F == kE2m1 ? G : 2 * G; // scale bytes of a position
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // F16 parts of a query element and of a weight
+  constexpr bool kBoth = N == 32;            // a lane holds a position's key or value scales, not both
+  extern __shared__ __attribute__((aligned(256))) char smem[];
+  __shared__ float states[4][3][16];
+  __shared__ half8 queries[P][G][64];
+
+  const Pages& c = a.pages;
+  const int KVH = c.kv_heads, shift = c.page_shift, in_row = KVH * a.head_groups;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int quad = lane >> 4, col = lane & 15;
+  const int me = blockIdx.x;
+  Share<kStep> share;
+  if (!share.first_pair(a, in_row, me, lane)) return;
+
+  bool again = false;
+  for (bool more = true; more; more = share.next_pair(a, in_row)) {
+  const int row = share.row, kvg = share.kvg, length = share.length;
+  // This share's steps of the pair, low .. high - 1, and the workgroups that have others.
+  const int steps = steps_of<kStep>(length), first_unit = share.start + kPairCost;
+  const int low = max(share.from - first_unit, 0), high = min(steps, share.to - first_unit);
+  if (steps > 0 ? low >= high : share.start < share.from) continue;  // only the cost of starting it is this share's
+  const int first = first_unit / share.budget;
+  const int parts = a.shared && steps > 0 ? (first_unit + steps - 1) / share.budget - first + 1 : 1;
+  const int kvh = kvg / a.head_groups, g0 = (kvg - kvh * a.head_groups) * 16;
+  const int begin = kStep * low, end = min(length, kStep * high);
+  if (again) __syncthreads();  // the workgroup has read the last pair's sums
+  again = true;
+  const int vectors = min(16, a.group - g0);
+
+  const int32_t* table = a.table + (uint64_t)row * a.table_stride + (uint64_t)kvh * a.table_head;
+  const int mask = (1 << shift) - 1;
+  const uint32_t token = c.token_stride;
+  char* tile = smem + wave * Layout::kBytes;
+  const uint32_t tile_at = (uint32_t)(size_t)((__attribute__((address_space(3))) char*)smem) + wave * Layout::kBytes;
+
+  // A lane's share of the copies: chunks of the positions `offset` (+ a step for each copy) of one eight. Copy i's
+  // first lane has slot 64 i / kChunks.
+  constexpr int kPer = 64 / Layout::kChunks;  // slots of a copy
+  const int s0 = lane / Layout::kChunks, offset0 = s0 / Layout::kGroups;
+  const int eight = s0 % Layout::kGroups ^ (D == 64 ? (offset0 >> 1 & 1) << 2 : 0);
+  constexpr int kOffsets = kPer / Layout::kGroups;  // 2 or 4 positions of each eight
+  const uint8_t* keys = c.keys + (uint64_t)kvh * c.head_stride + (uint64_t)offset0 * token;
+  const uint64_t values_at = (uint64_t)(c.values - c.keys);
+  // Its scales: of position lane (N = 64), or of position lane % 32, the keys' or the values'.
+  const int own = lane & (N - 1);
+  const uint8_t* scales = static_cast<const uint8_t*>(kBoth && lane >= 32 ? c.value_scales : c.key_scales);
+  const uint64_t value_scales_at = static_cast<const uint8_t*>(c.value_scales) - static_cast<const uint8_t*>(c.key_scales);
+
+  // The page of the lane's scales' position (of the last position's page behind the part).
+  const auto page_of = [&](int t) { return table[min(t + (own & ~7), end - 1) >> shift]; };
+  uint32_t held[2][SB > 4 ? SB / 4 : 1];  // scales as they are held, of the next tile
+  const auto load_scales = [&](uint32_t* to, const uint8_t* from) {
+    if constexpr (SB == 2) to[0] = *reinterpret_cast<const uint16_t*>(from);
+    if constexpr (SB == 4) to[0] = *reinterpret_cast<const uint32_t*>(from);
+    if constexpr (SB == 8) {
+      const uint2v w = *reinterpret_cast<const uint2v*>(from);
+      to[0] = w[0], to[1] = w[1];
+    }
+    if constexpr (SB == 16) {
+      const uint4v w = *reinterpret_cast<const uint4v*>(from);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = w[i];
+    }
+  };
+  // Starts a tile's copies and loads its scales; returns a bit for each eight whose page is not there.
+  const auto copy_tile = [&](int t, int id) {
+    const bool there = id >= 0 && id < c.pages;
+    const uint64_t absent = __ballot(!there);
+    const int page = there ? id : 0;
+    const int from_page = __shfl(page, eight * 8, 64);
+    const uint8_t* from = keys + (uint64_t)(uint32_t)from_page * c.page_stride + (uint64_t)(uint32_t)((t + 8 * eight) & mask) * token;
+#pragma unroll
+    for (int i = 0; i < Layout::kCopies; ++i) {
+      const int chunk = (lane % Layout::kChunks) ^ Layout::swizzle(eight, offset0 + i * kOffsets);
+      const uint8_t* at = from + (uint64_t)(i * kOffsets) * token + chunk * 16;
+      lds_stream16_at(at, tile_at + i * 1024);
+      lds_stream16_at(at + values_at, tile_at + Layout::kCodes + i * 1024);
+    }
+    const uint8_t* at = scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + own) & mask)) * SB;
+    load_scales(held[0], at);
+    if constexpr (!kBoth) load_scales(held[1], at + value_scales_at);
+    int missing = 0;
+#pragma unroll
+    for (int e = 0; e < Layout::kGroups; ++e) missing |= (int)(absent >> (8 * e) & 1) << e;
+    return missing;
+  };
+
+  int t = begin + N * wave, missing = 0, id = 0;
+  if (t < end) {
+    missing = copy_tile(t, page_of(t));
+    id = page_of(min(t + kStep, end - 1));
+  }
+
+  // Q^T as the B operand, kept in LDS for the four waves: group g's lane (col, quad) holds elements 32 g + 8 quad + j in the order of
+  // halves8. Each vector is divided by the power of two of its largest element, which puts F32 and BF16
+  // ranges into F16's and goes back into its scores.
+  float factor, factor_lo;
+  {
+    float x[G][8];
+    const T* src = at<const T>(a.q, row, kvh * a.group + g0 + min(col, vectors - 1), 8 * quad);
+    uint32_t most = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      load8(src + 32 * g, x[g]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(x[g][j]) & 0x7fffffffu);
+    }
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+    // 2^e <= largest < 2^(e+1), e at most 126 (the largest numbers are left below 4); vectors that are
+    // zero, below the normal range or not finite as they are.
+    const uint32_t exponent = min(most >> 23, 253u);
+    const bool usual = exponent >= 1 && most < 0x7f800000u;
+    const float down = usual ? __uint_as_float((254u - exponent) << 23) : 1.0f;
+    const float up = usual ? __uint_as_float(exponent << 23) : 1.0f;
+    factor = a.scale_hi * up;
+    factor_lo = a.scale_lo * up;
+    if (wave == 0) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        half8 part[P];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = x[g][F == kE2m1 ? j : (j >> 1) + 4 * (j & 1)] * down;
+          part[0][j] = (_Float16)y;
+          if constexpr (P == 2) part[1][j] = (_Float16)(y - (float)part[0][j]);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) queries[p][g][lane] = part[p];
+      }
+    }
+  }
+  __syncthreads();
+
+  // Weights, their scaling by r and the sums o as in kv_attention_kernel, r by each position's largest value scale.
+  // o[2 g + e]'s row c is element 32 g + 2 c + e.
+  floatx4 o[2 * G];
+#pragma unroll
+  for (int f = 0; f < 2 * G; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f, r = 0.0f;
+  bool any = false;  // whether the wave has had a position
+  float* key_scale = reinterpret_cast<float*>(tile + Layout::kScales);
+  float* value_scale = key_scale + G * N;
+  float* largest_scale = reinterpret_cast<float*>(tile + Layout::kLargest);
+
+  for (; t < end; t += kStep) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int gone = missing;
+    const bool whole = gone == 0 && t + N <= end;
+    any |= gone != (1 << Layout::kGroups) - 1;  // eights behind the end count as the last one's page
+    {
+      // The lane's scales as F32 numbers; positions past the part and in pages that are not there have none.
+      const bool counts = whole || (t + own < end && !(gone >> (own >> 3) & 1));
+      const auto keep = [&](const uint32_t* raw, float* to) {
+        float most = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t w = F == kE2m1 ? raw[g / 4] >> (8 * (g % 4)) & 255u : raw[g / 2] >> (16 * (g % 2)) & 0xffffu;
+          const float s = counts ? scale_of<F>(w) : 0.0f;
+          to[g * N] = s;
+          most = fmaxf(most, fabsf(s));  // NaN is not taken
+        }
+        return most;
+      };
+      if constexpr (kBoth) {
+        const float most = keep(held[0], (lane < 32 ? key_scale : value_scale) + own);
+        if (lane >= 32) largest_scale[own] = most;
+      } else {
+        keep(held[0], key_scale + own);
+        largest_scale[own] = keep(held[1], value_scale + own);
+      }
+    }
+    // The tile's positions in thirty-twos, one after the other.
+#pragma unroll 1
+    for (int s = 0; s < H; ++s) {
+      // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are positions 8 quad .. + 7, which are
+      // also its slots of the value products.
+      float d[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const int half = s * Layout::kHalf;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        half8 q[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) q[p] = queries[p][g][lane];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const half8 k = halves8<F>(*reinterpret_cast<const uint32_t*>(
+              tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
+          floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) x = mfma(k, q[p], x);
+          const floatx4 by = *reinterpret_cast<const floatx4*>(key_scale + g * N + 32 * s + 8 * quad + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[4 * h + i] = fmaf(x[i], by[i], d[4 * h + i]);
+        }
+      }
+      uint32_t vw[8][W];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const char* line = tile + Layout::kCodes + Layout::at(quad, j, G * col, half);
+        if constexpr (G == 2) vw[j][0] = *reinterpret_cast<const uint16_t*>(line);
+        if constexpr (G == 4) vw[j][0] = *reinterpret_cast<const uint32_t*>(line);
+        if constexpr (G == 8) {
+          const uint2v w = *reinterpret_cast<const uint2v*>(line);
+          vw[j][0] = w[0];
+          vw[j][1] = w[1];
+        }
+      }
+      // The tile is in registers: the next one's copies start.
+      if (s == H - 1 && t + kStep < end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        missing = copy_tile(t + kStep, id);
+        id = page_of(min(t + 2 * kStep, end - 1));
+      }
+      // F32 tensors keep the scores' factor as a sum of two floats and round a score once, after the maximum is taken away.
+      float sc[8], by_lo[8], most = -INFINITY;
+      const int valid = whole ? 8 : gone >> (4 * s + quad) & 1 ? 0 : end - (t + 32 * s + 8 * quad);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sc[j] = d[j] * factor;
+        if constexpr (P == 2)
+          by_lo[j] = j >= valid || sc[j] == -INFINITY ? 0.0f : fmaf(d[j], factor, -sc[j]) + d[j] * factor_lo;
+        sc[j] = j < valid ? sc[j] : -INFINITY;
+        most = fmaxf(most, sc[j]);
+      }
+      const float m_new = fmaxf(m, column_max(most));
+      const float base = m_new == -INFINITY ? 0.0f : m_new;
+      const float decay = exp2_fast(m - base);
+      float weight[8], ls[8], sum = 0.0f, largest = 0.0f;
+      load8(largest_scale + 32 * s + 8 * quad, ls);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        weight[j] = exp2_fast(P == 2 ? (sc[j] - base) + by_lo[j] : sc[j] - base);
+        sum += weight[j];
+        largest = fmaxf(largest, weight[j] * ls[j]);
+      }
+      l = l * decay + sum;
+      m = m_new;
+      r *= decay;
+      largest = column_max(largest);
+      if (__any(largest > 4096.0f * r)) {
+        const float raised = fmaxf(r, largest), rescale = raised > r ? r / raised : 1.0f;
+#pragma unroll
+        for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
+        r = raised;
+      }
+      const float over = r > 0x1p-125f ? __builtin_amdgcn_rcpf(r) : 0.0f;  // smaller weights are nothing
+#pragma unroll
+      for (int j = 0; j < 8; ++j) weight[j] *= over;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        // Two positions' codes are paired. E2M1: pairs[e] holds code e (of two) of both in each group's byte; INT4: pairs[k] both
+        // positions' bytes of groups 2 k and 2 k + 1.
+        uint32_t pairs[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = vw[2 * j][w], y = vw[2 * j + 1][w];
+          if constexpr (F == kE2m1) {
+            pairs[0][j] = (x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u);
+            pairs[1][j] = (x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u);
+          } else {
+            pairs[0][j] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+            pairs[1][j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+          }
+        }
+#pragma unroll
+        for (int gw = 0; gw < (G < 4 ? G : 4); ++gw) {
+          const int g = 4 * w + gw;
+          float vs[8];
+          load8(value_scale + g * N + 32 * s + 8 * quad, vs);
+          half8 pf[P];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float x = weight[j] * vs[j];
+            // As a value of its own: rounded with the product in one step, the first part would differ
+            // from the one that the second part is the rest of.
+            if constexpr (P == 2) asm("" : "+v"(x));
+            pf[0][j] = (_Float16)x;
+            if constexpr (P == 2) pf[1][j] = (_Float16)(x - (float)pf[0][j]);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            half8 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              half2v x;
+              if constexpr (F == kE2m1) {
+                x = gw == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(pairs[e][j], 1.0f, 0)
+                    : gw == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(pairs[e][j], 1.0f, 1)
+                    : gw == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(pairs[e][j], 1.0f, 2)
+                              : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(pairs[e][j], 1.0f, 3);
+              } else {
+                const uint32_t two = gw & 1 ? pairs[gw >> 1][j] >> 8 : pairs[gw >> 1][j];
+                x = e ? high_halves(two) : low_halves(two);
+              }
+              v[2 * j] = x[0];
+              v[2 * j + 1] = x[1];
+            }
+#pragma unroll
+            for (int p = P - 1; p >= 0; --p) o[2 * g + e] = mfma(v, pf[p], o[2 * g + e]);
+          }
+        }
+      }
+    }
+  }
+
+  // The four waves' states meet in LDS, each wave's in its own tile.
+  l = column_sum(l);
+  // Only scores of -inf (an infinite query's): a sum that is not 0 beside that maximum tells them from no positions.
+  if (any && l == 0.0f) l = 1.0f;
+  if (quad == 0) {
+    states[wave][0][col] = m;
+    states[wave][1][col] = l;
+    states[wave][2][col] = r;
+  }
+  static_assert(Layout::kBytes >= 64 * D, "a wave's sums lie in its tile");
+  // Components 2 k and 2 k + 1 of a group's two fragments: four elements that follow one another.
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      reinterpret_cast<floatx4*>(tile)[(2 * g + k) * 64 + lane] =
+          floatx4{o[2 * g][2 * k], o[2 * g + 1][2 * k], o[2 * g][2 * k + 1], o[2 * g + 1][2 * k + 1]};
+  __syncthreads();
+  T* out = at<T>(a.out, row, kvh * a.group + g0, 0);
+  if (a.cuts && low == 0 && threadIdx.x == 0) a.cuts[row * in_row + kvg] = int2{first, parts};
+  for (int e = threadIdx.x; e < vectors * (D / 4); e += kThreads) {
+    const int v = e / (D / 4), dim = e % (D / 4) * 4;
+    const int from = ((dim / 32 * 2 + dim / 4 % 2) * 64 + dim % 32 / 8 * 16) + v;
+    float top = -INFINITY, total = 0.0f, sums = 0.0f;
+    floatx4 x[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      x[w] = reinterpret_cast<const floatx4*>(smem + w * Layout::kBytes)[from];
+      top = fmaxf(top, states[w][0][v]);
+      sums += states[w][1][v];
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+    float decay[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      decay[w] = exp2_fast(states[w][0][v] - base);
+      total += states[w][1][v] * decay[w];
+    }
+    // Divided by the total before r's share of a value scale enters: a mean of large values is finite, their sum may not be.
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    floatx4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) y += x[w] * inverse * (states[w][2][v] * decay[w]);
+    const bool undefined = total == 0.0f && sums != 0.0f;  // no softmax of scores that are all -inf
+    if (parts == 1) {
+      store4(out + v * a.out.head + dim, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
+    } else {
+      if (undefined) total = 1.0f;  // NaN in the join, unless another part has finite scores
+      const uint64_t part = part_at(a, first, me - first, v);
+      *reinterpret_cast<floatx4*>(a.part + part * D + dim) = y;
+      if (dim == 0) *reinterpret_cast<float2*>(a.stats + 2 * part) = float2{top, total};
+    }
+  }
+  }
+}
+
+template <typename T, int F>
+void kv4_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
+  const uint64_t units = (uint64_t)a.rows * a.pages.kv_heads * (head_dim * sizeof(T) / 16);
+  const unsigned blocks = (unsigned)((units + kThreads - 1) / kThreads);
+  if (head_dim == 64) kv4_read_kernel<T, F, 64><<<blocks, kThreads, 0, stream>>>(a);
+  if (head_dim == 128) kv4_read_kernel<T, F, 128><<<blocks, kThreads, 0, stream>>>(a);
+  if (head_dim == 256) kv4_read_kernel<T, F, 256><<<blocks, kThreads, 0, stream>>>(a);
+}
+
+template <typename T, int F, int D>
+void attend4(hipStream_t stream, const AttendArgs& a) {
+  constexpr int kLds = Tile4<D>::kBlock;
+  static std::atomic<uint64_t> asked{0};
+  ask_for_lds(reinterpret_cast<const void*>(&kv4_attention_kernel<T, F, D>), kLds, asked);
+  kv4_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);
+}
+
+template <typename T, int F>
+void attend4_dim(hipStream_t stream, int head_dim, const AttendArgs& a) {
+  if (head_dim == 64) attend4<T, F, 64>(stream, a);
+  if (head_dim == 128) attend4<T, F, 128>(stream, a);
+  if (head_dim == 256) attend4<T, F, 256>(stream, a);
+}
+
+template <typename F>
+void by_dtype(uint32_t dtype, F&& run) {
+  if (dtype == HLLM_DTYPE_F16) return run(_Float16{});
+  if (dtype == HLLM_DTYPE_BF16) return run(bhalf{});
+  run(0.0f);
+}
+
+}  // namespace
+
+void launch_kv4_read(hipStream_t stream, uint32_t dtype, int format, int head_dim, const ReadArgs& a) {
+  by_dtype(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    if (format == kE2m1)
+      kv4_read<T, kE2m1>(stream, head_dim, a);
+    else
+      kv4_read<T, kInt4>(stream, head_dim, a);
+  });
+}
+
+void launch_kv4_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a) {
+  by_dtype(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    if (format == kE2m1)
+      attend4_dim<T, kE2m1>(stream, head_dim, a);
+    else
+      attend4_dim<T, kInt4>(stream, head_dim, a);
+  });
+}
+
+}  // namespace hllm_rocm

@@ -1,76 +1,17 @@
 // Operators on a caller's device memory: rotary positions, the 8-bit paged KV cache (written and
 // read back), and one new token's attention over it. The C entry points are at the end.
-#include "operators.hpp"
-
 #include <algorithm>
 #include <atomic>
-#include <climits>
 #include <cmath>
 #include <type_traits>
 
-#include "abi.hpp"
+#include "operators_check.hpp"
+#include "operators_device.hpp"
 
 namespace hllm_rocm {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr double kLog2e = 1.4426950408889634;
-
-typedef __bf16 bhalf;
-typedef bhalf bhalf4 __attribute__((ext_vector_type(4)));
-typedef bhalf bhalf8 __attribute__((ext_vector_type(8)));
-typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
-typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-
-// ---------------------------------------------------------------- eight values
-
-__device__ inline void load8(const _Float16* p, float* x) {
-  const half8 h = *reinterpret_cast<const half8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
-}
-__device__ inline void load8(const bhalf* p, float* x) {
-  const bhalf8 h = *reinterpret_cast<const bhalf8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
-}
-__device__ inline void load8(const float* p, float* x) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const floatx4 h = *reinterpret_cast<const floatx4*>(p + 4 * j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[4 * j + i] = h[i];
-  }
-}
-__device__ inline void store8(_Float16* p, const float* x) {
-  half8 h;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
-  *reinterpret_cast<half8*>(p) = h;
-}
-__device__ inline void store4(_Float16* p, floatx4 x) {
-  *reinterpret_cast<half4*>(p) = half4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-}
-__device__ inline void store4(bhalf* p, floatx4 x) {
-  *reinterpret_cast<bhalf4*>(p) = bhalf4{(bhalf)x[0], (bhalf)x[1], (bhalf)x[2], (bhalf)x[3]};
-}
-__device__ inline void store4(float* p, floatx4 x) { *reinterpret_cast<floatx4*>(p) = x; }
-__device__ inline void store8(bhalf* p, const float* x) {
-  bhalf8 h;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = (bhalf)x[i];
-  *reinterpret_cast<bhalf8*>(p) = h;
-}
-__device__ inline void store8(float* p, const float* x) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) *reinterpret_cast<floatx4*>(p + 4 * j) = floatx4{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
-}
-
-template <typename T>
-__device__ inline T* at(const Strided& s, int row, int head, int d) {
-  return static_cast<T*>(s.data) + (uint64_t)row * s.row + (uint64_t)head * s.head + d;
-}
 
 // ---------------------------------------------------------------- 8-bit codes
 
@@ -96,6 +37,39 @@ __device__ inline uint2v encode8(const float* x, float inverse) {
       }
       w[j] = c;
     }
+  }
+  return w;
+}
+
+// Eight elements' 4-bit codes and their group's scale as it is held; `most`: the bits of the group's largest magnitude. A group with a
+// value that is not finite has codes of 0 and the scale NaN.
+template <int F>
+__device__ inline uint32_t encode_four(const float* x, uint32_t most, uint32_t& held) {
+  const bool finite = most < 0x7f800000u;
+  most = max(most, 27u << 23);  // 2^-100
+  uint32_t w = 0;
+  if constexpr (F == kE2m1) {
+    // The smallest power of two that leaves the largest magnitude at most 7, which is as near to the largest code, 6, as a
+    // value inside may be to its code; 2^125 at most, so that every code's value is finite.
+    const uint32_t byte = min(((most + 0x1fffffu) >> 23) - 2, 252u);
+    const float down = __uint_as_float((254u - byte) << 23);
+    held = finite ? byte : 255u;
+    if (!finite) return 0;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(x[i] * down, -6.0f), 6.0f);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
+  } else {
+    // A seventh of the largest magnitude, its lower half cut off: the largest code's value is not above it.
+    const uint32_t scale = __float_as_uint(__uint_as_float(most) / 7.0f) & 0xffff0000u;
+    const float inverse = 1.0f / __uint_as_float(scale);
+    held = finite ? scale >> 16 : 0x7fc0u;
+    if (!finite) return 0x88888888u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= (uint32_t)((int)fminf(fmaxf(rintf(x[i] * inverse), -7.0f), 7.0f) + 8) << (4 * i);
   }
   return w;
 }
@@ -143,6 +117,61 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
 // F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
 // share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
 // heads of 256: 12.7 us, 4.3 TB/s; 64 rows 4.1 us, one chain of loads, sines, the largest value and the stores.
+// The last part for a 4-bit cache, of every thread of the workgroup. A group's 32 elements lie with two to four lanes, which depends
+// on the rotation's layout, so they meet in LDS: each eight's largest magnitude, then the
+// codes, which are written from there in whole words.
+template <int F>
+__device__ inline void append_four(const RotateArgs& a, const float* x, int slot, bool cached, bool is_v, int in_block, int u,
+                                   int h, int d0, int d1) {
+  __shared__ uint32_t eight_most[2 * kThreads], staged[2 * kThreads];
+  const Pages& c = a.pages;
+  const int G = a.lanes / 2;
+  uint32_t* most_of = eight_most + in_block * 2 * a.lanes;
+  uint32_t* codes = staged + in_block * 2 * a.lanes;
+  if (cached) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      // The bits of magnitudes order as the magnitudes, infinities and NaN above all others.
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[8 * k + i]) & 0x7fffffffu);
+      most_of[(k ? d1 : d0) / 8] = most;
+    }
+  }
+  __syncthreads();
+  const int page = slot >> c.page_shift, offset = slot & ((1 << c.page_shift) - 1);
+  if (cached) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int d = k ? d1 : d0, g = d / 32;
+      const uint32_t* of = most_of + 4 * g;
+      const uint32_t most = max(max(of[0], of[1]), max(of[2], of[3]));
+      const uint64_t scale_at = ((((uint64_t)page * c.kv_heads + h) << c.page_shift) + offset) * G + g;
+      uint32_t held;
+      const uint32_t w = encode_four<F>(x + 8 * k, most, held);
+      if (d % 32 == 0) {
+        void* scales = is_v ? c.value_scales : c.key_scales;
+        if constexpr (F == kE2m1)
+          static_cast<uint8_t*>(scales)[scale_at] = (uint8_t)held;
+        else
+          static_cast<uint16_t*>(scales)[scale_at] = (uint16_t)held;
+      }
+      if (is_v) {
+        uint8_t* to = reinterpret_cast<uint8_t*>(codes) + G * (d % 32 / 2) + g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[G * i] = (uint8_t)(w >> (8 * i));
+      } else {
+        codes[d / 8] = w;
+      }
+    }
+  }
+  __syncthreads();
+  if (!cached) return;
+  uint8_t* to = (is_v ? c.values : c.keys) + (uint64_t)page * c.page_stride + (uint64_t)offset * c.token_stride +
+                (uint64_t)h * c.head_stride + 8 * u;
+  *reinterpret_cast<uint2v*>(to) = uint2v{codes[2 * u], codes[2 * u + 1]};
+}
+
 template <typename T, int F, bool kExchange>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   __shared__ float2 cs[128];
@@ -178,8 +207,9 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
     for (int i = 0; i < 16; ++i) xs[t * 17 + i] = active ? x[i] : 0.0f;
   }
   __syncthreads();
-  if (!active) return;
-  if (!is_v) {
+  constexpr bool kFour = F >= kE2m1;
+  if (!kFour && !active) return;
+  if (active && !is_v) {
     if constexpr (kExchange) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -211,13 +241,15 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
       }
     }
   }
-  if (F < 0 || is_q) {
+  if (F < 0 || (is_q && active)) {
     const Strided& out = is_q ? a.q_out : a.k_out;
     store8(at<T>(out, row, h, d0), x);
     store8(at<T>(out, row, h, d1), x + 8);
-    return;
+    if constexpr (!kFour) return;
   }
-  if constexpr (F >= 0) {
+  if constexpr (kFour) {
+    append_four<F>(a, x, slot, active && !is_q, is_v, in_block, u, h, d0, d1);
+  } else if constexpr (F >= 0) {
     // The bits of magnitudes order as the magnitudes, infinities and NaN above all others.
     uint32_t most = 0;
 #pragma unroll
@@ -237,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
     *reinterpret_cast<uint2v*>(to + d0) = encode8<F>(x, inverse);
     *reinterpret_cast<uint2v*>(to + d1) = encode8<F>(x + 8, inverse);
     if (u == 0) {
-      float* scales = is_v ? c.value_scales : c.key_scales;
+      float* scales = static_cast<float*>(is_v ? c.value_scales : c.key_scales);
       scales[(((uint64_t)page * c.kv_heads + h) << c.page_shift) + offset] = finite ? largest / kPeak<F> : NAN;
     }
   }
@@ -269,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
     codes[0][j] = reinterpret_cast<const uint32_t*>(c.keys + from)[j];
     codes[1][j] = reinterpret_cast<const uint32_t*>(c.values + from)[j];
   }
-  const float scale[2] = {c.key_scales[scale_at], c.value_scales[scale_at]};
+  const float scale[2] = {static_cast<const float*>(c.key_scales)[scale_at], static_cast<const float*>(c.value_scales)[scale_at]};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T* to = at<T>(which ? a.v : a.k, (int)row, h, d);
@@ -290,23 +322,6 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
 
 // ---------------------------------------------------------------- attention
 
-__device__ inline floatx4 mfma(half8 a, half8 b, floatx4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// The largest of a value over the four lanes of a column (lanes 16 apart), with the row swaps
-// of the vector unit: shuffles through LDS cost 0.1 us a tile more.
-__device__ inline float column_max(float v) {
-  const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(half[0]), __uint_as_float(half[1]));
-  const auto row = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(row[0]), __uint_as_float(row[1]));
-}
-__device__ inline float column_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
-}
-
 // Four codes as F16, which holds every code of either format exactly. INT8: with the sign bit
 // turned over, the byte below 0x64 is the F16 number 1024 + 128 + code.
 template <int F>
@@ -322,35 +337,6 @@ __device__ inline void halves4(uint32_t w, half2v& lo, half2v& hi) {
   }
 }
 
-// Copies into LDS as lds_copy16, of cache lines that are not kept: a step reads a layer's cache once. With nt /
-// without, us, BF16, 8 KV heads of 128, caches not read just before: 3 x 200000 positions 204 / 229 (the first 6.2 TB/s, the
-// read probe 6.3), 64 rows to 8192 43.4 / 49.5, 64 rows of 200 to 1000 18.5 / 20.4; one cache of 67 MB read again and again
-// 17.3 / 17.1. Groups of more than sixteen query heads read a KV head twice, and lose the second reading's hits where
-// the cache is small: groups of 20 over 2 KV heads 17.2 / 16.1 at 17 MB, 30.6 / 29.7 at 50 MB, 112 / 115 at 317 MB.
-__device__ inline void lds_stream16(const void* sbase, uint32_t voffset, uint32_t lds_byte_offset) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voffset), "s"(sbase),
-               "s"(lds_byte_offset)
-               : "memory", "m0");
-#pragma clang diagnostic pop
-}
-// ... with an address a lane; and of one word a lane.
-__device__ inline void lds_stream16_at(const void* from, uint32_t lds_byte_offset) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(lds_byte_offset)
-               : "memory", "m0");
-#pragma clang diagnostic pop
-}
-__device__ inline void lds_stream4_at(const void* from, uint32_t lds_byte_offset) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off nt" ::"v"(from), "s"(lds_byte_offset)
-               : "memory", "m0");
-#pragma clang diagnostic pop
-}
-
 // A wave's tile of 32 positions in LDS: key and value rows and the 64 scales. A row's sixteen-byte
 // chunks are permuted (chunk k at k ^ swizzle) so that the eight rows whose chunks are read at once
 // lie in different banks.
@@ -364,27 +350,6 @@ struct Tile {
   }
   static __device__ int swizzle(int row) { return D == 64 ? row & 3 : (row & 3) + 4 * ((row >> 3) & 1); }
 };
-
-// Sum over the wave's lanes up to this one; lanes from `count` on do not matter.
-__device__ inline int wave_scan(int v, int lane, int count) {
-  for (int o = 1; o < 64 && o < count; o <<= 1) {
-    const int below = __shfl_up(v, o, 64);
-    if (lane >= o) v += below;
-  }
-  return v;
-}
-
-// The pairs (a row, a KV head, sixteen of its query heads) lie on a line, each as long as its steps of 128
-// positions (one tile a wave) and kPairCost more for starting it, and the line is cut into equal
-// shares: a workgroup may end one pair, take whole ones and begin another.
-__device__ inline int steps_of(int length) { return (length + 127) / 128; }
-__device__ inline int pair_units(int length) { return length < 0 ? 0 : steps_of(length) + kPairCost; }
-
-// Where vector v of a pair's part i lies in the workspace. A workgroup writes two parts at most: of a pair
-// that began before it and of one that goes on after it.
-__device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int v) {
-  return (uint64_t)(i == 0 ? 2 * first + 1 : 2 * (first + i)) * min(a.group, 16) + v;
-}
 
 // A pair's scores S = K Q^T (positions x query heads) and sums O^T = V^T P are products on the matrix
 // units: 16 query heads fill the columns of a 16 x 16 x 32 tile, so that groups of 1 to 16 heads read
@@ -418,78 +383,25 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int quad = lane >> 4, col = lane & 15;
   const int me = blockIdx.x;
-  const auto length_of = [&](int row) { return min(uniform_load(a.lengths + row), a.limit); };
-
-  // The share, units from .. to of the line, and its first pair. Without `shared` a workgroup
-  // takes one pair.
-  int row, kvg, start, from = 0, to, budget = INT_MAX, length, units;
-  if (a.shared) {
-    const int chunk = (a.rows + 63) / 64, lanes = (a.rows + chunk - 1) / chunk;  // rows of a lane, at most 16
-    int own = 0, own_length = 0;
-    for (int i = 0; i < chunk; ++i) {
-      const int r = lane * chunk + i;
-      if (r < a.rows) {
-        own_length = min(a.lengths[r], a.limit);
-        own += pair_units(own_length) * in_row;
-      }
-    }
-    int sum = wave_scan(own, lane, lanes);
-    const int total = __builtin_amdgcn_readlane(sum, lanes - 1);
-    budget = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    from = me * budget;
-    to = min(from + budget, total);
-    if (from >= to) return;
-    int at = __builtin_ctzll(__ballot(sum > from));
-    row = at * chunk;
-    start = __builtin_amdgcn_readlane(sum - own, at);
-    if (chunk > 1) {
-      own_length = min(a.lengths[min(row + lane, a.rows - 1)], a.limit);
-      own = lane < chunk && row + lane < a.rows ? pair_units(own_length) * in_row : 0;
-      sum = start + wave_scan(own, lane, chunk);
-      at = __builtin_ctzll(__ballot(sum > from));
-      row += at;
-      start = __builtin_amdgcn_readlane(sum - own, at);
-    }
-    length = __builtin_amdgcn_readlane(own_length, at);
-    units = pair_units(length);
-    kvg = (from - start) / units;
-    start += kvg * units;
-  } else {
-    row = me / in_row;
-    kvg = me - row * in_row;
-    start = 0;
-    length = length_of(row);
-    to = units = pair_units(length);
-    if (units == 0) return;
-  }
-  // The next pair of the share, if there is one: rows of negative lengths have none.
-  const auto next_pair = [&] {
-    start += units;
-    if (start >= to) return false;
-    if (++kvg < in_row) return true;
-    kvg = 0;
-    do {
-      length = length_of(++row);
-      units = pair_units(length);
-    } while (units == 0);
-    return true;
-  };
+  Share<128> share;
+  if (!share.first_pair(a, in_row, me, lane)) return;
 
   bool again = false;
-  for (bool more = true; more; more = next_pair()) {
+  for (bool more = true; more; more = share.next_pair(a, in_row)) {
+  const int row = share.row, kvg = share.kvg, length = share.length;
   // This share's steps of the pair, low .. high - 1, and the workgroups that have others.
-  const int steps = steps_of(length), first_unit = start + kPairCost;
-  const int low = max(from - first_unit, 0), high = min(steps, to - first_unit);
-  if (steps > 0 ? low >= high : start < from) continue;  // only the cost of starting it is this share's
-  const int first = first_unit / budget;
-  const int parts = a.shared && steps > 0 ? (first_unit + steps - 1) / budget - first + 1 : 1;
+  const int steps = steps_of<128>(length), first_unit = share.start + kPairCost;
+  const int low = max(share.from - first_unit, 0), high = min(steps, share.to - first_unit);
+  if (steps > 0 ? low >= high : share.start < share.from) continue;  // only the cost of starting it is this share's
+  const int first = first_unit / share.budget;
+  const int parts = a.shared && steps > 0 ? (first_unit + steps - 1) / share.budget - first + 1 : 1;
   const int kvh = kvg / a.head_groups, g0 = (kvg - kvh * a.head_groups) * 16;
   const int begin = 128 * low, end = min(length, 128 * high);
   if (again) __syncthreads();  // the workgroup has read the last pair's sums
   again = true;
   const int vectors = min(16, a.group - g0);
 
-  const int32_t* table = a.table + (uint64_t)row * a.table_stride;
+  const int32_t* table = a.table + (uint64_t)row * a.table_stride + (uint64_t)kvh * a.table_head;
   const int mask = (1 << shift) - 1;
   const uint32_t token = c.token_stride;
   const uint8_t* keys = c.keys + (uint64_t)kvh * c.head_stride;
@@ -513,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       lane_at[odd] = (uint32_t)r * token + chunk * 16;
     }
   }
-  const float* lane_scales = lane < 32 ? c.key_scales : c.value_scales;
+  const float* lane_scales = static_cast<const float*>(lane < 32 ? c.key_scales : c.value_scales);
   // The table's entries of a tile's four groups (of the last position's group behind the part).
   int ids[4];
   const auto load_ids = [&](int t) {
@@ -905,7 +817,9 @@ template <typename T>
 void rotate_to(hipStream_t stream, int format, int rows, const RotateArgs& a) {
   if (format < 0) return rotate<T, -1>(stream, rows, a);
   if (format == HLLM_KV_E4M3) return rotate<T, HLLM_KV_E4M3>(stream, rows, a);
-  rotate<T, HLLM_KV_INT8>(stream, rows, a);
+  if (format == HLLM_KV_INT8) return rotate<T, HLLM_KV_INT8>(stream, rows, a);
+  if (format == kE2m1) return rotate<T, kE2m1>(stream, rows, a);
+  rotate<T, kInt4>(stream, rows, a);
 }
 
 template <typename T, int F>
@@ -920,17 +834,9 @@ void kv_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
 template <typename T, int F, int D>
 void attend(hipStream_t stream, const AttendArgs& a) {
   constexpr int kLds = Tile<D>::kBlock;
-  // More than 64 KiB of LDS is asked for once on each device.
   static std::atomic<uint64_t> asked{0};
-  int device = 0;
-  HIP_CHECK(hipGetDevice(&device));
-  if (!(asked.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-    HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&kv_attention_kernel<T, F, D>),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-    asked.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
-  }
+  ask_for_lds(reinterpret_cast<const void*>(&kv_attention_kernel<T, F, D>), kLds, asked);
   kv_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);
-  if (a.cuts) kv_join_kernel<T, D><<<(unsigned)(a.rows * a.q_heads + 3) / 4, kThreads, 0, stream>>>(a);
 }
 template <typename T, int F>
 void attend_dim(hipStream_t stream, int head_dim, const AttendArgs& a) {
@@ -940,9 +846,18 @@ void attend_dim(hipStream_t stream, int head_dim, const AttendArgs& a) {
 }
 
 template <typename T>
-void attend_format(hipStream_t stream, int format, int head_dim, const AttendArgs& a) {
-  if (format == HLLM_KV_E4M3) return attend_dim<T, HLLM_KV_E4M3>(stream, head_dim, a);
-  attend_dim<T, HLLM_KV_INT8>(stream, head_dim, a);
+void join(hipStream_t stream, int head_dim, const AttendArgs& a) {
+  const unsigned blocks = (unsigned)(a.rows * a.q_heads + 3) / 4;
+  if (head_dim == 64) kv_join_kernel<T, 64><<<blocks, kThreads, 0, stream>>>(a);
+  if (head_dim == 128) kv_join_kernel<T, 128><<<blocks, kThreads, 0, stream>>>(a);
+  if (head_dim == 256) kv_join_kernel<T, 256><<<blocks, kThreads, 0, stream>>>(a);
+}
+template <typename T>
+void attend_format(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a) {
+  if (four_bits(format)) launch_kv4_attention(stream, dtype, format, head_dim, a);
+  if (format == HLLM_KV_E4M3) attend_dim<T, HLLM_KV_E4M3>(stream, head_dim, a);
+  if (format == HLLM_KV_INT8) attend_dim<T, HLLM_KV_INT8>(stream, head_dim, a);
+  if (a.cuts) join<T>(stream, head_dim, a);
 }
 
 }  // namespace
@@ -954,6 +869,7 @@ void launch_rotate(hipStream_t stream, uint32_t dtype, int format, int rows, con
 }
 
 void launch_kv_read(hipStream_t stream, uint32_t dtype, int format, int head_dim, const ReadArgs& a) {
+  if (four_bits(format)) return launch_kv4_read(stream, dtype, format, head_dim, a);
   const auto run = [&](auto zero) {
     using T = decltype(zero);
     if (format == HLLM_KV_E4M3)
@@ -967,74 +883,25 @@ void launch_kv_read(hipStream_t stream, uint32_t dtype, int format, int head_dim
 }
 
 void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a) {
-  if (dtype == HLLM_DTYPE_F16) return attend_format<_Float16>(stream, format, head_dim, a);
-  if (dtype == HLLM_DTYPE_BF16) return attend_format<bhalf>(stream, format, head_dim, a);
-  attend_format<float>(stream, format, head_dim, a);
+  if (dtype == HLLM_DTYPE_F16) return attend_format<_Float16>(stream, dtype, format, head_dim, a);
+  if (dtype == HLLM_DTYPE_BF16) return attend_format<bhalf>(stream, dtype, format, head_dim, a);
+  attend_format<float>(stream, dtype, format, head_dim, a);
 }
 
 // ---------------------------------------------------------------- argument checks
 
 namespace {
 
-// Rows of one call, and workgroups of kThreads threads of one launch: below 2^32 threads over all of a grid's dimensions.
-constexpr uint64_t kMostRows = 1u << 20;
-constexpr uint64_t kMostBlocks = (1u << 24) - 1;
-
-[[noreturn]] void refuse(const std::string& message) { fail(HLLM_INVALID_REQUEST, message); }
-
-size_t element_size(uint32_t dtype) { return dtype == HLLM_DTYPE_F32 ? 4 : 2; }
-
-// Whether vectors of `width` at strides a (of na) and b (of nb) are apart, one inside the other.
-bool apart(uint64_t width, uint64_t na, uint64_t a, uint64_t nb, uint64_t b) {
-  const auto nested = [&](uint64_t ni, uint64_t i, uint64_t no, uint64_t o) {
-    uint64_t extent = width;
-    if (ni > 1) {
-      if (i < width) return false;
-      extent = (ni - 1) * i + width;
-    }
-    return no <= 1 || o >= extent;
-  };
-  return nested(na, a, nb, b) || nested(nb, b, na, a);
-}
-
-Strided tensor(const hllm_rocm_tensor* t, const char* name, uint64_t rows, uint64_t width, bool output) {
-  const std::string who = name;
-  if (!t) refuse(who + " is null");
-  if (!t->data) refuse(who + " has no memory");
-  if (t->dtype != HLLM_DTYPE_F32 && t->dtype != HLLM_DTYPE_F16 && t->dtype != HLLM_DTYPE_BF16) refuse(who + ": unknown dtype");
-  if (t->heads < 1 || t->heads > 1024) refuse(who + ": 1 to 1024 heads");
-  const size_t size = element_size(t->dtype);
-  if ((uintptr_t)t->data % 16) refuse(who + ": memory must be 16-byte aligned");
-  if (t->row_stride > (1ull << 40) || t->head_stride > (1ull << 40)) refuse(who + ": stride too large");
-  if ((rows > 1 && t->row_stride * size % 16) || (t->heads > 1 && t->head_stride * size % 16))
-    refuse(who + ": strides must be multiples of 16 bytes");
-  if (output && !apart(width, rows, t->row_stride, t->heads, t->head_stride)) refuse(who + ": its vectors overlap");
-  return {t->data, t->row_stride, t->head_stride};
-}
-
-// An output that starts where its input does has to be that input.
-void check_in_place(const hllm_rocm_tensor* in, const hllm_rocm_tensor* out, uint64_t rows) {
-  if (in->data != out->data) return;
-  if ((rows > 1 && in->row_stride != out->row_stride) || (in->heads > 1 && in->head_stride != out->head_stride))
-    refuse("an output in its input's memory must have its strides");
-}
-
-// Two outputs, or an output and another tensor's input, that start at one address.
-void check_apart(const void* a, const char* name_a, const void* b, const char* name_b) {
-  if (a == b) refuse(std::string(name_a) + " and " + name_b + " are one memory");
-}
-
-void check_rows(uint64_t rows) {
-  if (rows > kMostRows) refuse("at most 1048576 rows a call");
-}
-
 void check_rotate_grid(uint64_t rows, const RotateArgs& a) {
   if (rows * rotate_blocks(a) > kMostBlocks) refuse("too many rows for these heads");
 }
 
-Pages pages_of(const hllm_rocm_kv_pages* p) {
+// A cache of either kind as the entry points take it: T is hllm_rocm_kv_pages or hllm_rocm_kv4_pages.
+template <typename T>
+Cache cache_of(const T* p) {
+  constexpr bool kFour = std::is_same_v<T, hllm_rocm_kv4_pages>;
   if (!p) refuse("pages is null");
-  if (p->format != HLLM_KV_E4M3 && p->format != HLLM_KV_INT8) refuse("unknown cache format");
+  if (p->format > 1) refuse("unknown cache format");
   if (p->head_dimension != 64 && p->head_dimension != 128 && p->head_dimension != 256)
     refuse("a cache's head dimension is 64, 128 or 256");
   if (p->kv_heads < 1 || p->kv_heads > 1024) refuse("1 to 1024 key-value heads");
@@ -1048,15 +915,18 @@ Pages pages_of(const hllm_rocm_kv_pages* p) {
     refuse("a cache's stride is too large");
   if ((p->pages > 1 && p->page_stride % 16) || p->token_stride % 16 || (p->kv_heads > 1 && p->head_stride % 16))
     refuse("a cache's strides must be multiples of 16 bytes");
+  const uint64_t width = kFour ? p->head_dimension / 2 : p->head_dimension;  // bytes of a vector
   const uint64_t head = p->kv_heads > 1 ? p->head_stride : 0;
-  const uint64_t extent = (p->page_tokens - 1) * p->token_stride + (p->kv_heads - 1) * head + p->head_dimension;
-  if (!apart(p->head_dimension, p->page_tokens, p->token_stride, p->kv_heads, head) ||
+  const uint64_t extent = (p->page_tokens - 1) * p->token_stride + (p->kv_heads - 1) * head + width;
+  if (!apart(width, p->page_tokens, p->token_stride, p->kv_heads, head) ||
       (p->pages > 1 && p->page_stride < extent))
     refuse("a cache's vectors overlap");
   int shift = 0;
   while ((1u << shift) < p->page_tokens) ++shift;
-  return {static_cast<uint8_t*>(p->keys), static_cast<uint8_t*>(p->values), p->key_scales, p->value_scales,
-          p->pages > 1 ? (uint32_t)p->page_stride : 0u, (uint32_t)p->token_stride, head, (int32_t)p->pages, shift, (int32_t)p->kv_heads};
+  const Pages pages = {static_cast<uint8_t*>(p->keys), static_cast<uint8_t*>(p->values), p->key_scales, p->value_scales,
+                       p->pages > 1 ? (uint32_t)p->page_stride : 0u, (uint32_t)p->token_stride, head, (int32_t)p->pages, shift,
+                       (int32_t)p->kv_heads};
+  return {pages, (int)p->format + (kFour ? kE2m1 : 0), (int)p->head_dimension, p->page_tokens};
 }
 
 void check_rope(const hllm_rocm_rope* rope, uint64_t head_dim) {
@@ -1074,33 +944,6 @@ void take_rope(const hllm_rocm_rope* rope, const int32_t* positions, RotateArgs&
   a.interleaved = rope->layout == HLLM_ROPE_INTERLEAVED;
   a.magnitude = rope->magnitude;
   std::copy(rope->turns, rope->turns + 128, a.turns);
-}
-
-// The call's device for its scope.
-class OnDevice {
- public:
-  explicit OnDevice(int32_t device) {
-    HIP_CHECK(hipGetDevice(&before_));
-    if (before_ != device) {
-      // Asked first: the error of a failed hipSetDevice would be reported by the next launch.
-      int devices = 0;
-      HIP_CHECK(hipGetDeviceCount(&devices));
-      if (device >= devices) refuse("there is no device " + std::to_string(device));
-      HIP_CHECK(hipSetDevice(device));
-      changed_ = true;
-    }
-  }
-  ~OnDevice() {
-    if (changed_) (void)hipSetDevice(before_);
-  }
-
- private:
-  int before_ = 0;
-  bool changed_ = false;
-};
-
-void check_device(int32_t device) {
-  if (device < 0) refuse("device is negative");
 }
 
 double positive(double x, double standard, const char* name) {
@@ -1216,84 +1059,76 @@ hllm_status hllm_rocm_rope_apply(int32_t device, void* stream, const hllm_rocm_r
   });
 }
 
-hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv_pages* pages, const int32_t* slots,
-                                uint64_t rows, const hllm_rocm_tensor* k, const hllm_rocm_tensor* v,
-                                const hllm_rocm_rope* rope, const int32_t* positions, const hllm_rocm_tensor* q,
-                                const hllm_rocm_tensor* q_out) {
-  return guarded([&] {
-    check_device(device);
-    check_rows(rows);
-    RotateArgs a{};
-    a.pages = pages_of(pages);
-    const uint64_t D = pages->head_dimension;
-    if (rope) check_rope(rope, D);
-    if (!q != !q_out) refuse("q and q_out come together");
-    if (q && !rope) refuse("q is taken to be rotated: it needs rope");
-    if (rows == 0) return;
-    if (!slots) refuse("slots is null");
-    a.slots = slots;
-    a.k = tensor(k, "k", rows, D, false);
-    a.v = tensor(v, "v", rows, D, false);
-    if (k->heads != pages->kv_heads || v->heads != pages->kv_heads) refuse("k and v must have the cache's heads");
-    if (k->dtype != v->dtype) refuse("k and v must have one dtype");
-    a.k_heads = a.v_heads = (int32_t)pages->kv_heads;
-    if (q) {
-      a.q = tensor(q, "q", rows, D, false);
-      a.q_out = tensor(q_out, "q_out", rows, D, true);
-      if (q->dtype != k->dtype) refuse("q and k must have one dtype");
-      if (q->dtype != q_out->dtype || q->heads != q_out->heads) refuse("q_out must have q's dtype and heads");
-      check_in_place(q, q_out, rows);
-      a.q_heads = (int32_t)q->heads;
-    }
-    a.lanes = (int32_t)D / 16;
-    check_rotate_grid(rows, a);
-    if (rope) take_rope(rope, positions, a);
-    check_apart(pages->keys, "the cache's keys", pages->values, "values");
-    check_apart(pages->keys, "the cache's keys", pages->key_scales, "key_scales");
-    check_apart(pages->keys, "the cache's keys", pages->value_scales, "value_scales");
-    check_apart(pages->values, "the cache's values", pages->key_scales, "key_scales");
-    check_apart(pages->values, "the cache's values", pages->value_scales, "value_scales");
-    check_apart(pages->key_scales, "the cache's key_scales", pages->value_scales, "value_scales");
-    if (q) {
-      check_apart(q_out->data, "q_out", k->data, "k");
-      check_apart(q_out->data, "q_out", v->data, "v");
-      check_apart(q_out->data, "q_out", pages->keys, "the cache's keys");
-      check_apart(q_out->data, "q_out", pages->values, "the cache's values");
-      check_apart(q_out->data, "q_out", pages->key_scales, "the cache's key_scales");
-      check_apart(q_out->data, "q_out", pages->value_scales, "the cache's value_scales");
-    }
-    OnDevice on(device);
-    launch_rotate(static_cast<hipStream_t>(stream), k->dtype, (int)pages->format, (int)rows, a);
-    HIP_CHECK(hipGetLastError());
-  });
-}
-
-hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_pages* pages, const int32_t* slots,
-                              uint64_t rows, const hllm_rocm_tensor* k_out, const hllm_rocm_tensor* v_out) {
-  return guarded([&] {
-    check_device(device);
-    check_rows(rows);
-    ReadArgs a{};
-    a.pages = pages_of(pages);
-    if (rows == 0) return;
-    if (!slots) refuse("slots is null");
-    a.slots = slots;
-    a.rows = (int32_t)rows;
-    a.k = tensor(k_out, "k_out", rows, pages->head_dimension, true);
-    a.v = tensor(v_out, "v_out", rows, pages->head_dimension, true);
-    if (k_out->heads != pages->kv_heads || v_out->heads != pages->kv_heads) refuse("k_out and v_out must have the cache's heads");
-    if (k_out->dtype != v_out->dtype) refuse("k_out and v_out must have one dtype");
-    if (rows * pages->kv_heads * (pages->head_dimension / 4) > kMostBlocks * kThreads) refuse("too many rows for these heads");
-    check_apart(k_out->data, "k_out", v_out->data, "v_out");
-    OnDevice on(device);
-    launch_kv_read(static_cast<hipStream_t>(stream), k_out->dtype, (int)pages->format, (int)pages->head_dimension, a);
-    HIP_CHECK(hipGetLastError());
-  });
-}
-
 }  // extern "C"
 
 namespace {
+
+void append(int32_t device, void* stream, const Cache& cache, const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
+            const hllm_rocm_tensor* v, const hllm_rocm_rope* rope, const int32_t* positions, const hllm_rocm_tensor* q,
+            const hllm_rocm_tensor* q_out) {
+  RotateArgs a{};
+  const Pages& pages = a.pages = cache.pages;
+  const uint64_t D = cache.head_dim;
+  if (rope) check_rope(rope, D);
+  if (!q != !q_out) refuse("q and q_out come together");
+  if (q && !rope) refuse("q is taken to be rotated: it needs rope");
+  if (rows == 0) return;
+  if (!slots) refuse("slots is null");
+  a.slots = slots;
+  a.k = tensor(k, "k", rows, D, false);
+  a.v = tensor(v, "v", rows, D, false);
+  if ((int32_t)k->heads != pages.kv_heads || (int32_t)v->heads != pages.kv_heads) refuse("k and v must have the cache's heads");
+  if (k->dtype != v->dtype) refuse("k and v must have one dtype");
+  a.k_heads = a.v_heads = pages.kv_heads;
+  if (q) {
+    a.q = tensor(q, "q", rows, D, false);
+    a.q_out = tensor(q_out, "q_out", rows, D, true);
+    if (q->dtype != k->dtype) refuse("q and k must have one dtype");
+    if (q->dtype != q_out->dtype || q->heads != q_out->heads) refuse("q_out must have q's dtype and heads");
+    check_in_place(q, q_out, rows);
+    a.q_heads = (int32_t)q->heads;
+  }
+  a.lanes = (int32_t)D / 16;
+  check_rotate_grid(rows, a);
+  if (rope) take_rope(rope, positions, a);
+  check_apart(pages.keys, "the cache's keys", pages.values, "values");
+  check_apart(pages.keys, "the cache's keys", pages.key_scales, "key_scales");
+  check_apart(pages.keys, "the cache's keys", pages.value_scales, "value_scales");
+  check_apart(pages.values, "the cache's values", pages.key_scales, "key_scales");
+  check_apart(pages.values, "the cache's values", pages.value_scales, "value_scales");
+  check_apart(pages.key_scales, "the cache's key_scales", pages.value_scales, "value_scales");
+  if (q) {
+    check_apart(q_out->data, "q_out", k->data, "k");
+    check_apart(q_out->data, "q_out", v->data, "v");
+    check_apart(q_out->data, "q_out", pages.keys, "the cache's keys");
+    check_apart(q_out->data, "q_out", pages.values, "the cache's values");
+    check_apart(q_out->data, "q_out", pages.key_scales, "the cache's key_scales");
+    check_apart(q_out->data, "q_out", pages.value_scales, "the cache's value_scales");
+  }
+  OnDevice on(device);
+  launch_rotate(static_cast<hipStream_t>(stream), k->dtype, cache.format, (int)rows, a);
+  HIP_CHECK(hipGetLastError());
+}
+
+void read(int32_t device, void* stream, const Cache& cache, const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k_out,
+          const hllm_rocm_tensor* v_out) {
+  ReadArgs a{};
+  a.pages = cache.pages;
+  const uint64_t heads = a.pages.kv_heads;
+  if (rows == 0) return;
+  if (!slots) refuse("slots is null");
+  a.slots = slots;
+  a.rows = (int32_t)rows;
+  a.k = tensor(k_out, "k_out", rows, cache.head_dim, true);
+  a.v = tensor(v_out, "v_out", rows, cache.head_dim, true);
+  if (k_out->heads != heads || v_out->heads != heads) refuse("k_out and v_out must have the cache's heads");
+  if (k_out->dtype != v_out->dtype) refuse("k_out and v_out must have one dtype");
+  if (rows * heads * (cache.head_dim / 4) > kMostBlocks * kThreads) refuse("too many rows for these heads");
+  check_apart(k_out->data, "k_out", v_out->data, "v_out");
+  OnDevice on(device);
+  launch_kv_read(static_cast<hipStream_t>(stream), k_out->dtype, cache.format, cache.head_dim, a);
+  HIP_CHECK(hipGetLastError());
+}
 
 // How a call's work is cut and what its workspace holds: each pair's cut, then outputs and statistics of
 // two parts of each workgroup.
@@ -1302,14 +1137,16 @@ struct AttendPlan {
   bool shared = false;
 };
 
-AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64_t query_heads, uint64_t limit) {
-  if (query_heads < 1 || query_heads > 1024 || query_heads % pages.kv_heads)
+AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_heads, uint64_t limit) {
+  const uint64_t kv_heads = cache.pages.kv_heads;
+  if (query_heads < 1 || query_heads > 1024 || query_heads % kv_heads)
     refuse("query heads are a multiple of the cache's heads, at most 1024");
   AttendPlan p;
   if (rows == 0) return p;
-  const uint64_t group = query_heads / pages.kv_heads;
+  const uint64_t group = query_heads / kv_heads;
   p.head_groups = (group + 15) / 16;
-  const uint64_t pairs = rows * pages.kv_heads * p.head_groups, steps = (limit + 127) / 128, cost = kPairCost + steps;
+  const uint64_t step = attend_step(cache.format, cache.head_dim), steps = (limit + step - 1) / step, cost = kPairCost + steps;
+  const uint64_t pairs = rows * kv_heads * p.head_groups;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
   // A workgroup for each pair where rows are short or pairs many: no row has more steps than 5 and 9 for each
   // pair a workgroup of the card. Shares cost 3 to 5 us more (each workgroup sums all rows' steps; the join), and
@@ -1323,7 +1160,7 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   // So the crossing lies at the line for some tens of rows, and below it by a third for hundreds (the line loses up to 13%
   // there) and for F32 heads of 256. Rows that are padding count as pairs, for the host does not know them: 16
   // rows to 8000 take 21.8, with 48 padding rows 22.0, with 900, where pairs stay whole, 73.
-  const uint64_t fit = attend_blocks((int)pages.head_dimension, false);
+  const uint64_t fit = attend_blocks(cache.format, cache.head_dim, false);
   const bool whole = steps * fit <= 5 * fit + 9 * pairs;
   p.blocks = pairs;
   if (whole || rows > kMostSharedRows) return p;
@@ -1334,7 +1171,7 @@ AttendPlan plan_attention(const hllm_rocm_kv_pages& pages, uint64_t rows, uint64
   if (p.shared) p.blocks = sharing;
   p.cuts = (pairs + 1) / 2 * 2;  // whole sixteen bytes
   p.parts = 2 * sharing * std::min<uint64_t>(group, 16);
-  p.bytes = p.cuts * sizeof(int2) + p.parts * (pages.head_dimension + 2) * sizeof(float);
+  p.bytes = p.cuts * sizeof(int2) + p.parts * (cache.head_dim + 2) * sizeof(float);
   return p;
 }
 
@@ -1343,69 +1180,139 @@ constexpr uint64_t kMostPositions = 1u << 30;
 
 uint64_t clamp_length(uint64_t max_length) { return std::min(max_length, kMostPositions); }
 
+void attend_workspace(const Cache& cache, uint64_t rows, uint32_t query_heads, uint64_t max_length, uint64_t* bytes) {
+  check_rows(rows);
+  *bytes = plan_attention(cache, rows, query_heads, clamp_length(max_length)).bytes;
+}
+
+void attend(int32_t device, void* stream, const Cache& cache, const hllm_rocm_kv_attention_args* args, uint64_t table_head_stride) {
+  AttendArgs a{};
+  a.pages = cache.pages;
+  if (!args) refuse("args is null");
+  const uint64_t rows = args->rows, D = cache.head_dim;
+  check_rows(rows);
+  if (rows == 0) return;
+  a.q = tensor(&args->q, "q", rows, D, false);
+  a.out = tensor(&args->out, "out", rows, D, true);
+  if (args->q.dtype != args->out.dtype || args->q.heads != args->out.heads) refuse("out must have q's dtype and heads");
+  if (args->q.data == args->out.data) refuse("out must not be q");
+  if (!std::isfinite((float)(args->scale * kLog2e))) refuse("scale is not finite");  // as the kernels take it, with log2 e
+  if (!args->lengths) refuse("lengths is null");
+  if (args->table_width > kMostPositions / cache.page_tokens) refuse("a page table's row holds at most 2^30 positions");
+  const uint64_t limit = std::min(clamp_length(args->max_length), args->table_width * cache.page_tokens);
+  if (limit > 0 && !args->page_table) refuse("page_table is null");
+  if (args->table_stride > (1ull << 40)) refuse("table_stride is too large");
+  if (table_head_stride > (1ull << 40)) refuse("table_head_stride is too large");
+  const AttendPlan plan = plan_attention(cache, rows, args->q.heads, limit);
+  if (plan.bytes > 0 && (!args->workspace || args->workspace_bytes < plan.bytes || (uintptr_t)args->workspace % 16))
+    refuse("the workspace is null, not 16-byte aligned or below " + std::to_string(plan.bytes) + " bytes");
+  if (plan.bytes > 0) {
+    check_apart(args->workspace, "the workspace", args->out.data, "out");
+    check_apart(args->workspace, "the workspace", args->q.data, "q");
+  }
+  a.table = args->page_table;
+  a.table_stride = args->table_stride;
+  a.table_head = table_head_stride;
+  a.lengths = args->lengths;
+  a.rows = (int32_t)rows;
+  a.q_heads = (int32_t)args->q.heads;
+  a.group = a.q_heads / a.pages.kv_heads;
+  a.head_groups = (int32_t)plan.head_groups;
+  a.limit = (int32_t)limit;
+  // F32 queries take twice the LDS.
+  const bool f32 = args->q.dtype == HLLM_DTYPE_F32;
+  a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks(cache.format, (int)D, f32)) : plan.blocks);
+  a.shared = plan.shared;
+  a.scale_hi = (float)(args->scale * kLog2e);
+  a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);
+  if (plan.shared) {
+    a.cuts = static_cast<int2*>(args->workspace);
+    a.part = reinterpret_cast<float*>(a.cuts + plan.cuts);
+    a.stats = a.part + plan.parts * D;
+  }
+  OnDevice on(device);
+  launch_kv_attention(static_cast<hipStream_t>(stream), args->q.dtype, cache.format, (int)D, a);
+  HIP_CHECK(hipGetLastError());
+}
+
 }  // namespace
 
 extern "C" {
+
+hllm_status hllm_rocm_kv_append(int32_t device, void* stream, const hllm_rocm_kv_pages* pages, const int32_t* slots,
+                                uint64_t rows, const hllm_rocm_tensor* k, const hllm_rocm_tensor* v,
+                                const hllm_rocm_rope* rope, const int32_t* positions, const hllm_rocm_tensor* q,
+                                const hllm_rocm_tensor* q_out) {
+  return guarded([&] {
+    check_device(device);
+    check_rows(rows);
+    append(device, stream, cache_of(pages), slots, rows, k, v, rope, positions, q, q_out);
+  });
+}
+
+hllm_status hllm_rocm_kv4_append(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages, const int32_t* slots,
+                                 uint64_t rows, const hllm_rocm_tensor* k, const hllm_rocm_tensor* v,
+                                 const hllm_rocm_rope* rope, const int32_t* positions, const hllm_rocm_tensor* q,
+                                 const hllm_rocm_tensor* q_out) {
+  return guarded([&] {
+    check_device(device);
+    check_rows(rows);
+    append(device, stream, cache_of(pages), slots, rows, k, v, rope, positions, q, q_out);
+  });
+}
+
+hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_pages* pages, const int32_t* slots,
+                              uint64_t rows, const hllm_rocm_tensor* k_out, const hllm_rocm_tensor* v_out) {
+  return guarded([&] {
+    check_device(device);
+    check_rows(rows);
+    read(device, stream, cache_of(pages), slots, rows, k_out, v_out);
+  });
+}
+
+hllm_status hllm_rocm_kv4_read(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages, const int32_t* slots,
+                               uint64_t rows, const hllm_rocm_tensor* k_out, const hllm_rocm_tensor* v_out) {
+  return guarded([&] {
+    check_device(device);
+    check_rows(rows);
+    read(device, stream, cache_of(pages), slots, rows, k_out, v_out);
+  });
+}
 
 hllm_status hllm_rocm_kv_attention_workspace(const hllm_rocm_kv_pages* pages, uint64_t rows, uint32_t query_heads,
                                              uint64_t max_length, uint64_t* bytes) {
   return guarded([&] {
     if (!bytes) refuse("null argument");
-    pages_of(pages);
-    check_rows(rows);
-    *bytes = plan_attention(*pages, rows, query_heads, clamp_length(max_length)).bytes;
+    attend_workspace(cache_of(pages), rows, query_heads, max_length, bytes);
+  });
+}
+
+hllm_status hllm_rocm_kv4_attention_workspace(const hllm_rocm_kv4_pages* pages, uint64_t rows, uint32_t query_heads,
+                                              uint64_t max_length, uint64_t* bytes) {
+  return guarded([&] {
+    if (!bytes) refuse("null argument");
+    attend_workspace(cache_of(pages), rows, query_heads, max_length, bytes);
   });
 }
 
 hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
                                    const hllm_rocm_kv_attention_args* args) {
+  return hllm_rocm_kv_attention_by_head(device, stream, pages, args, 0);
+}
+
+hllm_status hllm_rocm_kv_attention_by_head(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                                           const hllm_rocm_kv_attention_args* args, uint64_t table_head_stride) {
   return guarded([&] {
     check_device(device);
-    AttendArgs a{};
-    a.pages = pages_of(pages);
-    if (!args) refuse("args is null");
-    const uint64_t rows = args->rows, D = pages->head_dimension;
-    check_rows(rows);
-    if (rows == 0) return;
-    a.q = tensor(&args->q, "q", rows, D, false);
-    a.out = tensor(&args->out, "out", rows, D, true);
-    if (args->q.dtype != args->out.dtype || args->q.heads != args->out.heads) refuse("out must have q's dtype and heads");
-    if (args->q.data == args->out.data) refuse("out must not be q");
-    if (!std::isfinite((float)(args->scale * kLog2e))) refuse("scale is not finite");  // as the kernels take it, with log2 e
-    if (!args->lengths) refuse("lengths is null");
-    if (args->table_width > kMostPositions / pages->page_tokens) refuse("a page table's row holds at most 2^30 positions");
-    const uint64_t limit = std::min(clamp_length(args->max_length), args->table_width * pages->page_tokens);
-    if (limit > 0 && !args->page_table) refuse("page_table is null");
-    if (args->table_stride > (1ull << 40)) refuse("table_stride is too large");
-    const AttendPlan plan = plan_attention(*pages, rows, args->q.heads, limit);
-    if (plan.bytes > 0 && (!args->workspace || args->workspace_bytes < plan.bytes || (uintptr_t)args->workspace % 16))
-      refuse("the workspace is null, not 16-byte aligned or below " + std::to_string(plan.bytes) + " bytes");
-    if (plan.bytes > 0) {
-      check_apart(args->workspace, "the workspace", args->out.data, "out");
-      check_apart(args->workspace, "the workspace", args->q.data, "q");
-    }
-    a.table = args->page_table;
-    a.table_stride = args->table_stride;
-    a.lengths = args->lengths;
-    a.rows = (int32_t)rows;
-    a.q_heads = (int32_t)args->q.heads;
-    a.group = a.q_heads / a.pages.kv_heads;
-    a.head_groups = (int32_t)plan.head_groups;
-    a.limit = (int32_t)limit;
-    // F32 queries take twice the LDS.
-    const bool f32 = args->q.dtype == HLLM_DTYPE_F32;
-    a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks((int)D, f32)) : plan.blocks);
-    a.shared = plan.shared;
-    a.scale_hi = (float)(args->scale * kLog2e);
-    a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);
-    if (plan.shared) {
-      a.cuts = static_cast<int2*>(args->workspace);
-      a.part = reinterpret_cast<float*>(a.cuts + plan.cuts);
-      a.stats = a.part + plan.parts * D;
-    }
-    OnDevice on(device);
-    launch_kv_attention(static_cast<hipStream_t>(stream), args->q.dtype, (int)pages->format, (int)D, a);
-    HIP_CHECK(hipGetLastError());
+    attend(device, stream, cache_of(pages), args, table_head_stride);
+  });
+}
+
+hllm_status hllm_rocm_kv4_attention(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
+                                    const hllm_rocm_kv_attention_args* args, uint64_t table_head_stride) {
+  return guarded([&] {
+    check_device(device);
+    attend(device, stream, cache_of(pages), args, table_head_stride);
   });
 }
 

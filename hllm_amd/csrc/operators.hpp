@@ -13,15 +13,26 @@ struct Strided {
   uint64_t row, head;
 };
 
+// Formats of a cache's vectors: hllm_kv_format, then hllm_kv4_format.
+constexpr int kE2m1 = 2 + HLLM_KV4_E2M1, kInt4 = 2 + HLLM_KV4_INT4;
+inline bool four_bits(int format) { return format >= kE2m1; }
+
 // A cache as kernels take it; a slot is page << page_shift | position.
 struct Pages {
   uint8_t* keys;
   uint8_t* values;
-  float* key_scales;
-  float* value_scales;
+  void* key_scales;  // F32 for each vector; of 4 bits for each 32 elements: bytes (E2M1), BF16 (INT4)
+  void* value_scales;
   uint32_t page_stride, token_stride;  // bytes
   uint64_t head_stride;
   int32_t pages, page_shift, kv_heads;
+};
+
+// ... and as entry points do.
+struct Cache {
+  Pages pages;
+  int format, head_dim;
+  uint32_t page_tokens;
 };
 
 struct RotateArgs {
@@ -38,7 +49,7 @@ struct RotateArgs {
   uint64_t turns[128];
 };
 // q and k rotated into q_out and k_out (format -1), or k rotated and k and v quantised into the
-// cache (format: hllm_kv_format).
+// cache.
 void launch_rotate(hipStream_t stream, uint32_t dtype, int format, int rows, const RotateArgs& a);
 
 struct ReadArgs {
@@ -48,12 +59,13 @@ struct ReadArgs {
   int32_t rows;
 };
 void launch_kv_read(hipStream_t stream, uint32_t dtype, int format, int head_dim, const ReadArgs& a);
+void launch_kv4_read(hipStream_t stream, uint32_t dtype, int format, int head_dim, const ReadArgs& a);
 
 struct AttendArgs {
   Pages pages;
   Strided q, out;
   const int32_t* table;
-  uint64_t table_stride;
+  uint64_t table_stride, table_head;  // entries from one row's, and one KV head's, pages to the next
   const int32_t* lengths;
   int32_t rows, q_heads, group;  // group: query heads of one KV head
   int32_t head_groups;           // sixteens of a KV head's query heads
@@ -66,6 +78,8 @@ struct AttendArgs {
   float* stats;                  // [blocks][2][min(group, 16)][2]: their score maximum (base 2) and sum
 };
 void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
+// Without the join.
+void launch_kv4_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
 
 // Steps (of 128 positions) that starting a pair is counted as. With 1, 2, 3, 4: 128 rows to 8192 positions of head dimension
 // 256 52.8, 52.7, 53.7, 55.2 us; 32 rows to 4096 of 64 14.6, 15.0, 16.0, 16.1; 64 rows to 8192 of 128 43.5, 43.9, 44.1,
@@ -78,8 +92,19 @@ constexpr uint64_t kMostSharedRows = 1024;
 // D / 2); F32 queries of 256 elements leave room for one on a CU.
 template <int D>
 constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
-inline uint64_t attend_blocks(int head_dim, bool f32) {
+// Over a 4-bit cache: positions of a wave's tile, and workgroups on a CU.
+template <int D>
+constexpr int kAttend4Tile = D == 256 ? 32 : 64;
+template <int D>
+constexpr int kAttend4Blocks = D == 64 ? 4 : D == 128 ? 3 : 2;
+inline uint64_t attend_blocks(int format, int head_dim, bool f32) {
+  if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : kAttend4Blocks<256>);
   return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : f32 ? 1 : kAttendBlocks<256>);
+}
+// Positions of a step: one tile for each of a workgroup's four waves.
+inline uint64_t attend_step(int format, int head_dim) {
+  if (!four_bits(format)) return 128;
+  return 4 * (head_dim == 64 ? kAttend4Tile<64> : head_dim == 128 ? kAttend4Tile<128> : kAttend4Tile<256>);
 }
 
 }  // namespace hllm_rocm

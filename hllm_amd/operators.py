@@ -27,6 +27,8 @@ _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: cap
 _FORMATS = {torch.float8_e4m3fn: capi.KV_E4M3, torch.int8: capi.KV_INT8}
 _MOST = (1 << 32) - 1  # past every size that the library takes, and past every length that counts
 _CODES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_FORMATS4 = {torch.uint8: capi.KV4_E2M1, torch.bfloat16: capi.KV4_INT4}
+_SCALES4 = {"e2m1": torch.uint8, "int4": torch.bfloat16}
 # capi.Tensor and capi.KvAttentionArgs as bytes: a quarter of the time of filling a ctypes structure.
 TENSOR = struct.Struct("@PIIQQ")
 ATTENTION_ARGS = struct.Struct("@QPQQPQf4xPIIQQPIIQQPQ")
@@ -77,7 +79,27 @@ class Rope:
         capi.check(capi.library().hllm_rocm_rope_plan(C.byref(c), self.address))
 
 
-class KvPages:
+class _Pages:
+    """What both kinds of cache have in common: tensors that are held, and their description for the library."""
+
+    def _describe(self, keys, values, key_scales, value_scales, kind, format, head_dim):
+        for x in (values, key_scales, value_scales):
+            if x.device != keys.device:
+                raise ValueError("a cache lies on one device")
+        if min(keys.shape) < 1 or min(keys.stride()) < 0:
+            raise ValueError("a cache has pages")
+        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
+        self.device, self.kv_heads, self.head_dim = keys.device, keys.shape[1], head_dim
+        self.pages, self.page_tokens = keys.shape[0], keys.shape[2]
+        size = keys.element_size()
+        self.c = kind(format, self.pages, self.page_tokens, self.kv_heads, head_dim, keys.stride(0) * size,
+                      keys.stride(2) * size, keys.stride(1) * size, keys.data_ptr(), values.data_ptr(),
+                      key_scales.data_ptr(), value_scales.data_ptr())
+        self.address = C.addressof(self.c)
+        kv_attention_workspace(self, 0, self.kv_heads, 0)  # the library refuses a wrong description here
+
+
+class KvPages(_Pages):
     """An 8-bit paged cache in the caller's tensors: ``keys`` and ``values`` [pages, kv_heads,
     page_tokens, head_dim] (torch.float8_e4m3fn or torch.int8; any strides of whole sixteen bytes
     with a contiguous last dimension, so a permuted [pages, page_tokens, kv_heads, head_dim] too)
@@ -97,19 +119,7 @@ class KvPages:
         for name, x in (("key_scales", key_scales), ("value_scales", value_scales)):
             if x.shape != keys.shape[:3] or x.dtype != torch.float32 or not x.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float32 [pages, kv_heads, page_tokens]")
-        for x in (values, key_scales, value_scales):
-            if x.device != keys.device:
-                raise ValueError("a cache lies on one device")
-        if min(keys.shape) < 1 or min(keys.stride()) < 0:
-            raise ValueError("a cache has pages")
-        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
-        self.device, self.kv_heads, self.head_dim = keys.device, keys.shape[1], keys.shape[3]
-        self.pages, self.page_tokens = keys.shape[0], keys.shape[2]
-        self.c = capi.KvPages(_FORMATS[keys.dtype], self.pages, self.page_tokens, self.kv_heads, self.head_dim,
-                              keys.stride(0), keys.stride(2), keys.stride(1), keys.data_ptr(), values.data_ptr(),
-                              key_scales.data_ptr(), value_scales.data_ptr())
-        self.address = C.addressof(self.c)
-        kv_attention_workspace(self, 0, self.kv_heads, 0)  # the library refuses a wrong description here
+        self._describe(keys, values, key_scales, value_scales, capi.KvPages, _FORMATS[keys.dtype], keys.shape[3])
 
     @classmethod
     def empty(cls, format: str, pages: int, kv_heads: int, page_tokens: int, head_dim: int, device="cuda"):
@@ -124,6 +134,50 @@ class KvPages:
             return torch.zeros(pages, kv_heads, page_tokens, dtype=torch.float32, device=device)
 
         return cls(codes().view(_CODES[format]), codes().view(_CODES[format]), scales(), scales())
+
+
+class Kv4Pages(_Pages):
+    """A 4-bit paged cache in the caller's tensors: ``keys`` and ``values`` [pages, kv_heads, page_tokens,
+    head_dim / 2] (torch.uint8, two codes a byte; strides as in ``KvPages``) and scales [pages, kv_heads,
+    page_tokens, head_dim / 32], one for 32 elements: torch.uint8 for E2M1 codes (a power of two's exponent + 127) or
+    torch.bfloat16 for INT4 codes. include/hllm_rocm.h states the formats and the order of the codes. The
+    tensors are held, and must not be resized."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor,
+                 value_scales: torch.Tensor):
+        for name, x in (("keys", keys), ("values", values), ("key_scales", key_scales), ("value_scales", value_scales)):
+            _on_device(x, name)
+        if keys.dtype != torch.uint8 or keys.dim() != 4:
+            raise ValueError("keys must be [pages, kv_heads, page_tokens, head_dim / 2] of uint8")
+        if values.shape != keys.shape or values.dtype != keys.dtype or values.stride() != keys.stride():
+            raise ValueError("values must have the keys' shape, strides and dtype")
+        if keys.stride(3) != 1:
+            raise ValueError("the cache's last dimension must be contiguous")
+        shape = (*keys.shape[:3], keys.shape[3] // 16)
+        for name, x in (("key_scales", key_scales), ("value_scales", value_scales)):
+            if x.shape != shape or x.dtype not in _FORMATS4 or x.dtype != key_scales.dtype or not x.is_contiguous():
+                raise ValueError(f"{name} must be contiguous [pages, kv_heads, page_tokens, head_dim / 32] of uint8 "
+                                 "(E2M1) or bfloat16 (INT4)")
+        self._describe(keys, values, key_scales, value_scales, capi.Kv4Pages, _FORMATS4[key_scales.dtype], 2 * keys.shape[3])
+
+    @classmethod
+    def empty(cls, format: str, pages: int, kv_heads: int, page_tokens: int, head_dim: int, device="cuda"):
+        """A new cache; format "e2m1" or "int4"."""
+        if format not in _SCALES4:
+            raise ValueError(f"unknown cache format {format!r}")
+
+        def codes():
+            return torch.zeros(pages, kv_heads, page_tokens, head_dim // 2, dtype=torch.uint8, device=device)
+
+        def scales():
+            return torch.zeros(pages, kv_heads, page_tokens, head_dim // 32, dtype=_SCALES4[format], device=device)
+
+        return cls(codes(), codes(), scales(), scales())
+
+
+def _entry(pages: KvPages | Kv4Pages, name: str, name4: str):
+    """The library's function for this kind of cache."""
+    return getattr(capi.library(), "hllm_rocm_" + (name4 if isinstance(pages, Kv4Pages) else name))
 
 
 def _on_device(x: torch.Tensor, name: str) -> None:
@@ -158,6 +212,19 @@ def _numbers(x: torch.Tensor, name: str, device: torch.device, rows: int) -> int
     if x.dim() != 1 or x.shape[0] != rows or not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous [{rows}]")
     return x.data_ptr()
+
+
+def _table(page_table: torch.Tensor, device: torch.device, rows: int, kv_heads: int | None = None):
+    """(address, width, row stride, head stride) of a page table [rows, width], or [rows, kv_heads, width] where it may be."""
+    if not isinstance(page_table, torch.Tensor) or page_table.device != device or page_table.dtype != torch.int32:
+        raise ValueError(f"page_table must be int32 on {device}")
+    shape, stride = page_table.shape, page_table.stride()
+    by_head = len(shape) == 3 and kv_heads is not None
+    if shape[:-1] != ((rows, kv_heads) if by_head else (rows,)):
+        raise ValueError("page_table must be [rows, width]" + ("" if kv_heads is None else " or [rows, kv_heads, width]"))
+    if shape[-1] > 1 and stride[-1] != 1:
+        raise ValueError("a row of page_table must be contiguous")
+    return page_table.data_ptr(), shape[-1], stride[0], stride[1] if by_head else 0
 
 
 def _stream(device: torch.device) -> int:
@@ -200,7 +267,7 @@ def rope(plan: Rope, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor |
     return q_out if k is None else (q_out, k_out)
 
 
-def kv_append(pages: KvPages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+def kv_append(pages: KvPages | Kv4Pages, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               q: torch.Tensor | None = None, rope: Rope | None = None, positions: torch.Tensor | None = None,
               q_out: torch.Tensor | None = None):
     """Quantises k and v [rows, kv_heads, head_dim] into the cache at ``slots`` [rows] (int32, -1: a
@@ -221,12 +288,12 @@ def kv_append(pages: KvPages, slots: torch.Tensor, k: torch.Tensor, v: torch.Ten
         q_from, q_to = TENSOR.pack(*c), TENSOR.pack(*d)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    capi.check(capi.library().hllm_rocm_kv_append(device.index, _stream(device), pages.address, to, rows, a, b, plan, at,
-                                                  q_from, q_to))
+    capi.check(_entry(pages, "kv_append", "kv4_append")(device.index, _stream(device), pages.address, to, rows, a, b, plan, at,
+                                                       q_from, q_to))
     return q_out
 
 
-def kv_read(pages: KvPages, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
+def kv_read(pages: KvPages | Kv4Pages, slots: torch.Tensor, dtype: torch.dtype = torch.float16,
             k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
     """The cached keys and values at ``slots`` [rows] (int32): (k, v) [rows, kv_heads, head_dim] of
     ``dtype``, or in k_out and v_out. Rows of slots outside the cache are left as they were (in
@@ -241,16 +308,16 @@ def kv_read(pages: KvPages, slots: torch.Tensor, dtype: torch.dtype = torch.floa
     if k_out is None:
         k_out, v_out = pages.key_scales.new_empty((2, rows, heads, dim), dtype=dtype)
     a, b = _rows(k_out, "k_out", device, rows, dim, heads), _rows(v_out, "v_out", device, rows, dim, heads)
-    capi.check(capi.library().hllm_rocm_kv_read(device.index, _stream(device), pages.address, at, rows, a, b))
+    capi.check(_entry(pages, "kv_read", "kv4_read")(device.index, _stream(device), pages.address, at, rows, a, b))
     return k_out, v_out
 
 
-def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, lengths: torch.Tensor,
+def kv_attention(q: torch.Tensor, pages: KvPages | Kv4Pages, page_table: torch.Tensor, lengths: torch.Tensor,
                  max_length: int, scale: float | None = None, out: torch.Tensor | None = None,
                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q K^T) V of one new token a row, q [rows, q_heads, head_dim], over the first
     ``lengths`` [rows] (int32) positions of the row's pages in ``page_table`` [rows, width]
-    (int32). ``max_length`` bounds the lengths on the host; ``scale`` is 1 / sqrt(head_dim) unless
+    (int32), or of each KV head's own in [rows, kv_heads, width]. ``max_length`` bounds the lengths on the host; ``scale`` is 1 / sqrt(head_dim) unless
     given. A length of 0 gives zeros, a negative one leaves the row as it was (in a new output:
     undefined). ``workspace``: a contiguous uint8 tensor of at least ``kv_attention_workspace``
     bytes that no concurrent call uses; made for the call unless given."""
@@ -261,13 +328,7 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
     a = _fields(q, "q", device, rows, pages.head_dim)
     out, b = _output(out, q, a, "out")
     n = _numbers(lengths, "lengths", device, rows)
-    if not isinstance(page_table, torch.Tensor) or page_table.device != device or page_table.dtype != torch.int32 \
-            or page_table.dim() != 2 or page_table.shape[0] != rows:
-        raise ValueError(f"page_table must be int32 [rows, width] on {device}")
-    width = page_table.shape[1]
-    stride, last = page_table.stride()
-    if width > 1 and last != 1:
-        raise ValueError("a row of page_table must be contiguous")
+    table, width, stride, head_stride = _table(page_table, device, rows, pages.kv_heads)
     if max_length < 0:
         raise ValueError("max_length is negative")
     if scale is not None and not abs(scale) < 2e38:
@@ -281,20 +342,20 @@ def kv_attention(q: torch.Tensor, pages: KvPages, page_table: torch.Tensor, leng
             or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous uint8 on {device}")
     at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    args = ATTENTION_ARGS.pack(rows, page_table.data_ptr(), width, stride, n, max_length,
+    args = ATTENTION_ARGS.pack(rows, table, width, stride, n, max_length,
                                pages.head_dim ** -0.5 if scale is None else scale, *a, *b, at, size)
-    capi.check(capi.library().hllm_rocm_kv_attention(device.index, _stream(device), pages.address, args))
+    capi.check(_entry(pages, "kv_attention_by_head", "kv4_attention")(device.index, _stream(device), pages.address, args, head_stride))
     return out
 
 
-def kv_attention_workspace(pages: KvPages, rows: int, q_heads: int, max_length: int) -> int:
+def kv_attention_workspace(pages: KvPages | Kv4Pages, rows: int, q_heads: int, max_length: int) -> int:
     """Bytes of workspace that ``kv_attention`` needs for these sizes (0: none)."""
     if min(rows, q_heads, max_length) < 0:
         raise ValueError("rows, q_heads and max_length are not negative")
     return _workspace_bytes(pages, min(rows, _MOST), min(q_heads, _MOST), min(max_length, _MOST))
 
 
-def _workspace_bytes(pages: KvPages, rows: int, q_heads: int, max_length: int) -> int:
+def _workspace_bytes(pages: KvPages | Kv4Pages, rows: int, q_heads: int, max_length: int) -> int:
     need = C.c_uint64()
-    capi.check(capi.library().hllm_rocm_kv_attention_workspace(pages.address, rows, q_heads, max_length, C.byref(need)))
+    capi.check(_entry(pages, "kv_attention_workspace", "kv4_attention_workspace")(pages.address, rows, q_heads, max_length, C.byref(need)))
     return need.value

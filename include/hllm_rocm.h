@@ -496,11 +496,65 @@ typedef struct {
 
 hllm_status hllm_rocm_kv_attention(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
                                    const hllm_rocm_kv_attention_args* args);
+/* ... with pages of its own for each KV head: head h of a row finds them table_head_stride * h entries after
+ * the row's (0: every head the same), as a selection of pages by head leaves them. `lengths` counts the
+ * positions of those pages, the same for all heads of a row. */
+hllm_status hllm_rocm_kv_attention_by_head(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                                           const hllm_rocm_kv_attention_args* args,
+                                           uint64_t table_head_stride);
 /* The workspace that does for a call with `rows` rows of `query_heads` heads and this max_length or a
  * smaller one (0: none, and `workspace` may be NULL). Needs no device. */
 hllm_status hllm_rocm_kv_attention_workspace(const hllm_rocm_kv_pages* pages, uint64_t rows,
                                              uint32_t query_heads, uint64_t max_length,
                                              uint64_t* bytes);
+
+/* What a 4-bit cache holds of 32 elements x that follow one another in a vector, a group: codes and one scale, x ~= value of
+ * the code * scale. A group with an element that is not finite holds the scale NaN and reads back as NaN, its
+ * vector's other groups as they are.
+ *   E2M1  (OCP microscaling) codes of the numbers 0, 1/2, 1, 3/2, 2, 3, 4, 6, the fourth bit their sign; the scale is a
+ *         power of two, the byte e + 127 (0: 2^-127; 255: NaN). Written with the smallest e that leaves max(|x|max, 2^-100)
+ *         at most 7 * 2^e, but at most 125; x / 2^e is rounded to the nearest number, ties to the even code, 6 standing
+ *         for all that is larger. Off by at most 2^e: 2/7 of |x|max (of the largest numbers more).
+ *   INT4  codes -7 .. 7, held as code + 8; the scale is BF16 (the upper half of an F32 number; one that is not finite
+ *         counts as NaN). Written with scale = max(|x|max, 2^-100) / 7 in F32, its lower half cut off, and code =
+ *         x * (1 / scale) rounded to nearest even, at most 7: off by half a scale and 2^-7 |x|max at most.
+ * Two codes lie in a byte, the lower four bits first. A key's codes lie in order: byte i holds elements 2 i and 2 i + 1. A
+ * value's bytes go round its G = head_dimension / 32 groups: byte G c + g holds elements 32 g + 2 c and 32 g + 2 c + 1. */
+typedef enum { HLLM_KV4_E2M1 = 0, HLLM_KV4_INT4 = 1 } hllm_kv4_format;
+
+/* A paged 4-bit cache: as hllm_rocm_kv_pages, with head_dimension / 2 bytes a vector and
+ * head_dimension / 32 scales, [pages][kv_heads][page_tokens][head_dimension / 32]. */
+typedef struct {
+  uint32_t format;          /* hllm_kv4_format */
+  uint32_t pages;
+  uint32_t page_tokens;
+  uint32_t kv_heads;
+  uint32_t head_dimension;  /* 64, 128 or 256 */
+  uint64_t page_stride;     /* bytes, as in hllm_rocm_kv_pages */
+  uint64_t token_stride;
+  uint64_t head_stride;
+  void* keys;
+  void* values;
+  void* key_scales;         /* E2M1: bytes; INT4: BF16 */
+  void* value_scales;
+} hllm_rocm_kv4_pages;
+
+/* The 8-bit cache's operators over a 4-bit one, to the same rules. In attention a key's scale multiplies its group's
+ * part of the score and a value's its weight, in F32; a finite key's and query's products stay finite for keys
+ * below 2^115. `table_head_stride` as for hllm_rocm_kv_attention_by_head. */
+hllm_status hllm_rocm_kv4_append(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
+                                 const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
+                                 const hllm_rocm_tensor* v, const hllm_rocm_rope* rope,
+                                 const int32_t* positions, const hllm_rocm_tensor* q,
+                                 const hllm_rocm_tensor* q_out);
+hllm_status hllm_rocm_kv4_read(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
+                               const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k_out,
+                               const hllm_rocm_tensor* v_out);
+hllm_status hllm_rocm_kv4_attention(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
+                                    const hllm_rocm_kv_attention_args* args, uint64_t table_head_stride);
+hllm_status hllm_rocm_kv4_attention_workspace(const hllm_rocm_kv4_pages* pages, uint64_t rows,
+                                              uint32_t query_heads, uint64_t max_length,
+                                              uint64_t* bytes);
 
 #ifdef __cplusplus
 }
