@@ -39,7 +39,8 @@ EXPORTS = ("hllm_rocm_last_error", "hllm_rocm_abi_version", "hllm_rocm_stage_cre
            "hllm_rocm_device_reset_peak", "hllm_rocm_device_query", "hllm_rocm_measure_mfma_rate",
            "hllm_rocm_rope_plan", "hllm_rocm_rope_apply", "hllm_rocm_kv_append", "hllm_rocm_kv_read",
            "hllm_rocm_kv_attention", "hllm_rocm_kv_attention_workspace", "hllm_rocm_kv_attention_by_head",
-           "hllm_rocm_kv4_append", "hllm_rocm_kv4_read", "hllm_rocm_kv4_attention", "hllm_rocm_kv4_attention_workspace")
+           "hllm_rocm_kv4_append", "hllm_rocm_kv4_read", "hllm_rocm_kv4_attention", "hllm_rocm_kv4_attention_workspace",
+           "hllm_rocm_kv_bounds_update", "hllm_rocm_kv4_bounds_update", "hllm_rocm_kv_select", "hllm_rocm_kv_select_workspace")
 NOALLOC_MAX_VOCABULARY = 262144
 
 
@@ -139,6 +140,23 @@ class KvAttentionArgs(C.Structure):
                 ("workspace_bytes", C.c_uint64)]
 
 
+class KvBounds(C.Structure):
+    _fields_ = [("pages", C.c_uint32), ("page_tokens", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dimension", C.c_uint32),
+                ("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class KvBoundsArgs(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("page_table", C.c_void_p), ("table_width", C.c_uint64), ("table_stride", C.c_uint64),
+                ("starts", C.c_void_p), ("lengths", C.c_void_p), ("max_new", C.c_uint64)]
+
+
+class KvSelectArgs(C.Structure):
+    _fields_ = [("rows", C.c_uint64), ("page_table", C.c_void_p), ("table_width", C.c_uint64), ("table_stride", C.c_uint64),
+                ("lengths", C.c_void_p), ("max_length", C.c_uint64), ("keep", C.c_uint32), ("first", C.c_uint32),
+                ("last", C.c_uint32), ("q", Tensor), ("selected", C.c_void_p), ("selected_lengths", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 _LIB = None
 
 
@@ -208,6 +226,10 @@ def library() -> C.CDLL:
     L.hllm_rocm_kv4_read.argtypes = L.hllm_rocm_kv_read.argtypes
     L.hllm_rocm_kv4_attention.argtypes = L.hllm_rocm_kv_attention_by_head.argtypes
     L.hllm_rocm_kv4_attention_workspace.argtypes = L.hllm_rocm_kv_attention_workspace.argtypes
+    L.hllm_rocm_kv_bounds_update.argtypes = [i32, vp, vp, vp, vp]
+    L.hllm_rocm_kv4_bounds_update.argtypes = [i32, vp, vp, vp, vp]
+    L.hllm_rocm_kv_select.argtypes = [i32, vp, vp, vp]
+    L.hllm_rocm_kv_select_workspace.argtypes = [vp, u64, u64, u32, vp]
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is C.c_int or (fn.restype is None and name != "hllm_rocm_stage_destroy"):

@@ -74,17 +74,6 @@ __device__ inline uint32_t encode_four(const float* x, uint32_t most, uint32_t& 
   return w;
 }
 
-// The values of four codes, in F32.
-template <int F>
-__device__ inline floatx4 decode4(uint32_t w) {
-  if constexpr (F == HLLM_KV_E4M3) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    return floatx4{lo[0], lo[1], hi[0], hi[1]};
-  } else {
-    return floatx4{(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24)};
-  }
-}
-
 // ---------------------------------------------------------------- rotary positions
 
 // cos and sin of position x turns, `turns` a 64-bit binary fraction of a turn: the fraction of the
@@ -896,39 +885,6 @@ void check_rotate_grid(uint64_t rows, const RotateArgs& a) {
   if (rows * rotate_blocks(a) > kMostBlocks) refuse("too many rows for these heads");
 }
 
-// A cache of either kind as the entry points take it: T is hllm_rocm_kv_pages or hllm_rocm_kv4_pages.
-template <typename T>
-Cache cache_of(const T* p) {
-  constexpr bool kFour = std::is_same_v<T, hllm_rocm_kv4_pages>;
-  if (!p) refuse("pages is null");
-  if (p->format > 1) refuse("unknown cache format");
-  if (p->head_dimension != 64 && p->head_dimension != 128 && p->head_dimension != 256)
-    refuse("a cache's head dimension is 64, 128 or 256");
-  if (p->kv_heads < 1 || p->kv_heads > 1024) refuse("1 to 1024 key-value heads");
-  if (p->page_tokens < 8 || p->page_tokens > 4096 || (p->page_tokens & (p->page_tokens - 1)))
-    refuse("a page's tokens are a power of two, 8 to 4096");
-  if (p->pages < 1 || (uint64_t)p->pages * p->page_tokens > 0x7fffffffull) refuse("a cache has 1 to 2^31 - 1 slots");
-  if (!p->keys || !p->values || !p->key_scales || !p->value_scales) refuse("a cache's memory is null");
-  if (((uintptr_t)p->keys | (uintptr_t)p->values | (uintptr_t)p->key_scales | (uintptr_t)p->value_scales) % 16)
-    refuse("a cache's memory must be 16-byte aligned");
-  if (p->page_stride >= (1ull << 32) || p->token_stride > (1ull << 28) || p->head_stride > (1ull << 40))
-    refuse("a cache's stride is too large");
-  if ((p->pages > 1 && p->page_stride % 16) || p->token_stride % 16 || (p->kv_heads > 1 && p->head_stride % 16))
-    refuse("a cache's strides must be multiples of 16 bytes");
-  const uint64_t width = kFour ? p->head_dimension / 2 : p->head_dimension;  // bytes of a vector
-  const uint64_t head = p->kv_heads > 1 ? p->head_stride : 0;
-  const uint64_t extent = (p->page_tokens - 1) * p->token_stride + (p->kv_heads - 1) * head + width;
-  if (!apart(width, p->page_tokens, p->token_stride, p->kv_heads, head) ||
-      (p->pages > 1 && p->page_stride < extent))
-    refuse("a cache's vectors overlap");
-  int shift = 0;
-  while ((1u << shift) < p->page_tokens) ++shift;
-  const Pages pages = {static_cast<uint8_t*>(p->keys), static_cast<uint8_t*>(p->values), p->key_scales, p->value_scales,
-                       p->pages > 1 ? (uint32_t)p->page_stride : 0u, (uint32_t)p->token_stride, head, (int32_t)p->pages, shift,
-                       (int32_t)p->kv_heads};
-  return {pages, (int)p->format + (kFour ? kE2m1 : 0), (int)p->head_dimension, p->page_tokens};
-}
-
 void check_rope(const hllm_rocm_rope* rope, uint64_t head_dim) {
   if (!rope) refuse("rope is null");
   if (rope->rotary_dimension < 2 || rope->rotary_dimension > 256 || rope->rotary_dimension % 2 ||
@@ -1174,9 +1130,6 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   p.bytes = p.cuts * sizeof(int2) + p.parts * (cache.head_dim + 2) * sizeof(float);
   return p;
 }
-
-// Positions of one row: sums of a length and a tile's stay below 2^31.
-constexpr uint64_t kMostPositions = 1u << 30;
 
 uint64_t clamp_length(uint64_t max_length) { return std::min(max_length, kMostPositions); }
 

@@ -81,6 +81,35 @@ void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int hea
 // Without the join.
 void launch_kv4_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
 
+struct BoundsArgs {
+  Pages pages;
+  int8_t* codes;           // [pages][kv_heads][2][D]
+  float* scales;           // [pages][kv_heads]
+  const int32_t* table;
+  uint64_t table_stride;
+  const int32_t* starts;   // [rows]: the first position whose page is to be bounded
+  const int32_t* lengths;  // [rows]
+  int32_t rows, limit;
+  int32_t places;          // pages of a row at most
+  int32_t wide;            // a workgroup a page and head
+};
+
+struct SelectArgs {
+  Strided q;
+  const int8_t* codes;
+  const float* scales;
+  const int32_t* table;
+  uint64_t table_stride;
+  const int32_t* lengths;
+  int32_t* selected;          // [rows][kv_heads][keep]
+  int32_t* selected_lengths;  // [rows]
+  uint32_t* keys;             // [rows][kv_heads][stride]: the pages' scores as ordered whole numbers
+  uint64_t stride;
+  int32_t rows, kv_heads, group, pages, page_shift;
+  int32_t limit;              // positions of a row that count at most
+  int32_t keep, first, last;
+};
+
 // Steps (of 128 positions) that starting a pair is counted as. With 1, 2, 3, 4: 128 rows to 8192 positions of head dimension
 // 256 52.8, 52.7, 53.7, 55.2 us; 32 rows to 4096 of 64 14.6, 15.0, 16.0, 16.1; 64 rows to 8192 of 128 43.5, 43.9, 44.1,
 // 44.9; 16 rows to 2048 of 128 13.6, 13.2, 13.4, 14.2.

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "abi.hpp"
 #include "operators.hpp"
@@ -59,6 +60,42 @@ inline void check_apart(const void* a, const char* name_a, const void* b, const 
 
 inline void check_rows(uint64_t rows) {
   if (rows > kMostRows) refuse("at most 1048576 rows a call");
+}
+
+// Positions of one row: sums of a length and a tile's stay below 2^31.
+constexpr uint64_t kMostPositions = 1u << 30;
+
+// A cache of either kind as the entry points take it: T is hllm_rocm_kv_pages or hllm_rocm_kv4_pages.
+template <typename T>
+Cache cache_of(const T* p) {
+  constexpr bool kFour = std::is_same_v<T, hllm_rocm_kv4_pages>;
+  if (!p) refuse("pages is null");
+  if (p->format > 1) refuse("unknown cache format");
+  if (p->head_dimension != 64 && p->head_dimension != 128 && p->head_dimension != 256)
+    refuse("a cache's head dimension is 64, 128 or 256");
+  if (p->kv_heads < 1 || p->kv_heads > 1024) refuse("1 to 1024 key-value heads");
+  if (p->page_tokens < 8 || p->page_tokens > 4096 || (p->page_tokens & (p->page_tokens - 1)))
+    refuse("a page's tokens are a power of two, 8 to 4096");
+  if (p->pages < 1 || (uint64_t)p->pages * p->page_tokens > 0x7fffffffull) refuse("a cache has 1 to 2^31 - 1 slots");
+  if (!p->keys || !p->values || !p->key_scales || !p->value_scales) refuse("a cache's memory is null");
+  if (((uintptr_t)p->keys | (uintptr_t)p->values | (uintptr_t)p->key_scales | (uintptr_t)p->value_scales) % 16)
+    refuse("a cache's memory must be 16-byte aligned");
+  if (p->page_stride >= (1ull << 32) || p->token_stride > (1ull << 28) || p->head_stride > (1ull << 40))
+    refuse("a cache's stride is too large");
+  if ((p->pages > 1 && p->page_stride % 16) || p->token_stride % 16 || (p->kv_heads > 1 && p->head_stride % 16))
+    refuse("a cache's strides must be multiples of 16 bytes");
+  const uint64_t width = kFour ? p->head_dimension / 2 : p->head_dimension;  // bytes of a vector
+  const uint64_t head = p->kv_heads > 1 ? p->head_stride : 0;
+  const uint64_t extent = (p->page_tokens - 1) * p->token_stride + (p->kv_heads - 1) * head + width;
+  if (!apart(width, p->page_tokens, p->token_stride, p->kv_heads, head) ||
+      (p->pages > 1 && p->page_stride < extent))
+    refuse("a cache's vectors overlap");
+  int shift = 0;
+  while ((1u << shift) < p->page_tokens) ++shift;
+  const Pages pages = {static_cast<uint8_t*>(p->keys), static_cast<uint8_t*>(p->values), p->key_scales, p->value_scales,
+                       p->pages > 1 ? (uint32_t)p->page_stride : 0u, (uint32_t)p->token_stride, head, (int32_t)p->pages, shift,
+                       (int32_t)p->kv_heads};
+  return {pages, (int)p->format + (kFour ? kE2m1 : 0), (int)p->head_dimension, p->page_tokens};
 }
 
 // The call's device for its scope.

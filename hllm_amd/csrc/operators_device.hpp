@@ -68,7 +68,18 @@ __device__ inline T* at(const Strided& s, int row, int head, int d) {
   return static_cast<T*>(s.data) + (uint64_t)row * s.row + (uint64_t)head * s.head + d;
 }
 
-// ---------------------------------------------------------------- 4-bit codes
+// ---------------------------------------------------------------- codes
+
+// The values of four codes, in F32.
+template <int F>
+__device__ inline floatx4 decode4(uint32_t w) {
+  if constexpr (F == HLLM_KV_E4M3) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return floatx4{lo[0], lo[1], hi[0], hi[1]};
+  } else {
+    return floatx4{(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24)};
+  }
+}
 
 // INT4 codes, held as code + 8, of the low and of the high four bits of a byte in either half of a word, as F16: beside 0x64 they are
 // the numbers 1024 + n and 1024 + 16 n.

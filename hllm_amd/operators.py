@@ -32,6 +32,8 @@ _SCALES4 = {"e2m1": torch.uint8, "int4": torch.bfloat16}
 # capi.Tensor and capi.KvAttentionArgs as bytes: a quarter of the time of filling a ctypes structure.
 TENSOR = struct.Struct("@PIIQQ")
 ATTENTION_ARGS = struct.Struct("@QPQQPQf4xPIIQQPIIQQPQ")
+BOUNDS_ARGS = struct.Struct("@QPQQPPQ")
+SELECT_ARGS = struct.Struct("@QPQQPQIII4xPIIQQPPPQ")
 _SCALINGS = {
     "linear": (capi.ROPE_LINEAR, ("factor",), ()),
     "llama3": (capi.ROPE_LLAMA3, ("factor", "original_max_position_embeddings", "low_freq_factor",
@@ -173,6 +175,30 @@ class Kv4Pages(_Pages):
             return torch.zeros(pages, kv_heads, page_tokens, head_dim // 32, dtype=_SCALES4[format], device=device)
 
         return cls(codes(), codes(), scales(), scales())
+
+
+class KvBounds:
+    """The bounds of a cache's pages, by which ``kv_select`` selects some of them: for each page and KV head the largest and the
+    smallest key element of every channel, ``codes`` [pages, kv_heads, 2, head_dim] (int8) times ``scales`` [pages,
+    kv_heads] (F32). ``kv_bounds`` makes them. The tensors are held, and must not be resized."""
+
+    def __init__(self, pages: KvPages | Kv4Pages, codes: torch.Tensor, scales: torch.Tensor):
+        shape = (pages.pages, pages.kv_heads, 2, pages.head_dim)
+        for name, x, size, dtype in (("codes", codes, shape, torch.int8), ("scales", scales, shape[:2], torch.float32)):
+            if not isinstance(x, torch.Tensor) or x.device != pages.device or x.dtype != dtype or x.shape != size \
+                    or not x.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dtype} {list(size)} on {pages.device}")
+        self.codes, self.scales, self.device = codes, scales, pages.device
+        self.pages, self.kv_heads, self.head_dim, self.page_tokens = pages.pages, pages.kv_heads, pages.head_dim, pages.page_tokens
+        self.c = capi.KvBounds(self.pages, self.page_tokens, self.kv_heads, self.head_dim, codes.data_ptr(), scales.data_ptr())
+        self.address = C.addressof(self.c)
+        kv_select_workspace(self, 0, 0, 1)  # the library refuses a wrong description here
+
+    @classmethod
+    def empty(cls, pages: KvPages | Kv4Pages):
+        """Bounds for this cache, with nothing made yet."""
+        return cls(pages, torch.zeros(pages.pages, pages.kv_heads, 2, pages.head_dim, dtype=torch.int8, device=pages.device),
+                   torch.zeros(pages.pages, pages.kv_heads, dtype=torch.float32, device=pages.device))
 
 
 def _entry(pages: KvPages | Kv4Pages, name: str, name4: str):
@@ -358,4 +384,77 @@ def kv_attention_workspace(pages: KvPages | Kv4Pages, rows: int, q_heads: int, m
 def _workspace_bytes(pages: KvPages | Kv4Pages, rows: int, q_heads: int, max_length: int) -> int:
     need = C.c_uint64()
     capi.check(_entry(pages, "kv_attention_workspace", "kv4_attention_workspace")(pages.address, rows, q_heads, max_length, C.byref(need)))
+    return need.value
+
+
+def kv_bounds(pages: KvPages | Kv4Pages, bounds: KvBounds, page_table: torch.Tensor, starts: torch.Tensor,
+              lengths: torch.Tensor, max_new: int) -> None:
+    """Makes the bounds of the pages that hold positions ``starts`` .. ``lengths`` - 1 (int32 [rows]) of each row of
+    ``page_table`` [rows, width] (int32), from all of their positions below the length: after these positions were
+    written. ``max_new`` bounds lengths - starts on the host. Rows whose start is not below their length have nothing made."""
+    device = pages.device
+    if bounds.device != device:
+        raise ValueError("the bounds lie on another device than the cache")
+    if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
+        raise ValueError("lengths must be int32 [rows]")
+    rows = lengths.shape[0]
+    table, width, stride, _ = _table(page_table, device, rows)
+    begin, n = _numbers(starts, "starts", device, rows), _numbers(lengths, "lengths", device, rows)
+    if max_new < 0:
+        raise ValueError("max_new is negative")
+    args = BOUNDS_ARGS.pack(rows, table, width, stride, begin, n, min(max_new, width * pages.page_tokens))
+    capi.check(_entry(pages, "kv_bounds_update", "kv4_bounds_update")(device.index, _stream(device), pages.address, bounds.address, args))
+
+
+def kv_select(q: torch.Tensor, bounds: KvBounds, page_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int,
+              first: int = 1, last: int = 1, selected: torch.Tensor | None = None,
+              selected_lengths: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """The ``keep`` pages of each row, for each KV head, that q [rows, q_heads, head_dim] is taken to attend to most: the row's
+    ``first`` first and ``last`` last pages, and those whose bounds allow the largest score of one of the KV head's
+    queries. Returns (pages [rows, kv_heads, keep], lengths [rows], both int32) as ``kv_attention`` takes them, with the bound
+    keep * page_tokens of the lengths: the selected entries of ``page_table`` [rows, width] (int32) in their order, -1
+    behind them. A negative length is passed on, and the row's pages left as they were (in a new output:
+    undefined). ``workspace`` as in ``kv_attention``, of ``kv_select_workspace`` bytes."""
+    device = bounds.device
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be [rows, heads, head_dim]")
+    rows = q.shape[0]
+    a = _fields(q, "q", device, rows, bounds.head_dim)
+    n = _numbers(lengths, "lengths", device, rows)
+    table, width, stride, _ = _table(page_table, device, rows)
+    if max_length < 0:
+        raise ValueError("max_length is negative")
+    if not (0 <= first and 1 <= last and first + last <= keep < 1 << 31):
+        raise ValueError("first is at least 0, last at least 1 and keep at least their sum")
+    max_length = min(max_length, width * bounds.page_tokens)
+    if selected is None:
+        selected = lengths.new_empty((rows, bounds.kv_heads, keep))
+    elif not isinstance(selected, torch.Tensor) or selected.device != device or selected.dtype != torch.int32 \
+            or selected.shape != (rows, bounds.kv_heads, keep) or not selected.is_contiguous():
+        raise ValueError(f"selected must be contiguous int32 [{rows}, {bounds.kv_heads}, {keep}] on {device}")
+    if selected_lengths is None:
+        selected_lengths = torch.empty_like(lengths)
+        to = selected_lengths.data_ptr()
+    else:
+        to = _numbers(selected_lengths, "selected_lengths", device, rows)
+    if workspace is None:
+        need = kv_select_workspace(bounds, rows, max_length, keep)
+        if need:
+            workspace = lengths.new_empty(need, dtype=torch.uint8)
+    elif not isinstance(workspace, torch.Tensor) or workspace.device != device or workspace.dtype != torch.uint8 \
+            or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 on {device}")
+    at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    args = SELECT_ARGS.pack(rows, table, width, stride, n, max_length, keep, first, last, *a, selected.data_ptr(), to, at, size)
+    capi.check(capi.library().hllm_rocm_kv_select(device.index, _stream(device), bounds.address, args))
+    return selected, selected_lengths
+
+
+def kv_select_workspace(bounds: KvBounds, rows: int, max_length: int, keep: int) -> int:
+    """Bytes of workspace that ``kv_select`` needs for these sizes (0: none)."""
+    if min(rows, max_length, keep) < 0:
+        raise ValueError("rows, max_length and keep are not negative")
+    need = C.c_uint64()
+    capi.check(capi.library().hllm_rocm_kv_select_workspace(bounds.address, min(rows, _MOST), min(max_length, _MOST), min(keep, _MOST),
+                                                            C.byref(need)))
     return need.value

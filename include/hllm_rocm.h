@@ -556,6 +556,77 @@ hllm_status hllm_rocm_kv4_attention_workspace(const hllm_rocm_kv4_pages* pages, 
                                               uint32_t query_heads, uint64_t max_length,
                                               uint64_t* bytes);
 
+/* The bounds of a cache's pages, kept by the caller beside the cache: for each page and KV head the largest ([0]) and the
+ * smallest ([1]) key element of each channel over the page's positions, as whole numbers times one power of two, the
+ * smallest that leaves max(|x|max, 2^-100) of both at most 127 times it; x / scale is rounded to nearest even. Elements are
+ * what reading back gives in F32. A page and head with an element that is not finite has codes of 0 and the
+ * scale NaN. Both pointers are 16-byte aligned; sizes are the cache's. */
+typedef struct {
+  uint32_t pages;
+  uint32_t page_tokens;
+  uint32_t kv_heads;
+  uint32_t head_dimension;
+  int8_t* codes;            /* [pages][kv_heads][2][head_dimension] */
+  float* scales;            /* [pages][kv_heads] */
+} hllm_rocm_kv_bounds;
+
+/* Makes the bounds of the pages that hold positions starts[row] .. lengths[row] - 1 of each row (a negative start counts as
+ * 0), from all positions of those pages below lengths[row]: after a write of these positions. A row whose start is not
+ * below its length, and pages outside the cache, have nothing made. At most max_new positions of a row, and
+ * table_width * page_tokens in all, are looked at. Rows may share a page if their lengths agree on it. */
+typedef struct {
+  uint64_t rows;
+  const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */
+  uint64_t table_width;
+  uint64_t table_stride;
+  const int32_t* starts;      /* [rows] */
+  const int32_t* lengths;     /* [rows] */
+  uint64_t max_new;           /* the host's bound of lengths - starts */
+} hllm_rocm_kv_bounds_args;
+
+hllm_status hllm_rocm_kv_bounds_update(int32_t device, void* stream, const hllm_rocm_kv_pages* pages,
+                                       const hllm_rocm_kv_bounds* bounds,
+                                       const hllm_rocm_kv_bounds_args* args);
+hllm_status hllm_rocm_kv4_bounds_update(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
+                                        const hllm_rocm_kv_bounds* bounds,
+                                        const hllm_rocm_kv_bounds_args* args);
+
+/* Selects `keep` pages of each row for each KV head: its first `first` and last `last` pages (last at least 1, first + last at
+ * most keep), and of the others those with the largest scores, of equal scores the first. A page's score is the largest,
+ * over the KV head's query heads, of the sum over channels of max(q high, q low), with q as whole numbers times a power of
+ * two by the bounds' rule: a sum of whole numbers below 2^24, times the page's scale, times the query's, in F32. That is exact
+ * where it is in F32's normal range, so a selection depends on nothing but its row. A score that is NaN (a page or query that is not
+ * finite) is above all others, a page outside the cache below them.
+ *
+ * selected [rows][kv_heads][keep] gets the selected entries of the row's page table in their order, -1 behind them
+ * where the row has fewer pages, and selected_lengths [rows] the positions that they hold: what
+ * hllm_rocm_kv_attention_by_head and hllm_rocm_kv4_attention take as a table of rows kv_heads * keep entries apart
+ * and heads `keep` apart. A row's length counts at most max_length and table_width * page_tokens positions. A
+ * negative length marks a padding row: it is passed on and the row's part of `selected` left as it was. */
+typedef struct {
+  uint64_t rows;
+  const int32_t* page_table;
+  uint64_t table_width;       /* table_width * page_tokens at most 2^30, keep * page_tokens too */
+  uint64_t table_stride;
+  const int32_t* lengths;
+  uint64_t max_length;
+  uint32_t keep;
+  uint32_t first;
+  uint32_t last;
+  hllm_rocm_tensor q;         /* [rows][heads], heads a multiple of the cache's */
+  int32_t* selected;
+  int32_t* selected_lengths;
+  void* workspace;            /* as in hllm_rocm_kv_attention_args, of hllm_rocm_kv_select_workspace bytes */
+  uint64_t workspace_bytes;
+} hllm_rocm_kv_select_args;
+
+hllm_status hllm_rocm_kv_select(int32_t device, void* stream, const hllm_rocm_kv_bounds* bounds,
+                                const hllm_rocm_kv_select_args* args);
+/* The workspace that does for `rows` rows, this max_length or a smaller one and this `keep` or a larger one (0: none). Needs
+ * no device. */
+hllm_status hllm_rocm_kv_select_workspace(const hllm_rocm_kv_bounds* bounds, uint64_t rows,
+                                          uint64_t max_length, uint32_t keep, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -211,3 +211,55 @@ def attended(q, cache, kind, table, lengths, scale, max_length=1 << 31):
             if q.dtype == torch.float16:
                 off[r, mine] += 2.0 ** -25  # F16's subnormals
     return out, off
+
+
+# ------------------------------------------------------------------ selection
+
+
+def whole(x):
+    """(whole numbers of at most 127, powers of two) of vectors x in 64 bits: exact but for the numbers' rounding."""
+    power = two_to(least_power(x.abs().amax(-1, keepdim=True).clamp_min(2.0 ** -100), 127.0))
+    return torch.round(x / power), power.squeeze(-1)
+
+
+def bounds_of(cache, kind, page, head, count):
+    """(codes [2, dim], scale) of one page and KV head with `count` positions."""
+    numbers, scale = (cached[page, head, :count] for cached in parts(cache, kind, "keys"))
+    keys = (numbers * scale).float().double()  # what reading back gives in F32
+    if not torch.isfinite(keys).all():
+        return torch.zeros(2, keys.shape[-1], dtype=torch.int8, device=keys.device), math.nan
+    codes, power = whole(torch.cat((keys.amax(0), keys.amin(0))))
+    return codes.view(2, -1).to(torch.int8), power.item()
+
+
+def selected(q, bounds_codes, bounds_scales, table, lengths, page, keep, first, last, max_length=1 << 31):
+    """(pages [rows, heads, keep], lengths): the selection in 64 bits, in Python. Rows of negative lengths are left -7."""
+    rows, q_heads, dim = q.shape
+    pages, heads = bounds_scales.shape
+    out = torch.full((rows, heads, keep), -7, dtype=torch.int32)
+    new = torch.zeros(rows, dtype=torch.int32)
+    numbers, power = whole(torch.nan_to_num(q.double(), nan=0.0, posinf=0.0, neginf=0.0))
+    power = torch.where(torch.isfinite(q.double()).all(-1), power, math.nan)
+    for r in range(rows):
+        n = min(int(lengths[r]), max_length, table.shape[1] * page)
+        count = -(-n // page)
+        new[r] = n if count <= keep else n - (count - keep) * page
+        if n < 0:
+            continue
+        ids = table[r, :max(count, 0)].long()
+        if count <= keep:
+            out[r] = torch.cat((ids, torch.full((keep - count,), -1, device=ids.device))).int().cpu()
+            continue
+        there = (ids >= 0) & (ids < pages)
+        ids = torch.where(there, ids, 0)
+        for h in range(heads):
+            group = slice(h * q_heads // heads, (h + 1) * q_heads // heads)
+            both = numbers[r, group][:, None, None, :] * bounds_codes[ids, h].double()[None]       # [group, pages, 2, dim]
+            score = both.amax(2).sum(-1) * bounds_scales[ids, h].double() * power[r, group][:, None]
+            score = torch.where(torch.isnan(score).any(0), math.inf, score.amax(0))
+            score = torch.where(there, score, -math.inf).tolist()
+            forced = [p for p in range(count) if p < first or p >= count - last]
+            rest = sorted((p for p in range(count) if first <= p < count - last), key=lambda p: (-score[p], p))
+            places = sorted(forced + rest[:keep - len(forced)])
+            out[r, h] = table[r, places].cpu()
+    return out, new
