@@ -10,22 +10,23 @@ namespace {
 
 // ---------------------------------------------------------------- codes
 
-// Eight codes of a word as F16, which holds every code exactly: E2M1 in order, INT4 with code i beside i + 4.
-template <int F>
+// Eight E2M1 codes of a word times their group's power of two, as BF16.
+__device__ inline bhalf8 scaled8(uint32_t w, float scale) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
+             c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+  return bhalf8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Eight INT4 codes of a word as F16, which holds every code exactly; code i lies beside i + 4.
 __device__ inline half8 halves8(uint32_t w) {
-  half2v x[4];
-  if constexpr (F == kE2m1) {
-    x[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0);
-    x[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1);
-    x[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2);
-    x[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3);
-  } else {
-    x[0] = low_halves(w);
-    x[1] = high_halves(w);
-    x[2] = low_halves(w >> 8);
-    x[3] = high_halves(w >> 8);
-  }
-  return half8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+  const half2v a = low_halves(w), b = high_halves(w), c = low_halves(w >> 8), d = high_halves(w >> 8);
+  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The scale of group g among a position's.
+template <int F>
+__device__ inline float held_scale(const uint32_t* raw, int g) {
+  return scale_of<F>(F == kE2m1 ? raw[g / 4] >> (8 * (g % 4)) & 255u : raw[g / 2] >> (16 * (g % 2)) & 0xffffu);
 }
 
 // ---------------------------------------------------------------- reading back
@@ -78,14 +79,17 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
 
 // ---------------------------------------------------------------- attention
 
-// A wave's tile of N positions in LDS: the codes of keys and of values, then their scales as F32 numbers, each group's N
-// scales together, and each position's largest value scale. A position lies in slot `slot` and a row's
-// sixteen-byte chunks are permuted (chunk k at k ^ swizzle), so that the rows that are read at once, of four eights of
-// positions, lie in different banks, keys and values alike.
-template <int D>
+// A wave's tile of N positions in LDS: the codes of keys and of values, then their scales. A position lies in slot `slot` and a
+// row's sixteen-byte chunks are permuted (chunk k at k ^ swizzle), so that the rows that are read at once, of
+// four eights of positions, lie in different banks, keys and values alike. The keys' scales are kept as they are held (E2M1),
+// or as F32 numbers, each group's N together (INT4). The values' are too: as ratios to a power of two near the largest
+// of the position's, in F16 (16-bit tensors), or as themselves in F32; and that power, or the largest, for each position.
+template <typename T, int F, int D>
 struct Tile4 {
   static constexpr int N = kAttend4Tile<D>, kRow = D / 2, kChunks = kRow / 16, G = D / 32;
-  static constexpr int kCodes = N * kRow, kScales = 2 * kCodes, kLargest = kScales + 2 * G * N * 4;
+  static constexpr bool kRatios = sizeof(T) == 2;
+  static constexpr int kCodes = N * kRow, kScales = 2 * kCodes, kValueScales = kScales + G * N * (F == kE2m1 ? 1 : 4);
+  static constexpr int kLargest = kValueScales + G * N * (kRatios ? 2 : 4);
   static constexpr int kBytes = (std::max(kLargest + N * 4, 64 * D) + 255) / 256 * 256, kBlock = kThreads / 64 * kBytes;
   static constexpr int kGroups = N / 8;   // eights of positions, each in one page
   static constexpr int kCopies = kCodes / 1024;
@@ -112,15 +116,19 @@ struct Tile4 {
 // group: the sixteen rows of an output fragment have one group.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_kernel(AttendArgs a) {
-  using Layout = Tile4<D>;
+  using Layout = Tile4<T, F, D>;
   constexpr int N = Layout::N, G = Layout::G, H = N / 32, kStep = 4 * N;
   constexpr int W = (G + 3) / 4;             // words of a lane's value bytes of a position
   constexpr int SB = F == kE2m1 ? G : 2 * G; // scale bytes of a position
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // F16 parts of a query element and of a weight
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // F16 parts of a weight
+  using Query = std::conditional_t<F == kE2m1, bhalf, _Float16>;
+  constexpr int Q = F == kInt4 ? P : sizeof(T) == 4 ? 3 : std::is_same_v<T, bhalf> ? 1 : 2;  // parts of a query element
+  typedef Query query8 __attribute__((ext_vector_type(8)));
+  constexpr bool kRatios = Layout::kRatios;
   constexpr bool kBoth = N == 32;            // a lane holds a position's key or value scales, not both
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ float states[4][3][16];
-  __shared__ half8 queries[P][G][64];
+  __shared__ query8 queries[Q][G][64];
 
   const Pages& c = a.pages;
   const int KVH = c.kv_heads, shift = c.page_shift, in_row = KVH * a.head_groups;
@@ -211,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 
   // Q^T as the B operand, kept in LDS for the four waves: group g's lane (col, quad) holds elements 32 g + 8 quad + j in the order of
   // halves8. Each vector is divided by the power of two of its largest element, which puts F32 and BF16
-  // ranges into F16's and goes back into its scores.
+  // ranges into F16's and goes back into its scores. E2M1 keys take it as one to three BF16 numbers, its eight, eleven or 24 bits.
   float factor, factor_lo;
   {
     float x[G][8];
@@ -236,15 +244,18 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     if (wave == 0) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        half8 part[P];
+        query8 part[Q];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = x[g][F == kE2m1 ? j : (j >> 1) + 4 * (j & 1)] * down;
-          part[0][j] = (_Float16)y;
-          if constexpr (P == 2) part[1][j] = (_Float16)(y - (float)part[0][j]);
+          float y = x[g][F == kE2m1 ? j : (j >> 1) + 4 * (j & 1)] * down;
+#pragma unroll
+          for (int p = 0; p < Q; ++p) {
+            part[p][j] = (Query)y;
+            y -= (float)part[p][j];
+          }
         }
 #pragma unroll
-        for (int p = 0; p < P; ++p) queries[p][g][lane] = part[p];
+        for (int p = 0; p < Q; ++p) queries[p][g][lane] = part[p];
       }
     }
   }
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   float m = -INFINITY, l = 0.0f, r = 0.0f;
   bool any = false;  // whether the wave has had a position
   float* key_scale = reinterpret_cast<float*>(tile + Layout::kScales);
-  float* value_scale = key_scale + G * N;
+  char* value_scale = tile + Layout::kValueScales;
   float* largest_scale = reinterpret_cast<float*>(tile + Layout::kLargest);
 
   for (; t < end; t += kStep) {
@@ -267,25 +278,46 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     const bool whole = gone == 0 && t + N <= end;
     any |= gone != (1 << Layout::kGroups) - 1;  // eights behind the end count as the last one's page
     {
-      // The lane's scales as F32 numbers; positions past the part and in pages that are not there have none.
+      // The lane's scales. Values past the part and in pages that are not there have none.
       const bool counts = whole || (t + own < end && !(gone >> (own >> 3) & 1));
-      const auto keep = [&](const uint32_t* raw, float* to) {
-        float most = 0.0f;
+      const auto keep_keys = [&](const uint32_t* raw) {
+        if constexpr (F == kE2m1) {
+          char* to = tile + Layout::kScales + G * own;
+          if constexpr (G == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)raw[0];
+          if constexpr (G == 4) *reinterpret_cast<uint32_t*>(to) = raw[0];
+          if constexpr (G == 8) *reinterpret_cast<uint2v*>(to) = uint2v{raw[0], raw[1]};
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; ++g) key_scale[g * N + own] = held_scale<F>(raw, g);
+        }
+      };
+      const auto keep_values = [&](const uint32_t* raw) {
+        float v[G], most = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const uint32_t w = F == kE2m1 ? raw[g / 4] >> (8 * (g % 4)) & 255u : raw[g / 2] >> (16 * (g % 2)) & 0xffffu;
-          const float s = counts ? scale_of<F>(w) : 0.0f;
-          to[g * N] = s;
-          most = fmaxf(most, fabsf(s));  // NaN is not taken
+          v[g] = counts ? held_scale<F>(raw, g) : 0.0f;
+          most = fmaxf(most, fabsf(v[g]));  // NaN is not taken
         }
-        return most;
+        if constexpr (kRatios) {
+          const uint32_t power = max(__float_as_uint(most) >> 23, 1u);
+          largest_scale[own] = __uint_as_float(power << 23);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            reinterpret_cast<_Float16*>(value_scale)[g * N + own] = (_Float16)__builtin_amdgcn_ldexpf(v[g], 127 - (int)power);
+        } else {
+          largest_scale[own] = most;
+#pragma unroll
+          for (int g = 0; g < G; ++g) reinterpret_cast<float*>(value_scale)[g * N + own] = v[g];
+        }
       };
       if constexpr (kBoth) {
-        const float most = keep(held[0], (lane < 32 ? key_scale : value_scale) + own);
-        if (lane >= 32) largest_scale[own] = most;
+        if (lane < 32)
+          keep_keys(held[0]);
+        else
+          keep_values(held[0]);
       } else {
-        keep(held[0], key_scale + own);
-        largest_scale[own] = keep(held[1], value_scale + own);
+        keep_keys(held[0]);
+        keep_values(held[1]);
       }
     }
     // The tile's positions in thirty-twos, one after the other.
@@ -293,24 +325,49 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     for (int s = 0; s < H; ++s) {
       // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are positions 8 quad .. + 7, which are
       // also its slots of the value products.
-      float d[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       const int half = s * Layout::kHalf;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        half8 q[P];
-#pragma unroll
-        for (int p = 0; p < P; ++p) q[p] = queries[p][g][lane];
+      float d[8];
+      if constexpr (F == kE2m1) {
+        // A key's elements as BF16, which holds every code times its scale exactly.
+        floatx4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        uint32_t by[2][W];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const half8 k = halves8<F>(*reinterpret_cast<const uint32_t*>(
-              tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
-          floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int p = P - 1; p >= 0; --p) x = mfma(k, q[p], x);
-          const floatx4 by = *reinterpret_cast<const floatx4*>(key_scale + g * N + 32 * s + 8 * quad + 4 * h);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[4 * h + i] = fmaf(x[i], by[i], d[4 * h + i]);
+          const char* at = tile + Layout::kScales + G * (32 * s + 8 * (col >> 2) + 4 * h + (col & 3));
+          if constexpr (G == 2) by[h][0] = *reinterpret_cast<const uint16_t*>(at);
+          if constexpr (G == 4) by[h][0] = *reinterpret_cast<const uint32_t*>(at);
+          if constexpr (G == 8) {
+            const uint2v w = *reinterpret_cast<const uint2v*>(at);
+            by[h][0] = w[0], by[h][1] = w[1];
+          }
         }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bhalf8 k = scaled8(*reinterpret_cast<const uint32_t*>(tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)),
+                                     __uint_as_float((by[h][g / 4] >> (8 * (g % 4)) & 255u) << 23));
+#pragma unroll
+            for (int p = Q - 1; p >= 0; --p) x[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, queries[p][g][lane], x[h], 0, 0, 0);
+          }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = x[j >> 2][j & 3];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const half8 k = halves8(*reinterpret_cast<const uint32_t*>(
+                tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
+            floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = Q - 1; p >= 0; --p) x = mfma(k, queries[p][g][lane], x);
+            const floatx4 by = *reinterpret_cast<const floatx4*>(key_scale + g * N + 32 * s + 8 * quad + 4 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[4 * h + i] = fmaf(x[i], by[i], d[4 * h + i]);
+          }
       }
       uint32_t vw[8][W];
 #pragma unroll
@@ -350,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       for (int j = 0; j < 8; ++j) {
         weight[j] = exp2_fast(P == 2 ? (sc[j] - base) + by_lo[j] : sc[j] - base);
         sum += weight[j];
-        largest = fmaxf(largest, weight[j] * ls[j]);
+        ls[j] *= weight[j];
+        largest = fmaxf(largest, ls[j]);
       }
       l = l * decay + sum;
       m = m_new;
@@ -363,8 +421,15 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
         r = raised;
       }
       const float over = r > 0x1p-125f ? __builtin_amdgcn_rcpf(r) : 0.0f;  // smaller weights are nothing
+      // Weights with the power of two of their value's scales, as F16; or by themselves, to be multiplied by each scale.
+      half8 ratio_weight;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) weight[j] *= over;
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (kRatios)
+          ratio_weight[j] = (_Float16)(ls[j] * over);
+        else
+          weight[j] *= over;
+      }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         // Two positions' codes are paired. E2M1: pairs[e] holds code e (of two) of both in each group's byte; INT4: pairs[k] both
@@ -384,17 +449,21 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 #pragma unroll
         for (int gw = 0; gw < (G < 4 ? G : 4); ++gw) {
           const int g = 4 * w + gw;
-          float vs[8];
-          load8(value_scale + g * N + 32 * s + 8 * quad, vs);
           half8 pf[P];
+          if constexpr (kRatios) {
+            pf[0] = ratio_weight * *reinterpret_cast<const half8*>(value_scale + 2 * (g * N + 32 * s + 8 * quad));
+          } else {
+            float vs[8];
+            load8(reinterpret_cast<const float*>(value_scale) + g * N + 32 * s + 8 * quad, vs);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float x = weight[j] * vs[j];
-            // As a value of its own: rounded with the product in one step, the first part would differ
-            // from the one that the second part is the rest of.
-            if constexpr (P == 2) asm("" : "+v"(x));
-            pf[0][j] = (_Float16)x;
-            if constexpr (P == 2) pf[1][j] = (_Float16)(x - (float)pf[0][j]);
+            for (int j = 0; j < 8; ++j) {
+              float x = weight[j] * vs[j];
+              // As a value of its own: rounded with the product in one step, the first part would differ
+              // from the one that the second part is the rest of.
+              asm("" : "+v"(x));
+              pf[0][j] = (_Float16)x;
+              pf[P - 1][j] = (_Float16)(x - (float)pf[0][j]);
+            }
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -489,7 +558,7 @@ void kv4_read(hipStream_t stream, int head_dim, const ReadArgs& a) {
 
 template <typename T, int F, int D>
 void attend4(hipStream_t stream, const AttendArgs& a) {
-  constexpr int kLds = Tile4<D>::kBlock;
+  constexpr int kLds = Tile4<T, F, D>::kBlock;
   static std::atomic<uint64_t> asked{0};
   ask_for_lds(reinterpret_cast<const void*>(&kv4_attention_kernel<T, F, D>), kLds, asked);
   kv4_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);

@@ -167,12 +167,17 @@ def attended(q, cache, kind, table, lengths, scale, max_length=1 << 31):
     largest (2^-22 of each for two parts), dim roundings of the products' sums, one for each group's scale (8 at most) and 4 more,
     2 ulp of exp2 and 4 roundings of the score (base 2) itself. The weight is multiplied twice more (the
     reciprocal of the scaling, the value's scale): 4 roundings. Sums over positions round at most once for each 32
-    positions and 64 times in all joins."""
+    positions and 64 times in all joins.
+
+    16-bit tensors: the F16 weight has a power of two of its position's scales and is multiplied by the group's ratio to
+    it, in F16. E2M1: a power of two, at most 1, so there is no second rounding. INT4: the ratio has eight bits and is below 2, so
+    the product is rounded once more, and what is lost below the normal range is 2 * 2^-25 + 2^-25."""
     rows, q_heads, dim = q.shape
     pages, heads, page = cache["keys"].shape[:3]
     out = torch.full(q.shape, math.nan, dtype=torch.float64, device=q.device)
     off = torch.zeros_like(out)
     two = q.dtype == torch.float32
+    again = kind == "int4" and not two
     kn, ks = parts(cache, kind, "keys")
     vn, vs = parts(cache, kind, "values")
     group = q_heads // heads
@@ -199,12 +204,12 @@ def attended(q, cache, kind, table, lengths, scale, max_length=1 << 31):
             o = p @ v
             size = (qd.abs() @ k.abs()) * abs(scale)
             lost = (qd.abs().amax(-1, keepdim=True) * k.abs().sum(0)) * abs(scale) * 2.0 ** -25
-            rounding = 2.0 ** -22 if two else 2.0 ** -11
+            rounding = 2.0 ** -22 if two else 2.0 ** -10 if again else 2.0 ** -11
             e = lost + size * ((dim + 12) * 2.0 ** -24 + (2.0 ** -22 if two else 0.0))
             e = e + 4 * 2.0 ** -24 * (score - score.amax(-1, keepdim=True)).abs() + 4 * 2.0 ** -24 * score.abs().amax(-1, keepdim=True)
             e = e.amax(-1, keepdim=True) + 2.0 ** -22
             total = 2 * e + rounding + (len(at) / 32 + 68) * 2.0 ** -24
-            least = (p * w.abs().amax(-1)).amax(-1, keepdim=True) * 2.0 ** -25
+            least = (p * w.abs().amax(-1)).amax(-1, keepdim=True) * (3 if again else 1) * 2.0 ** -25
             bound = total * (p @ v.abs()) + least * vc.abs().sum(0)
             out[r, mine] = o
             off[r, mine] = bound + HALF_STEP[q.dtype] * (o.abs() + bound)

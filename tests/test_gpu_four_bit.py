@@ -243,3 +243,248 @@ def test_kv_attention_of_peaked_scores_and_uneven_values(ops, dim, dtype):
 @pytest.mark.parametrize("kind", KINDS)
 def test_kv_attention_of_large_and_small_queries(ops, kind, dtype, q_scale):
     attend_case(ops, kind, dtype, [70, 400], 8, 2, 128, 64, q_scale=q_scale, scale=0.05 / max(q_scale, 1e-30))
+
+
+# ------------------------------------------------------------------ numbers that are none, masks, sizes
+
+
+def cut(ops, pages, lengths, q_heads, most):
+    """Whether a call with these rows cuts pairs (a call that does not has no workspace)."""
+    return ops.kv_attention_workspace(pages, len(lengths), q_heads, most) > 0
+
+
+def not_finite(kind, x):
+    """The scale that stands for NaN, in scales x as held."""
+    return 255 if kind == "e2m1" else math.nan
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_stays_nan_where_work_is_cut(ops, kind, dtype, dim):
+    """A NaN in a query or in key scales makes that head's (or KV head's) output NaN; in value scales, their groups' elements; and
+    nothing else, at bounds of the lengths that cut a row and that do not."""
+    lengths, page = [5000, 40, 3000], 64
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim)
+    pages = ops.Kv4Pages(**cache)
+    q = draw(3, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
+
+    def check(q, bad):
+        for most in (5000, 2048, 300):
+            out = ops.kv_attention(q, pages, table, n, most)
+            assert torch.equal(torch.isnan(out), bad.expand_as(out)), most
+
+    bad = torch.zeros(3, 8, 1, dtype=torch.bool, device="cuda")
+    check(q, bad)
+    wrong = q.clone()
+    wrong[0, 3, 9] = math.nan
+    wrong[1, 7, 0] = math.nan
+    wrong[2] = math.nan
+    bad[0, 3] = bad[1, 7] = bad[2] = True
+    check(wrong, bad)
+    before = {x: cache[x].clone() for x in ("key_scales", "value_scales")}
+    cache["key_scales"][table[0].long(), 1, :, 1] = not_finite(kind, None)
+    cache["key_scales"][table[2, 2].long(), 0, 5:9, 0] = not_finite(kind, None)
+    if kind == "int4":
+        cache["key_scales"][table[1, 0].long(), 0, 7, 1] = -math.inf
+    bad[:] = False
+    bad[0, 4:] = bad[2, :4] = True
+    bad[1, :4] = kind == "int4"
+    check(q, bad)
+    cache["key_scales"].copy_(before["key_scales"])
+    bad = torch.zeros(3, 8, dim, dtype=torch.bool, device="cuda")
+    cache["value_scales"][table[0, 1].long(), 1, 3, 1] = not_finite(kind, None)
+    cache["value_scales"][table[2, 0].long(), 0] = not_finite(kind, None)
+    bad[0, 4:, 32:64] = bad[2, :4] = True
+    # The position's own value has no group left that is a number: NaN still, of the whole vector, and of no other position's.
+    check(q, bad)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("infinity", [math.inf, -math.inf])
+def test_infinite_queries_give_nan(ops, kind, dtype, infinity):
+    """Scores that are all infinite, of either sign, have no softmax: NaN, whether a row is cut or not; rows
+    without positions stay zeros."""
+    lengths, page = [5000, 40, 0, 700], 32
+    table, count = paged(lengths, page)
+    table[3] = -1
+    cache = forms.make_pages(kind, count, 2, page, 128)
+    cache["keys"][..., 4] = 0x33 if kind == "e2m1" else 0xbb  # elements 8 and 9: positive numbers
+    pages = ops.Kv4Pages(**cache)
+    q = draw(4, 8, 128, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert cut(ops, pages, lengths, 8, 5000) and not cut(ops, pages, lengths, 8, 300)
+    for most in (5000, 300):
+        clean = ops.kv_attention(q, pages, table, n, most)
+        assert not torch.isnan(clean).any()
+        wrong = q.clone()
+        wrong[:, 2, 9] = infinity
+        out = ops.kv_attention(wrong, pages, table, n, most)
+        assert torch.isnan(out[:2, 2]).all() and (out[2:] == 0).all()
+        out[:, 2] = clean[:, 2] = 0
+        assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_near_the_largest_number(ops, kind, dtype, dim):
+    """Means of values up to 1.3e38 are finite, though sums of three of them are not."""
+    lengths, page = [5000, 300, 2, 9000], 32
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim)
+    if kind == "e2m1":
+        cache["values"].copy_(cache["values"] & 0x77 | 0x44)     # 2 .. 6
+        cache["value_scales"].fill_(127 + 124)                     # times 2.1e37
+    else:
+        cache["values"].copy_(cache["values"] & 0x33 | 0xcc)     # 4 .. 7
+        cache["value_scales"].copy_((0.5 + cache["value_scales"]) * 1.8e37)
+    q = draw(4, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    pages = ops.Kv4Pages(**cache)
+    assert cut(ops, pages, lengths, 8, 9000)
+    for most in (9000, 300):
+        expect, off = forms.attended(q, cache, kind, table, lengths, dim ** -0.5, most)
+        assert expect.max() > 6e37
+        near(ops.kv_attention(q, pages, table, n, most), expect, off)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", KINDS)
+def test_groups_of_very_different_scales(ops, kind, dim, dtype):
+    """Groups of one vector, and vectors of one row, up to 2^20 and 2^40 apart, in keys and in values; INT4 scales of
+    either sign; E2M1's smallest and largest."""
+    lengths, page = [300, 1, 2000, 63], 16
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+
+    def exponents(least, most):
+        vector = torch.randint(least, most, cache["keys"].shape[:3], generator=g, device="cuda")
+        return vector[..., None] + torch.randint(-10, 11, cache["key_scales"].shape, generator=g, device="cuda")
+
+    def held(e):
+        if kind == "e2m1":
+            return (e + 127).to(torch.uint8)
+        sign = torch.randint(0, 2, e.shape, generator=g, device="cuda") * 2 - 1
+        return (sign * (1 + torch.rand(e.shape, generator=g, device="cuda")) * 2.0 ** e).to(torch.bfloat16)
+
+    cache["key_scales"].copy_(held(exponents(-14, -12)))
+    cache["value_scales"].copy_(held(exponents(-20, 20) - (9 if dtype == torch.float16 else 0)))
+    if kind == "e2m1":
+        cache["value_scales"][table[0, 3].long(), 0, 2] = 0
+        if dtype != torch.float16:
+            cache["value_scales"][table[2, 5].long(), 1, 7, 1] = 127 + 125
+    q = draw(4, 8, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for scale in (dim ** -0.5, 0.0):
+        out = ops.kv_attention(q, ops.Kv4Pages(**cache), table, n, 2000, scale=scale)
+        expect, off = forms.attended(q, cache, kind, table, lengths, scale)
+        fits = expect.abs() + off < torch.finfo(dtype).max
+        assert fits.float().mean() > 0.9
+        near(torch.where(fits, out, 0), torch.where(fits, expect, 0.0), off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_pairs_of_more_than_64_parts(ops, kind, dtype, dim):
+    """A pair that most workgroups share, whose first two thirds hold nothing."""
+    lengths, page = [300000], 64
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 1, page, dim, stale=True)
+    forms.fill(cache, kind, table, lengths)
+    q = draw(1, 4, dim, dtype, 1)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    pages = ops.Kv4Pages(**cache)
+    near(ops.kv_attention(q, pages, table, n, 300000), *forms.attended(q, cache, kind, table, lengths, dim ** -0.5))
+    table[0, :3200] = -1
+    near(ops.kv_attention(q, pages, table, n, 300000), *forms.attended(q, cache, kind, table, lengths, dim ** -0.5))
+
+
+@pytest.mark.parametrize("kind,dtype,dim", [("e2m1", torch.float16, 128), ("int4", torch.bfloat16, 256), ("e2m1", torch.float32, 64),
+                                            ("int4", torch.float32, 256)])
+@pytest.mark.parametrize("lengths", [
+    [10000] + [0, -1, 5, 40] * 16, [3, 0] * 32 + [8191], [-1] * 129 + [6000], [130, 1] * 40 + [12000, -1, 7000] + [0] * 47,
+    [9000] + [20, -1, 0, 129, 3] * 139 + [-1, 2500, 1, 0], [-1, 64] * 511 + [20000, 9], [0] * 500 + [26000] + [1] * 523,
+    ([3, 0, 70, -1, 600] * 220)[:1090]])
+def test_shares_of_many_rows(ops, kind, dtype, dim, lengths):
+    attend_case(ops, kind, dtype, lengths, 2, 1, dim, 16)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128), (torch.float32, 128), (torch.float16, 256)])
+@pytest.mark.parametrize("q_heads,heads", [(20, 1), (40, 2), (17, 1), (64, 1)])
+def test_groups_of_more_than_sixteen_heads(ops, kind, dtype, dim, q_heads, heads):
+    for lengths in ([5000], [129, 20000, -1, 0, 6400]):
+        attend_case(ops, kind, dtype, lengths, q_heads, heads, dim, 32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_kv_attention_leaves_out_dropped_pages(ops, kind):
+    """Positions of pages that are not in the cache count as masked: some of a row's, then all."""
+    for page, dim in ((8, 64), (16, 128), (64, 256)):
+        lengths = [300, 5, 1000, 640]
+        table, count = paged(lengths, page)
+        table[0, 1::3] = -1
+        table[2, : 1000 // page // 2] = count  # past the cache
+        table[2, -1] = 2 ** 31 - 1
+        table[3] = -7
+        cache = forms.make_pages(kind, count, 2, page, dim, stale=True)
+        forms.fill(cache, kind, table, lengths)
+        q = draw(4, 6, dim, torch.float16, 1)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        out = ops.kv_attention(q, ops.Kv4Pages(**cache), table, n, 1000)
+        near(out, *forms.attended(q, cache, kind, table, lengths, dim ** -0.5))
+        assert (out[3] == 0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_page_offsets_past_32_bits(ops, kind):
+    """A cache of more than 4 GiB of codes: written, read, bounded and attended at its end."""
+    page, heads, dim = 4096, 8, 128
+    count = (1 << 32) // (page * heads * dim // 2) + 3
+    pages = ops.Kv4Pages.empty(kind, count, heads, page, dim)
+    small = ops.Kv4Pages.empty(kind, 3, heads, page, dim)
+    rows = 300
+    k, v, q = draw(rows, heads, dim, torch.float16, 1), draw(rows, heads, dim, torch.float16, 2), draw(1, 16, dim, torch.float16, 3)
+    at = torch.arange(rows, dtype=torch.int32, device="cuda") + page - 100
+    ops.kv_append(pages, at + (count - 3) * page, k, v)
+    ops.kv_append(small, at, k, v)
+    for x, y in zip(ops.kv_read(pages, at + (count - 3) * page), ops.kv_read(small, at)):
+        assert torch.equal(x, y)
+    n = torch.tensor([page + 200], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.kv_attention(q, pages, table + count - 3, n, page + 200), ops.kv_attention(q, small, table, n, page + 200))
+    a, b = ops.KvBounds.empty(pages), ops.KvBounds.empty(small)
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.kv_bounds(pages, a, table + count - 3, zero, n, page + 200)
+    ops.kv_bounds(small, b, table, zero, n, page + 200)
+    assert torch.equal(a.codes[-3:], b.codes) and torch.equal(a.scales[-3:], b.scales) and b.codes[:2].any(-1).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_views(ops, kind):
+    """Heads of one projection's rows, strided outputs, rows that repeat memory, a table inside a wider one."""
+    lengths, dim = [100, 0, 400, 33], 128
+    q, pages, table, n, most, out = attend_case(ops, kind, torch.float16, lengths, 8, 2, dim, 16)
+    joint = draw(4, 20, dim, torch.float16, 9)
+    joint[:, 3:11] = q
+    wide = torch.full((4, 12, dim), 7.0, dtype=torch.float16, device="cuda")
+    big = torch.full((4, table.shape[1] + 9), -1, dtype=torch.int32, device="cuda")
+    big[:, 2:2 + table.shape[1]] = table
+    assert torch.equal(ops.kv_attention(joint[:, 3:11], pages, big[:, 2:2 + table.shape[1]], n, most, out=wide[:, 2:10]), out)
+    assert (wide[:, :2] == 7).all() and (wide[:, 10:] == 7).all()
+    k = joint[:, 12:14]
+    slots = torch.arange(4, dtype=torch.int32, device="cuda") * 5
+    fresh, plain = (ops.Kv4Pages.empty(kind, 2, 2, 16, dim) for _ in range(2))
+    ops.kv_append(fresh, slots, k, k[:1].expand(4, 2, dim))
+    ops.kv_append(plain, slots, k.contiguous(), k[:1].repeat(4, 1, 1))
+    for name in ("keys", "values", "key_scales", "value_scales"):
+        assert torch.equal(getattr(fresh, name), getattr(plain, name))
