@@ -88,7 +88,8 @@ template <typename T, int F, int D>
 struct Tile4 {
   static constexpr int N = kAttend4Tile<D>, kRow = D / 2, kChunks = kRow / 16, G = D / 32;
   static constexpr bool kRatios = sizeof(T) == 2;
-  static constexpr int kCodes = N * kRow, kScales = 2 * kCodes, kValueScales = kScales + G * N * (F == kE2m1 ? 1 : 4);
+  static constexpr int kBuffers = kAttend4Buffers<D>;
+  static constexpr int kCodes = N * kRow, kScales = kBuffers * 2 * kCodes, kValueScales = kScales + G * N * 4;
   static constexpr int kLargest = kValueScales + G * N * (kRatios ? 2 : 4);
   static constexpr int kBytes = (std::max(kLargest + N * 4, 64 * D) + 255) / 256 * 256, kBlock = kThreads / 64 * kBytes;
   static constexpr int kGroups = N / 8;   // eights of positions, each in one page
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     }
   };
   // Starts a tile's copies and loads its scales; returns a bit for each eight whose page is not there.
-  const auto copy_tile = [&](int t, int id) {
+  const auto copy_tile = [&](int t, int id, int buffer) {
     const bool there = id >= 0 && id < c.pages;
     const uint64_t absent = __ballot(!there);
     const int page = there ? id : 0;
@@ -199,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     for (int i = 0; i < Layout::kCopies; ++i) {
       const int chunk = (lane % Layout::kChunks) ^ Layout::swizzle(eight, offset0 + i * kOffsets);
       const uint8_t* at = from + (uint64_t)(i * kOffsets) * token + chunk * 16;
-      lds_stream16_at(at, tile_at + i * 1024);
-      lds_stream16_at(at + values_at, tile_at + Layout::kCodes + i * 1024);
+      lds_stream16_at(at, tile_at + buffer + i * 1024);
+      lds_stream16_at(at + values_at, tile_at + buffer + Layout::kCodes + i * 1024);
     }
     const uint8_t* at = scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + own) & mask)) * SB;
     load_scales(held[0], at);
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 
   int t = begin + N * wave, missing = 0, id = 0;
   if (t < end) {
-    missing = copy_tile(t, page_of(t));
+    missing = copy_tile(t, page_of(t), 0);
     id = page_of(min(t + kStep, end - 1));
   }
 
@@ -267,11 +268,13 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 #pragma unroll
   for (int f = 0; f < 2 * G; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f, r = 0.0f;
+  int unit = -1000;  // 16-bit tensors: the exponent of the value scales' unit
   bool any = false;  // whether the wave has had a position
   float* key_scale = reinterpret_cast<float*>(tile + Layout::kScales);
   char* value_scale = tile + Layout::kValueScales;
   float* largest_scale = reinterpret_cast<float*>(tile + Layout::kLargest);
 
+  int buffer = 0;
   for (; t < end; t += kStep) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int gone = missing;
@@ -282,16 +285,18 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       const bool counts = whole || (t + own < end && !(gone >> (own >> 3) & 1));
       const auto keep_keys = [&](const uint32_t* raw) {
         if constexpr (F == kE2m1) {
-          char* to = tile + Layout::kScales + G * own;
-          if constexpr (G == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)raw[0];
-          if constexpr (G == 4) *reinterpret_cast<uint32_t*>(to) = raw[0];
-          if constexpr (G == 8) *reinterpret_cast<uint2v*>(to) = uint2v{raw[0], raw[1]};
+          float v[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) v[g] = __uint_as_float((raw[g / 4] >> (8 * (g % 4)) & 255u) << 23);
+          if constexpr (G == 2) *reinterpret_cast<float2*>(key_scale + G * own) = float2{v[0], v[1]};
+#pragma unroll
+          for (int g = 0; g + 3 < G; g += 4) *reinterpret_cast<floatx4*>(key_scale + G * own + g) = floatx4{v[g], v[g + 1], v[g + 2], v[g + 3]};
         } else {
 #pragma unroll
           for (int g = 0; g < G; ++g) key_scale[g * N + own] = held_scale<F>(raw, g);
         }
       };
-      const auto keep_values = [&](const uint32_t* raw) {
+      const auto keep_values = [&](const uint32_t* raw, bool mine) {
         float v[G], most = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -299,27 +304,41 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           most = fmaxf(most, fabsf(v[g]));  // NaN is not taken
         }
         if constexpr (kRatios) {
-          const uint32_t power = max(__float_as_uint(most) >> 23, 1u);
-          largest_scale[own] = __uint_as_float(power << 23);
+          const int power = mine ? max((int)(__float_as_uint(most) >> 23), 1) : 0;
+          if (__any(power > unit + 60)) {
+            int top = power;
+            for (int step = 1; step < 64; step <<= 1) top = max(top, __shfl_xor(top, step, 64));
+            top = __builtin_amdgcn_readfirstlane(top);
+            const float rescale = __builtin_amdgcn_ldexpf(1.0f, max(unit - top, -300));
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-            reinterpret_cast<_Float16*>(value_scale)[g * N + own] = (_Float16)__builtin_amdgcn_ldexpf(v[g], 127 - (int)power);
-        } else {
+            for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
+            unit = top;
+          }
+          if (mine) {
+            largest_scale[own] = __uint_as_float((uint32_t)max(power - unit + 127, 1) << 23);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+              reinterpret_cast<_Float16*>(value_scale)[g * N + own] = (_Float16)__builtin_amdgcn_ldexpf(v[g], 127 - power);
+          }
+        } else if (mine) {
           largest_scale[own] = most;
 #pragma unroll
           for (int g = 0; g < G; ++g) reinterpret_cast<float*>(value_scale)[g * N + own] = v[g];
         }
       };
-      if constexpr (kBoth) {
-        if (lane < 32)
-          keep_keys(held[0]);
-        else
-          keep_values(held[0]);
-      } else {
-        keep_keys(held[0]);
-        keep_values(held[1]);
-      }
+      if (!kBoth || lane < 32) keep_keys(held[0]);
+      keep_values(held[kBoth ? 0 : 1], !kBoth || lane >= 32);
     }
+    const char* codes = tile + buffer;
+    const auto next_tile = [&] {
+      if (t + kStep < end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (Layout::kBuffers > 1) buffer = 2 * Layout::kCodes - buffer;
+        missing = copy_tile(t + kStep, id, buffer);
+        id = page_of(min(t + 2 * kStep, end - 1));
+      }
+    };
+    if constexpr (Layout::kBuffers > 1) next_tile();
     // The tile's positions in thirty-twos, one after the other.
 #pragma unroll 1
     for (int s = 0; s < H; ++s) {
@@ -330,23 +349,27 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       if constexpr (F == kE2m1) {
         // A key's elements as BF16, which holds every code times its scale exactly.
         floatx4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        uint32_t by[2][W];
+        float by[2][G];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const char* at = tile + Layout::kScales + G * (32 * s + 8 * (col >> 2) + 4 * h + (col & 3));
-          if constexpr (G == 2) by[h][0] = *reinterpret_cast<const uint16_t*>(at);
-          if constexpr (G == 4) by[h][0] = *reinterpret_cast<const uint32_t*>(at);
-          if constexpr (G == 8) {
-            const uint2v w = *reinterpret_cast<const uint2v*>(at);
-            by[h][0] = w[0], by[h][1] = w[1];
+          const float* at = key_scale + G * (32 * s + 8 * (col >> 2) + 4 * h + (col & 3));
+          if constexpr (G == 2) {
+            const float2 w = *reinterpret_cast<const float2*>(at);
+            by[h][0] = w.x, by[h][1] = w.y;
+          }
+#pragma unroll
+          for (int g = 0; g + 3 < G; g += 4) {
+            const floatx4 w = *reinterpret_cast<const floatx4*>(at + g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) by[h][g + i] = w[i];
           }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const bhalf8 k = scaled8(*reinterpret_cast<const uint32_t*>(tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)),
-                                     __uint_as_float((by[h][g / 4] >> (8 * (g % 4)) & 255u) << 23));
+            const bhalf8 k = scaled8(
+                *reinterpret_cast<const uint32_t*>(codes + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)), by[h][g]);
 #pragma unroll
             for (int p = Q - 1; p >= 0; --p) x[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, queries[p][g][lane], x[h], 0, 0, 0);
           }
@@ -360,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const half8 k = halves8(*reinterpret_cast<const uint32_t*>(
-                tile + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
+                codes + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
             floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int p = Q - 1; p >= 0; --p) x = mfma(k, queries[p][g][lane], x);
@@ -372,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       uint32_t vw[8][W];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const char* line = tile + Layout::kCodes + Layout::at(quad, j, G * col, half);
+        const char* line = codes + Layout::kCodes + Layout::at(quad, j, G * col, half);
         if constexpr (G == 2) vw[j][0] = *reinterpret_cast<const uint16_t*>(line);
         if constexpr (G == 4) vw[j][0] = *reinterpret_cast<const uint32_t*>(line);
         if constexpr (G == 8) {
@@ -382,53 +405,87 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
         }
       }
       // The tile is in registers: the next one's copies start.
-      if (s == H - 1 && t + kStep < end) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        missing = copy_tile(t + kStep, id);
-        id = page_of(min(t + 2 * kStep, end - 1));
-      }
-      // F32 tensors keep the scores' factor as a sum of two floats and round a score once, after the maximum is taken away.
-      float sc[8], by_lo[8], most = -INFINITY;
+      if (Layout::kBuffers == 1 && s == H - 1) next_tile();
       const int valid = whole ? 8 : gone >> (4 * s + quad) & 1 ? 0 : end - (t + 32 * s + 8 * quad);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sc[j] = d[j] * factor;
-        if constexpr (P == 2)
-          by_lo[j] = j >= valid || sc[j] == -INFINITY ? 0.0f : fmaf(d[j], factor, -sc[j]) + d[j] * factor_lo;
-        sc[j] = j < valid ? sc[j] : -INFINITY;
-        most = fmaxf(most, sc[j]);
-      }
-      const float m_new = fmaxf(m, column_max(most));
-      const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float decay = exp2_fast(m - base);
-      float weight[8], ls[8], sum = 0.0f, largest = 0.0f;
-      load8(largest_scale + 32 * s + 8 * quad, ls);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        weight[j] = exp2_fast(P == 2 ? (sc[j] - base) + by_lo[j] : sc[j] - base);
-        sum += weight[j];
-        ls[j] *= weight[j];
-        largest = fmaxf(largest, ls[j]);
-      }
-      l = l * decay + sum;
-      m = m_new;
-      r *= decay;
-      largest = column_max(largest);
-      if (__any(largest > 4096.0f * r)) {
-        const float raised = fmaxf(r, largest), rescale = raised > r ? r / raised : 1.0f;
-#pragma unroll
-        for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
-        r = raised;
-      }
-      const float over = r > 0x1p-125f ? __builtin_amdgcn_rcpf(r) : 0.0f;  // smaller weights are nothing
-      // Weights with the power of two of their value's scales, as F16; or by themselves, to be multiplied by each scale.
+      float weight[8], ls[8];
       half8 ratio_weight;
+      load8(largest_scale + 32 * s + 8 * quad, ls);
+      if constexpr (kRatios) {
+        // Weights are 2^(score - m) for an m that is seldom changed: where a wave's first scores are found, and where a weight times its
+        // value scales (in `unit`s) is above 2^12, or a weight above 2^100. So most tiles need no
+        // maximum, and F16 holds every weight to 2^-11 or to 2^-25 of the largest.
+        float sum, largest;
+        const auto weigh = [&] {
+          const float base = m == -INFINITY ? 0.0f : m;
+          sum = largest = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (kRatios)
-          ratio_weight[j] = (_Float16)(ls[j] * over);
-        else
-          weight[j] *= over;
+          for (int j = 0; j < 8; ++j) weight[j] = exp2_fast(fmaf(d[j], factor, -base));
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) weight[j] = j < valid ? weight[j] : 0.0f;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum += weight[j];
+            const float w = weight[j] * ls[j];
+            largest = fmaxf(largest, w);
+            ratio_weight[j] = (_Float16)w;
+          }
+        };
+        weigh();
+        const bool raise = largest > 4096.0f || sum > 0x1p100f || m == -INFINITY;
+        if (__any(raise)) {
+          float top = -INFINITY, high = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float sc = j < valid ? d[j] * factor : -INFINITY;
+            top = fmaxf(top, sc);
+            high = fmaxf(high, sc + (float)((int)(__float_as_uint(ls[j]) >> 23) - 127));
+          }
+          // Of the columns that need it: a head's sums do not depend on the heads beside it.
+          const bool own_raise = column_max(raise ? 1.0f : 0.0f) > 0.0f;
+          const float raised = own_raise ? fmaxf(m, fmaxf(column_max(high), column_max(top) - 100.0f)) : m;
+          const float rescale = raised == m ? 1.0f : exp2_fast(m - raised);
+#pragma unroll
+          for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
+          l *= rescale;
+          m = raised;
+          weigh();
+        }
+        l += sum;
+      } else {
+        // F32 tensors keep the scores' factor as a sum of two floats and round a score once, after the maximum is taken away.
+        float sc[8], by_lo[8], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sc[j] = d[j] * factor;
+          by_lo[j] = j >= valid || sc[j] == -INFINITY ? 0.0f : fmaf(d[j], factor, -sc[j]) + d[j] * factor_lo;
+          sc[j] = j < valid ? sc[j] : -INFINITY;
+          most = fmaxf(most, sc[j]);
+        }
+        const float m_new = fmaxf(m, column_max(most));
+        const float base = m_new == -INFINITY ? 0.0f : m_new;
+        const float decay = exp2_fast(m - base);
+        float sum = 0.0f, largest = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          weight[j] = exp2_fast((sc[j] - base) + by_lo[j]);
+          sum += weight[j];
+          largest = fmaxf(largest, weight[j] * ls[j]);
+        }
+        l = l * decay + sum;
+        m = m_new;
+        r *= decay;
+        largest = column_max(largest);
+        if (__any(largest > 4096.0f * r)) {
+          const float raised = fmaxf(r, largest), rescale = raised > r ? r / raised : 1.0f;
+#pragma unroll
+          for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
+          r = raised;
+        }
+        const float over = r > 0x1p-125f ? __builtin_amdgcn_rcpf(r) : 0.0f;  // smaller weights are nothing
+#pragma unroll
+        for (int j = 0; j < 8; ++j) weight[j] *= over;
       }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
@@ -492,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   }
 
   // The four waves' states meet in LDS, each wave's in its own tile.
+  if constexpr (kRatios) r = unit < 0 ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127);
   l = column_sum(l);
   // Only scores of -inf (an infinite query's): a sum that is not 0 beside that maximum tells them from no positions.
   if (any && l == 0.0f) l = 1.0f;

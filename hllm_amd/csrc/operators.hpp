@@ -122,10 +122,17 @@ constexpr uint64_t kMostSharedRows = 1024;
 template <int D>
 constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
 // Over a 4-bit cache: positions of a wave's tile, and workgroups on a CU.
+#ifndef A4T
+#define A4T D == 256 ? 32 : 64
+#define A4BUF 1
+#define A4BL D == 64 ? 4 : D == 128 ? 3 : 2
+#endif
 template <int D>
-constexpr int kAttend4Tile = D == 256 ? 32 : 64;
+constexpr int kAttend4Tile = A4T;
 template <int D>
-constexpr int kAttend4Blocks = D == 64 ? 4 : D == 128 ? 3 : 2;
+constexpr int kAttend4Buffers = A4BUF;
+template <int D>
+constexpr int kAttend4Blocks = A4BL;
 inline uint64_t attend_blocks(int format, int head_dim, bool f32) {
   if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : kAttend4Blocks<256>);
   return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : f32 ? 1 : kAttendBlocks<256>);
