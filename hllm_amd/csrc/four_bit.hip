@@ -88,8 +88,7 @@ template <typename T, int F, int D>
 struct Tile4 {
   static constexpr int N = kAttend4Tile<D>, kRow = D / 2, kChunks = kRow / 16, G = D / 32;
   static constexpr bool kRatios = sizeof(T) == 2;
-  static constexpr int kBuffers = kAttend4Buffers<D>;
-  static constexpr int kCodes = N * kRow, kScales = kBuffers * 2 * kCodes, kValueScales = kScales + G * N * 4;
+  static constexpr int kCodes = N * kRow, kScales = 4 * kCodes, kValueScales = kScales + G * N * 4;
   static constexpr int kLargest = kValueScales + G * N * (kRatios ? 2 : 4);
   static constexpr int kBytes = (std::max(kLargest + N * 4, 64 * D) + 255) / 256 * 256, kBlock = kThreads / 64 * kBytes;
   static constexpr int kGroups = N / 8;   // eights of positions, each in one page
@@ -107,6 +106,13 @@ struct Tile4 {
     return D == 64 ? first ^ half : first + half;
   }
 };
+
+// Which pair or share a workgroup takes. The workgroups of a cluster, whose pairs read the same cache lines, take the same share of
+// each of them, at once and on the same of the card's eight dies, round which workgroups go and which have a cache each.
+__device__ inline int place_of(const AttendArgs& a, int block) {
+  const int die = block & 7, i = block >> 3;
+  return ((i / a.cluster) * 8 + die) * a.cluster + i % a.cluster;
+}
 
 // As kv_attention_kernel (operators.hip): a pair's scores S = K Q^T and sums O^T = V^T P are products on the matrix units,
 // with the softmax's running maximum and sum in F32. What differs comes from the scales that 32 elements of a
@@ -135,15 +141,18 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   const int KVH = c.kv_heads, shift = c.page_shift, in_row = KVH * a.head_groups;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int quad = lane >> 4, col = lane & 15;
-  const int me = blockIdx.x;
-  Share<kStep> share;
-  if (!share.first_pair(a, in_row, me, lane)) return;
+  const int place = place_of(a, blockIdx.x);
+  if (place >= a.blocks) return;
+  // Shares are counted in clusters.
+  const int cluster = a.cluster, me = place / cluster, member = place - me * cluster;
+  Share<kStep, kPair4Cost> share;
+  if (!share.first_pair(a, in_row / cluster, me, a.blocks / cluster, lane)) return;
 
   bool again = false;
-  for (bool more = true; more; more = share.next_pair(a, in_row)) {
-  const int row = share.row, kvg = share.kvg, length = share.length;
+  for (bool more = true; more; more = share.next_pair(a, in_row / cluster)) {
+  const int row = share.row, kvg = share.kvg * cluster + member, length = share.length;
   // This share's steps of the pair, low .. high - 1, and the workgroups that have others.
-  const int steps = steps_of<kStep>(length), first_unit = share.start + kPairCost;
+  const int steps = steps_of<kStep>(length), first_unit = share.start + kPair4Cost;
   const int low = max(share.from - first_unit, 0), high = min(steps, share.to - first_unit);
   if (steps > 0 ? low >= high : share.start < share.from) continue;  // only the cost of starting it is this share's
   const int first = first_unit / share.budget;
@@ -200,8 +209,13 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     for (int i = 0; i < Layout::kCopies; ++i) {
       const int chunk = (lane % Layout::kChunks) ^ Layout::swizzle(eight, offset0 + i * kOffsets);
       const uint8_t* at = from + (uint64_t)(i * kOffsets) * token + chunk * 16;
-      lds_stream16_at(at, tile_at + buffer + i * 1024);
-      lds_stream16_at(at + values_at, tile_at + buffer + Layout::kCodes + i * 1024);
+      if (cluster > 1) {
+        lds_copy16_at(at, tile_at + buffer + i * 1024);
+        lds_copy16_at(at + values_at, tile_at + buffer + Layout::kCodes + i * 1024);
+      } else {
+        lds_stream16_at(at, tile_at + buffer + i * 1024);
+        lds_stream16_at(at + values_at, tile_at + buffer + Layout::kCodes + i * 1024);
+      }
     }
     const uint8_t* at = scales + ((((uint64_t)page * KVH + kvh) << shift) + ((t + own) & mask)) * SB;
     load_scales(held[0], at);
@@ -261,6 +275,16 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     }
   }
   __syncthreads();
+
+  // Where they are few, in registers.
+  constexpr bool kHeld = Q * G <= 4;
+  query8 held_q[kHeld ? Q : 1][kHeld ? G : 1];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int p = 0; p < Q; ++p) held_q[p][g] = queries[p][g][lane];
+  }
 
   // Weights, their scaling by r and the sums o as in kv_attention_kernel, r by each position's largest value scale.
   // o[2 g + e]'s row c is element 32 g + 2 c + e.
@@ -333,18 +357,32 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     const auto next_tile = [&] {
       if (t + kStep < end) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if constexpr (Layout::kBuffers > 1) buffer = 2 * Layout::kCodes - buffer;
+        buffer = 2 * Layout::kCodes - buffer;
         missing = copy_tile(t + kStep, id, buffer);
         id = page_of(min(t + 2 * kStep, end - 1));
       }
     };
-    if constexpr (Layout::kBuffers > 1) next_tile();
+    next_tile();
     // The tile's positions in thirty-twos, one after the other.
 #pragma unroll 1
     for (int s = 0; s < H; ++s) {
       // Score fragment h's row 4 q + i is position 8 q + 4 h + i: a lane's scores are positions 8 quad .. + 7, which are
       // also its slots of the value products.
       const int half = s * Layout::kHalf;
+      // What a product needs is read from LDS well before it: a read takes as long as some thirty instructions.
+      uint32_t kw[G][2];
+      query8 q[kHeld ? 1 : Q][kHeld ? 1 : G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          kw[g][h] = *reinterpret_cast<const uint32_t*>(codes + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half));
+        if constexpr (!kHeld) {
+#pragma unroll
+          for (int p = 0; p < Q; ++p) q[p][g] = queries[p][g][lane];
+        }
+      }
+      const auto query = [&](int p, int g) { return kHeld ? held_q[kHeld ? p : 0][kHeld ? g : 0] : q[kHeld ? 0 : p][kHeld ? 0 : g]; };
       float d[8];
       if constexpr (F == kE2m1) {
         // A key's elements as BF16, which holds every code times its scale exactly.
@@ -364,32 +402,36 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
             for (int i = 0; i < 4; ++i) by[h][g + i] = w[i];
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const bhalf8 k = scaled8(
-                *reinterpret_cast<const uint32_t*>(codes + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)), by[h][g]);
+            const bhalf8 k = scaled8(kw[g][h], by[h][g]);
 #pragma unroll
-            for (int p = Q - 1; p >= 0; --p) x[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, queries[p][g][lane], x[h], 0, 0, 0);
+            for (int p = Q - 1; p >= 0; --p) x[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(p, g), x[h], 0, 0, 0);
           }
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] = x[j >> 2][j & 3];
       } else {
+        floatx4 by[G][2];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) by[g][h] = *reinterpret_cast<const floatx4*>(key_scale + g * N + 32 * s + 8 * quad + 4 * h);
+        if constexpr (G <= 4) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const half8 k = halves8(*reinterpret_cast<const uint32_t*>(
-                codes + Layout::at(col >> 2, 4 * h + (col & 3), 16 * g + 4 * quad, half)));
+            const half8 k = halves8(kw[g][h]);
             floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int p = Q - 1; p >= 0; --p) x = mfma(k, queries[p][g][lane], x);
-            const floatx4 by = *reinterpret_cast<const floatx4*>(key_scale + g * N + 32 * s + 8 * quad + 4 * h);
+            for (int p = Q - 1; p >= 0; --p) x = mfma(k, query(p, g), x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[4 * h + i] = fmaf(x[i], by[i], d[4 * h + i]);
+            for (int i = 0; i < 4; ++i) d[4 * h + i] = fmaf(x[i], by[g][h][i], d[4 * h + i]);
           }
       }
       uint32_t vw[8][W];
@@ -404,12 +446,15 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           vw[j][1] = w[1];
         }
       }
-      // The tile is in registers: the next one's copies start.
-      if (Layout::kBuffers == 1 && s == H - 1) next_tile();
       const int valid = whole ? 8 : gone >> (4 * s + quad) & 1 ? 0 : end - (t + 32 * s + 8 * quad);
       float weight[8], ls[8];
-      half8 ratio_weight;
+      half8 ratio_weight, ratios[kRatios ? G : 1];
       load8(largest_scale + 32 * s + 8 * quad, ls);
+      if constexpr (kRatios) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) ratios[g] = *reinterpret_cast<const half8*>(value_scale + 2 * (g * N + 32 * s + 8 * quad));
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if constexpr (kRatios) {
         // Weights are 2^(score - m) for an m that is seldom changed: where a wave's first scores are found, and where a weight times its
         // value scales (in `unit`s) is above 2^12, or a weight above 2^100. So most tiles need no
@@ -508,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           const int g = 4 * w + gw;
           half8 pf[P];
           if constexpr (kRatios) {
-            pf[0] = ratio_weight * *reinterpret_cast<const half8*>(value_scale + 2 * (g * N + 32 * s + 8 * quad));
+            pf[0] = ratio_weight * ratios[g];
           } else {
             float vs[8];
             load8(reinterpret_cast<const float*>(value_scale) + g * N + 32 * s + 8 * quad, vs);
@@ -597,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       store4(out + v * a.out.head + dim, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
     } else {
       if (undefined) total = 1.0f;  // NaN in the join, unless another part has finite scores
-      const uint64_t part = part_at(a, first, me - first, v);
+      const uint64_t part = part_at(a, first, me - first, member, v);
       *reinterpret_cast<floatx4*>(a.part + part * D + dim) = y;
       if (dim == 0) *reinterpret_cast<float2*>(a.stats + 2 * part) = float2{top, total};
     }
@@ -619,7 +664,8 @@ void attend4(hipStream_t stream, const AttendArgs& a) {
   constexpr int kLds = Tile4<T, F, D>::kBlock;
   static std::atomic<uint64_t> asked{0};
   ask_for_lds(reinterpret_cast<const void*>(&kv4_attention_kernel<T, F, D>), kLds, asked);
-  kv4_attention_kernel<T, F, D><<<a.blocks, kThreads, kLds, stream>>>(a);
+  const int round = 8 * a.cluster;
+  kv4_attention_kernel<T, F, D><<<(a.blocks + round - 1) / round * round, kThreads, kLds, stream>>>(a);
 }
 
 template <typename T, int F>

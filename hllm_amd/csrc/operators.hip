@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int quad = lane >> 4, col = lane & 15;
   const int me = blockIdx.x;
-  Share<128> share;
-  if (!share.first_pair(a, in_row, me, lane)) return;
+  Share<128, kPairCost> share;
+  if (!share.first_pair(a, in_row, me, (int)gridDim.x, lane)) return;
 
   bool again = false;
   for (bool more = true; more; more = share.next_pair(a, in_row)) {
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       store4(out + v * a.out.head + d, undefined ? floatx4{NAN, NAN, NAN, NAN} : y);
     } else {
       if (undefined) total = 1.0f;  // NaN in the join, unless another part has finite scores
-      const uint64_t part = part_at(a, first, me - first, v);
+      const uint64_t part = part_at(a, first, me - first, 0, v);
       *reinterpret_cast<floatx4*>(a.part + part * D + d) = y;
       if (d == 0) *reinterpret_cast<float2*>(a.stats + 2 * part) = float2{top, total};
     }
@@ -730,10 +730,10 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
   const int row = vector / a.q_heads, head = vector - row * a.q_heads, kvh = head / a.group, g = head - kvh * a.group;
   const int length = uniform_load(a.lengths + row);
   const int2 cut = uniform_cut(a.cuts + (row * a.pages.kv_heads + kvh) * a.head_groups + g / 16);
-  const int first = cut.x, parts = cut.y;
+  const int first = cut.x, parts = cut.y, member = (kvh * a.head_groups + g / 16) % a.cluster;
   if (min(length, a.limit) <= 0 || parts <= 1) return;  // a row without positions has no cut there
   const int v = g % 16, slot = lane / kLanes, d = lane % kLanes * 4;
-  const auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.stats + 2 * part_at(a, first, min(i, parts - 1), v)); };
+  const auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.stats + 2 * part_at(a, first, min(i, parts - 1), member, v)); };
   floatx4 y = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, total = 0.0f;
   bool held = false;
@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(AttendArgs a) {
       floatx4 x[kDeep];
 #pragma unroll
       for (int j = 0; j < kDeep; ++j)
-        x[j] = *reinterpret_cast<const floatx4*>(a.part + part_at(a, first, i0 + min(j0 + j * kSlots + slot, n - 1), v) * D + d);
+        x[j] = *reinterpret_cast<const floatx4*>(a.part + part_at(a, first, i0 + min(j0 + j * kSlots + slot, n - 1), member, v) * D + d);
       if (j0 == 0) {
         // The first lanes hold the parts: as many steps as those take, and the result from lane 0.
         for (int o = 1; o < n; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
@@ -1089,7 +1089,7 @@ void read(int32_t device, void* stream, const Cache& cache, const int32_t* slots
 // How a call's work is cut and what its workspace holds: each pair's cut, then outputs and statistics of
 // two parts of each workgroup.
 struct AttendPlan {
-  uint64_t head_groups = 1, blocks = 0, cuts = 0, parts = 0, bytes = 0;
+  uint64_t head_groups = 1, cluster = 1, blocks = 0, cuts = 0, parts = 0, bytes = 0;
   bool shared = false;
 };
 
@@ -1101,7 +1101,13 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   if (rows == 0) return p;
   const uint64_t group = query_heads / kv_heads;
   p.head_groups = (group + 15) / 16;
-  const uint64_t step = attend_step(cache.format, cache.head_dim), steps = (limit + step - 1) / step, cost = kPairCost + steps;
+  // Pairs beside each other that read the same cache lines: sixteens of a KV head's query heads, and heads within 128 bytes.
+  if (four_bits(cache.format)) {
+    const uint64_t stride = cache.pages.head_stride, beside = stride > 0 && stride < 128 ? 128 / stride : 1;
+    p.cluster = p.head_groups * (kv_heads % beside == 0 ? beside : 1);
+    if (p.cluster > 16) p.cluster = 1;
+  }
+  const uint64_t step = attend_step(cache.format, cache.head_dim), steps = (limit + step - 1) / step, cost = attend_cost(cache.format) + steps;
   const uint64_t pairs = rows * kv_heads * p.head_groups;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
   // A workgroup for each pair where rows are short or pairs many: no row has more steps than 5 and 9 for each
@@ -1117,13 +1123,17 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   // there) and for F32 heads of 256. Rows that are padding count as pairs, for the host does not know them: 16
   // rows to 8000 take 21.8, with 48 padding rows 22.0, with 900, where pairs stay whole, 73.
   const uint64_t fit = attend_blocks(cache.format, cache.head_dim, false);
-  const bool whole = steps * fit <= 5 * fit + 9 * pairs;
+  bool whole = steps * fit <= 5 * fit + 9 * pairs;
+  if (four_bits(cache.format)) {
+    const uint64_t most = cache.head_dim == 256 ? 600 : 750;
+    whole = 5 * limit * fit <= most * (5 * fit + 8 * std::min(pairs, fit * 5 / 4));
+  }
   p.blocks = pairs;
   if (whole || rows > kMostSharedRows) return p;
   // The line of all pairs is counted in 31 bits. Where it could be longer the pairs stay whole, but the
   // workspace is that of shares: a bound of the lengths is never given less than a smaller bound.
   p.shared = pairs <= (1u << 30) / cost;
-  const uint64_t sharing = std::min<uint64_t>(fit, pairs * cost);
+  const uint64_t sharing = std::min<uint64_t>(fit / p.cluster, pairs / p.cluster * cost) * p.cluster;
   if (p.shared) p.blocks = sharing;
   p.cuts = (pairs + 1) / 2 * 2;  // whole sixteen bytes
   p.parts = 2 * sharing * std::min<uint64_t>(group, 16);
@@ -1174,8 +1184,9 @@ void attend(int32_t device, void* stream, const Cache& cache, const hllm_rocm_kv
   a.limit = (int32_t)limit;
   // F32 queries take twice the LDS.
   const bool f32 = args->q.dtype == HLLM_DTYPE_F32;
-  a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks(cache.format, (int)D, f32)) : plan.blocks);
+  a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks(cache.format, (int)D, f32) / plan.cluster * plan.cluster) : plan.blocks);
   a.shared = plan.shared;
+  a.cluster = (int32_t)plan.cluster;
   a.scale_hi = (float)(args->scale * kLog2e);
   a.scale_lo = (float)(args->scale * kLog2e - a.scale_hi);
   if (plan.shared) {

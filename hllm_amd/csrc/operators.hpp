@@ -71,6 +71,7 @@ struct AttendArgs {
   int32_t head_groups;           // sixteens of a KV head's query heads
   int32_t limit;                 // positions of a row that count at most
   int32_t blocks;                // workgroups
+  int32_t cluster;               // pairs that follow one another and read the same cache lines; pairs are a multiple of it
   int32_t shared;                // the rows' work is cut into the workgroups' shares (else a pair each)
   float scale_hi, scale_lo;      // the scores' scale times log2 e as a sum of two floats
   int2* cuts;                    // [pairs]: the first workgroup and the number of its parts (null: no pair is cut)
@@ -122,21 +123,19 @@ constexpr uint64_t kMostSharedRows = 1024;
 template <int D>
 constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
 // Over a 4-bit cache: positions of a wave's tile, and workgroups on a CU.
-#ifndef A4T
-#define A4T D == 256 ? 32 : 64
-#define A4BUF 1
-#define A4BL D == 64 ? 4 : D == 128 ? 3 : 2
+#ifndef A4COST
+#define A4COST 2
 #endif
+constexpr int kPair4Cost = A4COST;
 template <int D>
-constexpr int kAttend4Tile = A4T;
+constexpr int kAttend4Tile = D == 64 ? 64 : 32;
 template <int D>
-constexpr int kAttend4Buffers = A4BUF;
-template <int D>
-constexpr int kAttend4Blocks = A4BL;
+constexpr int kAttend4Blocks = D == 256 ? 2 : 3;
 inline uint64_t attend_blocks(int format, int head_dim, bool f32) {
-  if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : kAttend4Blocks<256>);
+  if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : f32 ? 1 : kAttend4Blocks<256>);
   return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : f32 ? 1 : kAttendBlocks<256>);
 }
+inline int attend_cost(int format) { return four_bits(format) ? kPair4Cost : kPairCost; }
 // Positions of a step: one tile for each of a workgroup's four waves.
 inline uint64_t attend_step(int format, int head_dim) {
   if (!four_bits(format)) return 128;

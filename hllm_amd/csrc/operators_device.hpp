@@ -160,6 +160,14 @@ __device__ inline void lds_stream16_at(const void* from, uint32_t lds_byte_offse
                : "memory", "m0");
 #pragma clang diagnostic pop
 }
+// ... of lines that another workgroup of the die reads as well.
+__device__ inline void lds_copy16_at(const void* from, uint32_t lds_byte_offset) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds_byte_offset)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
 __device__ inline void lds_stream4_at(const void* from, uint32_t lds_byte_offset) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -178,30 +186,30 @@ __device__ inline int wave_scan(int v, int lane, int count) {
 }
 
 // The pairs (a row, a KV head, sixteen of its query heads) lie on a line, each as long as its steps of kStep
-// positions (one tile a wave) and kPairCost more for starting it, and the line is cut into equal
+// positions (one tile a wave) and kCost more for starting it, and the line is cut into equal
 // shares: a workgroup may end one pair, take whole ones and begin another.
 template <int kStep>
 __device__ inline int steps_of(int length) {
   return (length + kStep - 1) / kStep;
 }
-template <int kStep>
+template <int kStep, int kCost>
 __device__ inline int pair_units(int length) {
-  return length < 0 ? 0 : steps_of<kStep>(length) + kPairCost;
+  return length < 0 ? 0 : steps_of<kStep>(length) + kCost;
 }
 
-// Where vector v of a pair's part i lies in the workspace. A workgroup writes two parts at most: of a pair
-// that began before it and of one that goes on after it.
-__device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int v) {
-  return (uint64_t)(i == 0 ? 2 * first + 1 : 2 * (first + i)) * min(a.group, 16) + v;
+// Where vector v of a pair's part i lies in the workspace. A share has two parts at most: of a pair
+// that began before it and of one that goes on after it; and those of each of a cluster's pairs.
+__device__ inline uint64_t part_at(const AttendArgs& a, int first, int i, int member, int v) {
+  return (uint64_t)((i == 0 ? 2 * first + 1 : 2 * (first + i)) * a.cluster + member) * min(a.group, 16) + v;
 }
 
 // A workgroup's share, units from .. to of the line, and the pair it is at. Without `shared` a workgroup takes one pair.
-template <int kStep>
+template <int kStep, int kCost>
 struct Share {
   int row, kvg, start, from = 0, to, budget = INT_MAX, length, units;
 
-  // The share's first pair; false where there is none. in_row: pairs of a row.
-  __device__ inline bool first_pair(const AttendArgs& a, int in_row, int me, int lane) {
+  // The share's first pair; false where there is none. in_row: pairs of a row; me: which of the `blocks` shares.
+  __device__ inline bool first_pair(const AttendArgs& a, int in_row, int me, int blocks, int lane) {
     if (a.shared) {
       const int chunk = (a.rows + 63) / 64, lanes = (a.rows + chunk - 1) / chunk;  // rows of a lane, at most 16
       int own = 0, own_length = 0;
@@ -209,12 +217,12 @@ struct Share {
         const int r = lane * chunk + i;
         if (r < a.rows) {
           own_length = min(a.lengths[r], a.limit);
-          own += pair_units<kStep>(own_length) * in_row;
+          own += pair_units<kStep, kCost>(own_length) * in_row;
         }
       }
       int sum = wave_scan(own, lane, lanes);
       const int total = __builtin_amdgcn_readlane(sum, lanes - 1);
-      budget = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+      budget = (total + blocks - 1) / blocks;
       from = me * budget;
       to = min(from + budget, total);
       if (from >= to) return false;
@@ -223,14 +231,14 @@ struct Share {
       start = __builtin_amdgcn_readlane(sum - own, at);
       if (chunk > 1) {
         own_length = min(a.lengths[min(row + lane, a.rows - 1)], a.limit);
-        own = lane < chunk && row + lane < a.rows ? pair_units<kStep>(own_length) * in_row : 0;
+        own = lane < chunk && row + lane < a.rows ? pair_units<kStep, kCost>(own_length) * in_row : 0;
         sum = start + wave_scan(own, lane, chunk);
         at = __builtin_ctzll(__ballot(sum > from));
         row += at;
         start = __builtin_amdgcn_readlane(sum - own, at);
       }
       length = __builtin_amdgcn_readlane(own_length, at);
-      units = pair_units<kStep>(length);
+      units = pair_units<kStep, kCost>(length);
       kvg = (from - start) / units;
       start += kvg * units;
     } else {
@@ -238,7 +246,7 @@ struct Share {
       kvg = me - row * in_row;
       start = 0;
       length = min(uniform_load(a.lengths + row), a.limit);
-      to = units = pair_units<kStep>(length);
+      to = units = pair_units<kStep, kCost>(length);
       if (units == 0) return false;
     }
     return true;
@@ -251,7 +259,7 @@ struct Share {
     kvg = 0;
     do {
       length = min(uniform_load(a.lengths + ++row), a.limit);
-      units = pair_units<kStep>(length);
+      units = pair_units<kStep, kCost>(length);
     } while (units == 0);
     return true;
   }

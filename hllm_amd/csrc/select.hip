@@ -173,8 +173,8 @@ __device__ inline uint32_t row_max(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + O, 0xf, 0xf, false));
 }
 
-// The scores of a row's pages for one KV head, as ordered whole numbers: keep(page's place, number). A wave takes sixteen pages at once,
-// from tile `first` on in steps of `step`: with a query's positive and negative elements apart, the sum over channels of the larger product
+// The scores of a row's pages for one KV head, as ordered whole numbers: keep(page's place, number). A wave takes sixty-four pages at once,
+// from sixty-four `first` on in steps of `step`: with a query's positive and negative elements apart, the sum over channels of the larger product
 // is one product [high, low] x [max(q, 0), min(q, 0)] of twice the length, on the matrix units in bytes, with the query heads of a KV
 // head as columns. Sums of whole numbers below 2^24 and powers of two are exact.
 template <typename T, int D, typename Keep>
@@ -215,36 +215,50 @@ __device__ inline void score_pages(const SelectArgs& a, int row, int kvh, int co
         up[kk][2 * i] = (int)pw[0], up[kk][2 * i + 1] = (int)pw[1];
         down[kk][2 * i] = (int)nw[0], down[kk][2 * i + 1] = (int)nw[1];
       }
-    for (int t = first; 16 * t < count; t += step) {
-      const int id = table[min(16 * t + col, count - 1)];
+    // 64 pages at a time, a lane's one of them, whose loads are under way together: in two halves where their bounds take many registers.
+    for (int t = 64 * first; t < count; t += 64 * step) {
+      const int id = table[min(t + lane, count - 1)];
       const bool there = id >= 0 && id < a.pages;
-      const uint64_t page = (uint64_t)(there ? id : 0) * a.kv_heads + kvh;
-      const int8_t* from = a.codes + page * (2 * D) + 16 * quad;
-      int4v high[KK], low[KK];
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        high[kk] = *reinterpret_cast<const int4v*>(from + 64 * kk);
-        low[kk] = *reinterpret_cast<const int4v*>(from + D + 64 * kk);
-      }
-      const float scale = a.scales[page];
-      int4v dot = {0, 0, 0, 0};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[kk], up[kk], dot, 0, 0, 0);
-        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[kk], down[kk], dot, 0, 0, 0);
-      }
       const uint64_t absent = __ballot(!there);
-      uint32_t mine = 0;
+      const int own = there ? id : 0;
+      const float scale = a.scales[(uint64_t)own * a.kv_heads + kvh];
+      constexpr int kTiles = KK < 4 ? 4 : 2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float by = __shfl(scale, 4 * quad + i, 64);
-        uint32_t v = col < vectors ? ordered((float)dot[i] * by * q_scale) : 0u;
-        v = row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
-        if (absent >> (4 * quad + i) & 1) v = 0;
-        if (col == i) mine = v;
+      for (int part = 0; part < 4; part += kTiles) {
+        int4v high[kTiles][KK], low[kTiles][KK];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          const uint64_t page = (uint64_t)__shfl(own, 16 * (part + i) + col, 64) * a.kv_heads + kvh;
+          const int8_t* from = a.codes + page * (2 * D) + 16 * quad;
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            high[i][kk] = *reinterpret_cast<const int4v*>(from + 64 * kk);
+            low[i][kk] = *reinterpret_cast<const int4v*>(from + D + 64 * kk);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          int4v dot = {0, 0, 0, 0};
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[i][kk], up[kk], dot, 0, 0, 0);
+            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[i][kk], down[kk], dot, 0, 0, 0);
+          }
+          uint32_t mine = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int of = 16 * (part + i) + 4 * quad + e;
+            const float by = __shfl(scale, of, 64);
+            uint32_t v = col < vectors ? ordered((float)dot[e] * by * q_scale) : 0u;
+            v = row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
+            if (absent >> of & 1) v = 0;
+            if (col == e) mine = v;
+          }
+          const int place = t + 16 * (part + i) + 4 * quad + col;
+          if (col < 4 && place < count) keep(place, mine, g0 > 0);
+        }
       }
-      const int place = 16 * t + 4 * quad + col;
-      if (col < 4 && place < count) keep(place, mine, g0 > 0);
     }
   }
 }
@@ -508,6 +522,9 @@ void update_bounds(int32_t device, void* stream, const Cache& cache, const hllm_
   HIP_CHECK(hipGetLastError());
 }
 
+// Pages that the workgroup that selects scores itself at most: 64 for each of its waves, twice.
+constexpr uint64_t kHerePages = 512;
+
 // How a selection's rows are scored: `chunks` workgroups a row and KV head before the one that selects, 0: by that one.
 struct SelectPlan {
   uint64_t limit = 0, stride = 0, bytes = 0;
@@ -520,9 +537,9 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   const uint64_t pages = (p.limit + b.page_tokens - 1) / b.page_tokens, pairs = rows * b.kv_heads;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
   if (rows == 0 || pages <= keep) return p;
-  if (pages <= kThreads * kOwn) return p;
-  p.chunks = (int)std::clamp<uint64_t>(2048 / pairs, 1, (pages + 63) / 64);
-  if (pairs * p.chunks > kMostBlocks) p.chunks = 1;
+  if (pages <= kHerePages) return p;
+  p.chunks = (int)((pages + 255) / 256);  // a wave scores 64 pages
+  if (pairs * p.chunks > kMostBlocks) p.chunks = (int)(kMostBlocks / pairs);
   p.stride = (pages + 3) / 4 * 4;
   p.bytes = pairs * p.stride * sizeof(uint32_t);
   return p;
