@@ -93,6 +93,7 @@ struct BoundsArgs {
   int32_t rows, limit;
   int32_t places;          // pages of a row at most
   int32_t wide;            // a workgroup a page and head
+  int32_t heads;           // heads that a wave takes one after the other
 };
 
 struct SelectArgs {

@@ -25,8 +25,9 @@ __device__ inline uint2v bytes8(const int* x) {
 
 // ---------------------------------------------------------------- bounds
 
+// Eight elements of a position's key as they are held.
 template <int F, int D>
-struct Keys8 {  // eight elements of a position's key as they are held
+struct Keys8 {
   uint32_t codes[F < kE2m1 ? 2 : 1];
   uint32_t scale;
   __device__ void load(const Pages& c, const uint8_t* from, uint64_t vector, int d) {
@@ -40,55 +41,87 @@ struct Keys8 {  // eight elements of a position's key as they are held
       scale = F == kE2m1 ? static_cast<const uint8_t*>(c.key_scales)[group] : static_cast<const uint16_t*>(c.key_scales)[group];
     }
   }
-  __device__ void values(float* x) const {
-    if constexpr (F < kE2m1) {
+  // The elements in F32; false where they are not numbers (infinite ones show in their maximum).
+  __device__ bool values(float* x) const {
+    if constexpr (F == kE2m1) {
+      const float by = __uint_as_float(scale << 23);
+      const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], by, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], by, 1),
+                 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], by, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], by, 3);
+      x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
+      return scale != 255;
+    } else if constexpr (F == kInt4) {
+      // (n - 8) scale of four bits n, as one rounding of what F32 holds exactly.
+      const float by = __uint_as_float(scale << 16);
+      const uint32_t even = codes[0] & 0x0f0f0f0fu, odd = codes[0] >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = fmaf((float)(even >> (8 * i) & 255u), by, -8.0f * by);
+        x[2 * i + 1] = fmaf((float)(odd >> (8 * i) & 255u), by, -8.0f * by);
+      }
+      return (scale & 0x7f80u) != 0x7f80u;
+    } else {
+      bool numbers = (scale & 0x7f800000u) != 0x7f800000u;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const floatx4 v = decode4<F>(codes[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i] * __uint_as_float(scale);
+        if constexpr (F == HLLM_KV_E4M3) numbers &= (((codes[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0;
       }
-    } else {
-      values8<F>(codes[0], x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= scale_of<F>(scale);
+      return numbers;
     }
   }
 };
 
-// A value's partner O lanes away in its half, quarter or eighth of the wave, and the value itself, in either order.
-template <int O>
-__device__ inline float2 both(float v) {
-  const uint32_t w = __float_as_uint(v);
-  if constexpr (O == 32) {
-    const auto x = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
-  } else if constexpr (O == 16) {
-    const auto x = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-    return float2{__uint_as_float(x[0]), __uint_as_float(x[1])};
-  } else {  // a row's lanes go round by O
-    return float2{v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x120 + O, 0xf, 0xf, false))};
+// Over the slots of a wave that hold other positions, eight channels each: the channels are parted among the slots in
+// step with the maximum, so that a lane ends with 8 / slots channels (from `first` on) and half the work.
+template <int L, typename Op>
+__device__ inline void reduce_slots(float* x, Op&& op) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[e]), __float_as_uint(x[e + 4]), false, false);
+    x[e] = op(__uint_as_float(both[0]), __uint_as_float(both[1]));
+  }
+  if constexpr (L <= 16) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(x[e + 2]), false, false);
+      x[e] = op(__uint_as_float(both[0]), __uint_as_float(both[1]));
+    }
+  }
+  if constexpr (L == 8) {
+    const bool upper = threadIdx.x & 8;
+    const float send = upper ? x[0] : x[1];
+    x[0] = op(upper ? x[1] : x[0],
+              __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(send), 0x128, 0xf, 0xf, false)));
   }
 }
+
 template <int O>
-__device__ inline void widen(float& high, float& low) {
-  const float2 h = both<O>(high), l = both<O>(low);
-  high = fmaxf(h.x, h.y);
-  low = fminf(l.x, l.y);
+__device__ inline uint32_t row_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + O, 0xf, 0xf, false));
+}
+__device__ inline uint32_t wave_max(uint32_t v) {
+  const auto half = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max(half[0], half[1]);
+  const auto row = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(row[0], row[1]);
+  return row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
 }
 
-// One wave takes a page and KV head (kWaves = 1), or a workgroup's four share it: a lane has eight channels of every
-// (D = 64: eighth, 128: fourth, 256: second) position.
+// One wave takes a page and some KV heads one after the other (kWaves = 1), or a workgroup's four share a page and head: a lane has
+// eight channels of every (D = 64: eighth, 128: fourth, 256: second) position. The next positions are under way while some are
+// compared.
 template <int F, int D, int kWaves>
 __global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
-  constexpr int L = D / 8, S = 64 / L, kDeep = 4;  // lanes of a vector, positions at once, and of them in flight
+  constexpr int L = D / 8, S = 64 / L, C = 8 / S, kDeep = 4;  // lanes of a vector, positions at once, channels left, loads in flight
   __shared__ float meet[kWaves > 1 ? kWaves : 1][2][kWaves > 1 ? D : 1];
   __shared__ int spoiled[kWaves];
   const Pages& c = a.pages;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int parts = (c.kv_heads + a.heads - 1) / a.heads;  // of a page's heads
   const uint64_t item = kWaves > 1 ? blockIdx.x : (uint64_t)blockIdx.x * 4 + wave;
-  const int h = (int)(item % c.kv_heads);
-  const uint64_t place = item / c.kv_heads;
+  const uint64_t place = item / parts;
   const int row = (int)(place / a.places), j = (int)(place - (uint64_t)row * a.places);
   if (row >= a.rows) return;
   const int shift = c.page_shift, length = min(uniform_load(a.lengths + row), a.limit), start = max(uniform_load(a.starts + row), 0);
@@ -98,167 +131,212 @@ __global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
   if (id < 0 || id >= c.pages) return;
   const int count = min(1 << shift, length - (p << shift));
   const int slot = lane / L, d = lane % L * 8;
-  const uint64_t page = (uint64_t)id * c.kv_heads + h;
-  const uint8_t* from = c.keys + (uint64_t)id * c.page_stride + (uint64_t)h * c.head_stride;
-  float high[8], low[8], spoil = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
-  for (int t = kWaves > 1 ? wave * S * kDeep : 0; t < count; t += kWaves * S * kDeep) {
-    Keys8<F, D> k[kDeep];
+  int h = (int)(item - place * parts) * a.heads;
+  const int last = min(h + a.heads, c.kv_heads);
+  const int first = kWaves > 1 ? wave * S * kDeep : 0;
+  int t = first;
+  Keys8<F, D> k[kDeep];
+  const auto load = [&] {
+    const uint8_t* from = c.keys + (uint64_t)id * c.page_stride + (uint64_t)h * c.head_stride;
+    const uint64_t vector = ((uint64_t)id * c.kv_heads + h) << shift;
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
       const int at = min(t + i * S + slot, count - 1);  // the last position again changes nothing
-      k[i].load(c, from + (uint64_t)(uint32_t)at * c.token_stride, (page << shift) + at, d);
+      k[i].load(c, from + (uint64_t)(uint32_t)at * c.token_stride, vector + at, d);
     }
+  };
+  float high[8], low[8];
+  bool numbers = true;
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-      float x[8];
-      k[i].values(x);
+  for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
+  load();
+  for (;;) {
+    Keys8<F, D> now[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) now[i] = k[i];
+    const int head = h;
+    t += kWaves * S * kDeep;
+    if (t >= count) ++h, t = first;
+    if (h < last) load();
+#pragma unroll
+    for (int i = 0; i < kDeep; i += 2) {
+      float x[8], y[8];
+      numbers &= now[i].values(x);
+      numbers &= now[i + 1].values(y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        high[e] = fmaxf(high[e], x[e]);
-        low[e] = fminf(low[e], x[e]);
-        spoil = fmaf(x[e], 0.0f, spoil);  // NaN once an element is not finite
+        high[e] = fmaxf(fmaxf(high[e], x[e]), y[e]);
+        low[e] = fminf(fminf(low[e], x[e]), y[e]);
       }
     }
-  }
-  bool bad = spoil != 0.0f;  // NaN is not equal
+    if (h == head) continue;
+    reduce_slots<L>(high, [](float x, float y) { return fmaxf(x, y); });
+    reduce_slots<L>(low, [](float x, float y) { return fminf(x, y); });
+    bool bad = __any(!numbers);
+    const int channel = d + (lane & 32 ? 4 : 0) + (L <= 16 && (lane & 16) ? 2 : 0) + (L == 8 && (lane & 8) ? 1 : 0);
+    if constexpr (kWaves > 1) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (L == 8) widen<8>(high[e], low[e]);
-    if constexpr (L <= 16) widen<16>(high[e], low[e]);
-    widen<32>(high[e], low[e]);
-  }
-  bad = __any(bad);
-  if constexpr (kWaves > 1) {
-    if (slot == 0) {
+      for (int e = 0; e < C; ++e) meet[wave][0][channel + e] = high[e], meet[wave][1][channel + e] = low[e];
+      if (lane == 0) spoiled[wave] = bad;
+      __syncthreads();
+      if (wave > 0) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) meet[wave][0][d + e] = high[e], meet[wave][1][d + e] = low[e];
+      for (int w = 1; w < kWaves; ++w) {
+        bad |= spoiled[w] != 0;
+#pragma unroll
+        for (int e = 0; e < C; ++e) high[e] = fmaxf(high[e], meet[w][0][channel + e]), low[e] = fminf(low[e], meet[w][1][channel + e]);
+      }
     }
-    if (lane == 0) spoiled[wave] = bad;
-    __syncthreads();
-    if (wave > 0) return;
+    uint32_t most = 0;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      bad |= spoiled[w] != 0;
+    for (int e = 0; e < C; ++e) most = max(most, max(__float_as_uint(high[e]) & 0x7fffffffu, __float_as_uint(low[e]) & 0x7fffffffu));
+    most = wave_max(most);
+    bad |= most >= 0x7f800000u;
+    const uint32_t power = whole_power(most);
+    const float inverse = __uint_as_float((254u - power) << 23);
+    const uint64_t page = (uint64_t)id * c.kv_heads + head;
+    uint32_t codes[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) high[e] = fmaxf(high[e], meet[w][0][d + e]), low[e] = fminf(low[e], meet[w][1][d + e]);
+    for (int e = 0; e < C; ++e) {
+      codes[0] |= ((uint32_t)(int)rintf(high[e] * inverse) & 255u) << (8 * e);
+      codes[1] |= ((uint32_t)(int)rintf(low[e] * inverse) & 255u) << (8 * e);
     }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      int8_t* to = a.codes + (page * 2 + which) * D + channel;
+      const uint32_t w = bad ? 0u : codes[which];
+      if constexpr (C == 1) *reinterpret_cast<uint8_t*>(to) = (uint8_t)w;
+      if constexpr (C == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
+      if constexpr (C == 4) *reinterpret_cast<uint32_t*>(to) = w;
+    }
+    if (lane == 0) a.scales[page] = bad ? NAN : __uint_as_float(power << 23);
+    if (h >= last) return;
+    numbers = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
   }
-  uint32_t most = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) most = max(most, max(__float_as_uint(high[e]) & 0x7fffffffu, __float_as_uint(low[e]) & 0x7fffffffu));
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-  const uint32_t power = whole_power(most);
-  const float inverse = __uint_as_float((254u - power) << 23);
-  int x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = bad ? 0 : (int)rintf((slot == 0 ? high[e] : low[e]) * inverse);
-  if (slot < 2) *reinterpret_cast<uint2v*>(a.codes + (page * 2 + slot) * D + d) = bytes8(x);
-  if (lane == 0) a.scales[page] = bad ? NAN : __uint_as_float(power << 23);
 }
 
 // ---------------------------------------------------------------- scores
 
-// Numbers' bits so that whole numbers order as the numbers do, -0 as 0; NaN above all of them.
+// Numbers' bits so that whole numbers order as the numbers do, -0 as 0; NaN is above all of them.
+constexpr uint32_t kNoNumber = 0xfffffffeu;
 __device__ inline uint32_t ordered(float x) {
   const uint32_t bits = __float_as_uint(x + 0.0f);
-  if (x != x) return 0xfffffffeu;
-  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+  return bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u);
 }
 
+// The largest over the sixteen lanes of a row.
 template <int O>
-__device__ inline uint32_t row_max(uint32_t v) {
-  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + O, 0xf, 0xf, false));
+__device__ inline float row_max(float v) {
+  return fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x120 + O, 0xf, 0xf, false)));
 }
 
-// The scores of a row's pages for one KV head, as ordered whole numbers: keep(page's place, number). A wave takes sixty-four pages at once,
-// from sixty-four `first` on in steps of `step`: with a query's positive and negative elements apart, the sum over channels of the larger product
-// is one product [high, low] x [max(q, 0), min(q, 0)] of twice the length, on the matrix units in bytes, with the query heads of a KV
-// head as columns. Sums of whole numbers below 2^24 and powers of two are exact.
-template <typename T, int D, typename Keep>
-__device__ inline void score_pages(const SelectArgs& a, int row, int kvh, int count, int first, int step, Keep&& keep) {
-  constexpr int KK = D / 64;
+// Sixteen queries as whole numbers, positive and negative elements apart, and their powers of two.
+template <int D>
+struct Queries {
+  uint2v up[16][D / 8], down[16][D / 8];
+  float scale[16];
+};
+
+// The scores of a row's pages for one KV head, as ordered whole numbers: keep(page's place, number, whether it is another
+// sixteen query heads' and the larger counts). Every thread of a workgroup of kWaves waves is here. A wave takes kPages pages at once, from
+// kPages `first` on in steps of `step`. With a query's positive and negative elements apart, the sum over channels of the
+// larger product is one product [high, low] x [max(q, 0), min(q, 0)] of twice the length, on the matrix units in
+// bytes, with the query heads of a KV head as columns. Sums of whole numbers below 2^24 and powers of two are exact. The first
+// bounds are under way while the workgroup rounds the queries.
+template <int D>
+constexpr int kScorePages = D == 64 ? 64 : D == 128 ? 32 : 16;
+template <typename T, int D, int kWaves, typename Keep>
+__device__ inline void score_pages(const SelectArgs& a, Queries<D>& queries, int row, int kvh, int count, int first, int step,
+                                   Keep&& keep) {
+  constexpr int KK = D / 64, kPages = kScorePages<D>, kTiles = kPages / 16;
   const int lane = threadIdx.x & 63, quad = lane >> 4, col = lane & 15;
   const int32_t* table = a.table + (uint64_t)row * a.table_stride;
+  int4v high[kTiles][KK], low[kTiles][KK];
+  float scale = 0.0f;    // of the lane's page
+  bool absent = false;   // whether it is outside the cache
+  const auto load = [&](int t) {
+    const int id = table[min(t + lane % kPages, count - 1)];
+    absent = id < 0 || id >= a.pages;
+    const int own = absent ? 0 : id;
+    scale = a.scales[(uint64_t)own * a.kv_heads + kvh];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const uint64_t page = (uint64_t)__shfl(own, 16 * i + col, 64) * a.kv_heads + kvh;
+      const int8_t* from = a.codes + page * (2 * D) + 16 * quad;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        high[i][kk] = *reinterpret_cast<const int4v*>(from + 64 * kk);
+        low[i][kk] = *reinterpret_cast<const int4v*>(from + D + 64 * kk);
+      }
+    }
+  };
   for (int g0 = 0; g0 < a.group; g0 += 16) {
     const int vectors = min(16, a.group - g0);
-    float x[KK][16];
-    const T* src = at<const T>(a.q, row, kvh * a.group + g0 + min(col, vectors - 1), 16 * quad);
-    uint32_t most = 0;
+    int t = kPages * first;
+    if (t < count) load(t);
+    if (g0 > 0) __syncthreads();
+    // D / 8 threads a query; queries behind the last repeat it.
+    constexpr int kEach = D / 8;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      load8(src + 64 * kk, x[kk]);
-      load8(src + 64 * kk + 8, x[kk] + 8);
+    for (int at = 0; at < 16 * kEach; at += 64 * kWaves) {
+      const int of = (at + (int)threadIdx.x) / kEach, u = (at + (int)threadIdx.x) % kEach;
+      if (16 * kEach < 64 * kWaves && of >= 16) break;  // whole waves
+      float x[8];
+      load8(hllm_rocm::at<const T>(a.q, row, kvh * a.group + g0 + min(of, vectors - 1), 8 * u), x);
+      uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(x[kk][i]) & 0x7fffffffu);
+      for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 1; o < kEach; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+      const bool finite = most < 0x7f800000u;
+      const uint32_t power = whole_power(most);
+      const float inverse = __uint_as_float((254u - power) << 23);
+      int p[8], n[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int v = finite ? (int)rintf(x[i] * inverse) : 0;
+        p[i] = max(v, 0);
+        n[i] = min(v, 0);
+      }
+      queries.up[of][u] = bytes8(p);
+      queries.down[of][u] = bytes8(n);
+      if (u == 0) queries.scale[of] = finite ? __uint_as_float(power << 23) : NAN;
     }
-    most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-    most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
-    const bool finite = most < 0x7f800000u;
-    const uint32_t power = whole_power(most);
-    const float inverse = __uint_as_float((254u - power) << 23), q_scale = finite ? __uint_as_float(power << 23) : NAN;
+    __syncthreads();
     int4v up[KK], down[KK];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < KK; ++kk) {
+      up[kk] = *reinterpret_cast<const int4v*>(&queries.up[col][8 * kk + 2 * quad]);
+      down[kk] = *reinterpret_cast<const int4v*>(&queries.down[col][8 * kk + 2 * quad]);
+    }
+    const float q_scale = queries.scale[col];
+    const bool no_query = __any(q_scale != q_scale);
+    for (; t < count; t += kPages * step) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int p[8], n[8];
+      for (int i = 0; i < kTiles; ++i) {
+        int4v dot = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int v = finite ? (int)rintf(x[kk][8 * i + e] * inverse) : 0;
-          p[e] = max(v, 0);
-          n[e] = min(v, 0);
+        for (int kk = 0; kk < KK; ++kk) {
+          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[i][kk], up[kk], dot, 0, 0, 0);
+          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[i][kk], down[kk], dot, 0, 0, 0);
         }
-        const uint2v pw = bytes8(p), nw = bytes8(n);
-        up[kk][2 * i] = (int)pw[0], up[kk][2 * i + 1] = (int)pw[1];
-        down[kk][2 * i] = (int)nw[0], down[kk][2 * i + 1] = (int)nw[1];
+        float mine = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = row_max<1>(row_max<2>(row_max<4>(row_max<8>((float)dot[e] * q_scale))));
+          mine = col == e ? v : mine;
+        }
+        // A lane of the first four of its row has the page 16 i + 4 quad + col; a page's scale does not change which head is the largest.
+        const int of = 16 * i + 4 * quad + (col & 3), place = t + of;
+        const float by = __shfl(scale, of, 64);
+        const bool gone = __shfl((int)absent, of, 64);
+        uint32_t key = by != by || no_query ? kNoNumber : ordered(mine * by);
+        if (gone) key = 0;
+        if (col < 4 && place < count) keep(place, key, g0 > 0);
       }
-    // 64 pages at a time, a lane's one of them, whose loads are under way together: in two halves where their bounds take many registers.
-    for (int t = 64 * first; t < count; t += 64 * step) {
-      const int id = table[min(t + lane, count - 1)];
-      const bool there = id >= 0 && id < a.pages;
-      const uint64_t absent = __ballot(!there);
-      const int own = there ? id : 0;
-      const float scale = a.scales[(uint64_t)own * a.kv_heads + kvh];
-      constexpr int kTiles = KK < 4 ? 4 : 2;
-#pragma unroll
-      for (int part = 0; part < 4; part += kTiles) {
-        int4v high[kTiles][KK], low[kTiles][KK];
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          const uint64_t page = (uint64_t)__shfl(own, 16 * (part + i) + col, 64) * a.kv_heads + kvh;
-          const int8_t* from = a.codes + page * (2 * D) + 16 * quad;
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            high[i][kk] = *reinterpret_cast<const int4v*>(from + 64 * kk);
-            low[i][kk] = *reinterpret_cast<const int4v*>(from + D + 64 * kk);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          int4v dot = {0, 0, 0, 0};
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[i][kk], up[kk], dot, 0, 0, 0);
-            dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[i][kk], down[kk], dot, 0, 0, 0);
-          }
-          uint32_t mine = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int of = 16 * (part + i) + 4 * quad + e;
-            const float by = __shfl(scale, of, 64);
-            uint32_t v = col < vectors ? ordered((float)dot[e] * by * q_scale) : 0u;
-            v = row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
-            if (absent >> of & 1) v = 0;
-            if (col == e) mine = v;
-          }
-          const int place = t + 16 * (part + i) + 4 * quad + col;
-          if (col < 4 && place < count) keep(place, mine, g0 > 0);
-        }
-      }
+      if (t + kPages * step < count) load(t + kPages * step);
     }
   }
 }
@@ -270,30 +348,44 @@ __device__ inline int pages_of(const SelectArgs& a, int row, int& length) {
 
 // Scores into the workspace, for rows of more pages than one workgroup scores.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv_score_kernel(SelectArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) kv_score_kernel(SelectArgs a) {
   const int row = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
   int length;
   const int count = pages_of(a, row, length);
   if (count <= a.keep) return;
+  __shared__ Queries<D> queries;
   uint32_t* keys = a.keys + (uint64_t)blockIdx.x * a.stride;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  score_pages<T, D>(a, row, kvh, count, blockIdx.y * 4 + wave, gridDim.y * 4,
+  // Workgroups without a page: every other takes the queries' barriers.
+  if ((int)blockIdx.y * 4 * kScorePages<D> >= count) return;
+  score_pages<T, D, 4>(a, queries, row, kvh, count, blockIdx.y * 4 + wave, gridDim.y * 4,
                     [&](int place, uint32_t key, bool again) { keys[place] = again ? max(keys[place], key) : key; });
 }
 
 // ---------------------------------------------------------------- selection
 
-constexpr int kOwn = 16;  // scores that a thread holds
+// How a selection is made: by workgroups of four or of sixteen waves that score their pages themselves, or by ones of sixteen
+// waves whose pages others have scored. Threads, and scores that each holds at once.
+enum Select { kSmall, kLarge, kScored };
+template <Select kHow>
+constexpr int kSelectThreads = kHow == kSmall ? 256 : 1024;
+template <Select kHow>
+constexpr int kSelectOwn = kHow == kSmall ? 2 : kHow == kLarge ? 4 : 16;
+constexpr int kDigit = 11;  // bits that a pass over the scores settles
 
-// A workgroup selects a row's pages for one KV head: it finds, from the upper bit down, the largest number that `keep` scores
-// reach, then writes the pages above it, and of those at it the first ones, in their order. kHere: it has scored
-// them itself (at most kThreads * kOwn).
-template <typename T, int D, bool kHere>
-__global__ void __launch_bounds__(kThreads) kv_select_kernel(SelectArgs a) {
-  __shared__ uint32_t scored[kHere ? kThreads * kOwn : 1];
-  __shared__ uint32_t range[4][2];
-  __shared__ int counts[2][4];
-  __shared__ int before[kOwn][4][2];
+// A workgroup selects a row's pages for one KV head. Passes over the scores, upper bits first, count how many there are of each value of
+// the next bits among those that may still be the last one selected; then the pages above it are written, and of those at
+// it the first ones, in their order.
+template <typename T, int D, Select kHow>
+__global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectArgs a) {
+  constexpr bool kHere = kHow != kScored;
+  constexpr int kThreadsHere = kSelectThreads<kHow>, W = kThreadsHere / 64, kOwn = kSelectOwn<kHow>;
+  constexpr int kTile = kThreadsHere * kOwn, kBins = 1 << kDigit, kEach = kBins / kThreadsHere;
+  __shared__ uint32_t scored[kHere ? kTile : 1];
+  __shared__ int bins[kBins];
+  __shared__ uint32_t range[W][2];
+  __shared__ int sums[W], found[3];
+  __shared__ int before[kOwn * W];
   const int row = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int length;
@@ -304,38 +396,41 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(SelectArgs a) {
   const int32_t* table = a.table + (uint64_t)row * a.table_stride;
   int32_t* out = a.selected + (uint64_t)blockIdx.x * a.keep;
   if (n <= a.keep) {
-    for (int i = threadIdx.x; i < a.keep; i += kThreads) out[i] = i < n ? table[i] : -1;
+    for (int i = threadIdx.x; i < a.keep; i += kThreadsHere) out[i] = i < n ? table[i] : -1;
     return;
   }
   const uint32_t* keys = a.keys + (uint64_t)blockIdx.x * a.stride;
   if constexpr (kHere) {
-    score_pages<T, D>(a, row, kvh, n, wave, 4,
-                      [&](int place, uint32_t key, bool again) { scored[place] = again ? max(scored[place], key) : key; });
+    __shared__ Queries<D> queries;
+    score_pages<T, D, W>(a, queries, row, kvh, n, wave, W,
+                         [&](int place, uint32_t key, bool again) { scored[place] = again ? max(scored[place], key) : key; });
     __syncthreads();
   }
-  const int tiles = kHere ? 1 : (n + kThreads * kOwn - 1) / (kThreads * kOwn);
-  uint32_t v[kOwn];
-  int used = 0;  // of v, the same for all threads
+  // A thread's scores of a tile: of places from + j * kThreadsHere. `open` has a bit for each that is selected by its score.
+  const int tiles = (n + kTile - 1) / kTile;
+  uint32_t v[kOwn], open = 0;
+  int ids[kOwn], used = 0;
   const auto load = [&](int tile) {
-    const int from = tile * kThreads * kOwn;
-    used = min(kOwn, (n - from + kThreads - 1) / kThreads);
+    const int from = tile * kTile + (int)threadIdx.x;
+    used = min(kOwn, (n - tile * kTile + kThreadsHere - 1) / kThreadsHere);
+    open = 0;
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
-      const int i = from + j * kThreads + (int)threadIdx.x;
+      const int i = from + j * kThreadsHere;
       v[j] = 0;
-      if (i < n) v[j] = i < a.first || i >= n - a.last ? 0xffffffffu : kHere ? scored[i] : keys[i];
+      if (j < used && i < n) {
+        if (i >= a.first && i < n - a.last) open |= 1u << j;
+        v[j] = kHere ? scored[i] : keys[i];
+        ids[j] = table[i];
+      }
     }
   };
-  load(0);
-  // Bits that all scores share are the threshold's. Places behind the last page are left out; forced ones have every bit.
   uint32_t all = 0xffffffffu, some = 0;
   for (int tile = 0; tile < tiles; ++tile) {
-    if (tile > 0) load(tile);
+    load(tile);
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-      const int i = tile * kThreads * kOwn + j * kThreads + (int)threadIdx.x;
-      if (i < n && i >= a.first && i < n - a.last) all &= v[j], some |= v[j];
-    }
+    for (int j = 0; j < kOwn; ++j)
+      if (open >> j & 1) all &= v[j], some |= v[j];
   }
   for (int o = 1; o < 64; o <<= 1) {
     all &= (uint32_t)__shfl_xor((int)all, o, 64);
@@ -343,81 +438,93 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(SelectArgs a) {
   }
   if (lane == 0) range[wave][0] = all, range[wave][1] = some;
   __syncthreads();
-  all = range[0][0] & range[1][0] & range[2][0] & range[3][0];
-  some = range[0][1] | range[1][1] | range[2][1] | range[3][1];
-  // keep > first + last: some score is selected by its number, and the threshold is one of theirs.
-  const int forced = a.first + a.last;
-  uint32_t threshold = 0xffffffffu;
-  int above = forced;   // scores that are larger than the threshold
-  bool whole = a.keep == forced;   // the threshold's own scores are all selected
-  if (!whole) {
-    const int bits = all == some ? 0 : 32 - __builtin_clz(all ^ some);
-    threshold = bits == 32 ? 0 : all >> bits << bits;
-    for (int b = bits - 1; b >= 0 && !whole; --b) {
-      const uint32_t next = threshold | 1u << b;
-      int reach = 0;
-      for (int tile = 0; tile < tiles; ++tile) {
-        if (tiles > 1) load(tile);
+  for (int w = 0; w < W; ++w) all &= range[w][0], some |= range[w][1];
+  // The scores that are open are those whose upper bits, from `bits` on, are `prefix`; `need` of them are to be selected.
+  int bits = all == some ? 0 : 32 - __builtin_clz(all ^ some), need = a.keep - a.first - a.last;
+  uint64_t prefix = (uint64_t)all >> bits;
+  bool whole = need == 0;  // all that are left are selected, or (none needed) none
+  if (whole) prefix = ~0ull;
+  while (bits > 0 && !whole) {
+    const int shift = max(bits - kDigit, 0), mask = (1 << (bits - shift)) - 1;
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j)
-          if (j < used) reach += __popcll(__ballot(v[j] >= next));
-      }
-      if (lane == 0) counts[b & 1][wave] = reach;
-      __syncthreads();
-      reach = counts[b & 1][0] + counts[b & 1][1] + counts[b & 1][2] + counts[b & 1][3];
-      if (reach >= a.keep) threshold = next;
-      whole = reach == a.keep;
-    }
-  }
-  // Places in order: first by v's index, then by wave and lane.
-  int larger = 0, equal = 0;  // of the tiles before, and of this tile's places before the thread's
-  const uint64_t below = (1ull << lane) - 1;
-  if (!whole) {
-    above = 0;
+    for (int i = 0; i < kEach; ++i) bins[i * kThreadsHere + threadIdx.x] = 0;
+    __syncthreads();
     for (int tile = 0; tile < tiles; ++tile) {
       if (tiles > 1) load(tile);
 #pragma unroll
       for (int j = 0; j < kOwn; ++j)
-        if (j < used) above += __popcll(__ballot(v[j] > threshold));
+        if ((open >> j & 1) && (uint64_t)v[j] >> bits == prefix) atomicAdd(&bins[v[j] >> shift & mask], 1);
     }
     __syncthreads();
-    if (lane == 0) counts[0][wave] = above;
+    // Bins from the largest down: a thread's kEach, and how many scores the threads before it have.
+    const int top = kBins - 1 - (int)threadIdx.x * kEach;
+    int own = 0, sum;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) own += bins[top - i];
+    sum = wave_scan(own, lane, 64);
+    if (lane == 63) sums[wave] = sum;
     __syncthreads();
-    above = counts[0][0] + counts[0][1] + counts[0][2] + counts[0][3];
+    for (int w = 0; w < wave; ++w) sum += sums[w];
+    if (sum >= need && sum - own < need) {
+      int above = sum - own, i = 0;
+      while (above + bins[top - i] < need) above += bins[top - i++];
+      found[0] = top - i, found[1] = need - above, found[2] = bins[top - i];
+    }
+    __syncthreads();
+    prefix = prefix << (bits - shift) | (uint32_t)found[0];
+    need = found[1];
+    whole = need == found[2];
+    bits = shift;
   }
-  const int take = whole ? 0x7fffffff : a.keep - above;  // of the threshold's own scores
+  const int take = whole ? 0x7fffffff : need;  // of those at the prefix
+  int larger = 0, equal = 0;  // of the tiles before
   for (int tile = 0; tile < tiles; ++tile) {
     if (tiles > 1) load(tile);
-    if (tile > 0) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-      if (j >= used) continue;
-      const int i = tile * kThreads * kOwn + j * kThreads + (int)threadIdx.x;
-      const int g = __popcll(__ballot(i < n && v[j] > threshold)), e = __popcll(__ballot(i < n && v[j] == threshold));
-      if (lane == 0) before[j][wave][0] = g, before[j][wave][1] = e;
-    }
+    uint32_t gt = 0, eq = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
-      if (j >= used) continue;
-      const int i = tile * kThreads * kOwn + j * kThreads + (int)threadIdx.x;
-      const bool gt = i < n && v[j] > threshold, eq = i < n && v[j] == threshold;
-      int g = larger, e = equal;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (w < wave) g += before[j][w][0], e += before[j][w][1];
-        larger += before[j][w][0], equal += before[j][w][1];
+      if (j < used) {
+        const int i = tile * kTile + j * kThreadsHere + (int)threadIdx.x;
+        const uint64_t upper = (uint64_t)v[j] >> bits;
+        const bool is_open = open >> j & 1, g = i < n && (!is_open || upper > prefix), e = is_open && upper == prefix;
+        gt |= (uint32_t)g << j;
+        eq |= (uint32_t)e << j;
+        const int counts = __popcll(__ballot(g)) | __popcll(__ballot(e)) << 16;
+        if (lane == 0) before[j * W + wave] = counts;
       }
-      g += __popcll(__ballot(gt) & below);
-      e += __popcll(__ballot(eq) & below);
-      if (gt || (eq && e < take)) out[g + min(e, take)] = table[i];
     }
+    __syncthreads();
+    // How many lie before each wave's places: an exclusive sum over the places in their order.
+    int total = 0;
+    if (wave == 0) {
+      for (int at = 0; at < used * W; at += 64) {
+        const int own = at + lane < used * W ? before[at + lane] : 0;
+        const int sum = wave_scan(own, lane, 64) + total;
+        if (at + lane < used * W) before[at + lane] = sum - own;
+        total = __builtin_amdgcn_readlane(sum, 63);
+      }
+      if (lane == 0) found[0] = total;
+    }
+    __syncthreads();
+    const uint64_t lower = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      if (j < used) {
+        const int at = before[j * W + wave];
+        const int g = larger + (at & 0xffff) + __popcll(__ballot(gt >> j & 1) & lower);
+        const int e = equal + (at >> 16) + __popcll(__ballot(eq >> j & 1) & lower);
+        if ((gt >> j & 1) || ((eq >> j & 1) && e < take)) out[g + min(e, take)] = ids[j];
+      }
+    }
+    larger += found[0] & 0xffff;
+    equal += found[0] >> 16;
   }
 }
 
 template <int F>
 void bounds_format(hipStream_t stream, int head_dim, const BoundsArgs& a) {
-  const uint64_t items = (uint64_t)a.rows * a.places * a.pages.kv_heads;
+  const uint64_t items = (uint64_t)a.rows * a.places * ((a.pages.kv_heads + a.heads - 1) / a.heads);
   const auto run = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
     if (a.wide)
@@ -438,22 +545,22 @@ void launch_bounds(hipStream_t stream, int format, int head_dim, const BoundsArg
 }
 
 template <typename T, int D>
-void select_dim(hipStream_t stream, int chunks, const SelectArgs& a) {
+void select_dim(hipStream_t stream, Select how, int chunks, const SelectArgs& a) {
   const unsigned pairs = (unsigned)(a.rows * a.kv_heads);
-  if (chunks == 0) {
-    kv_select_kernel<T, D, true><<<pairs, kThreads, 0, stream>>>(a);
-  } else {
+  if (how == kSmall) kv_select_kernel<T, D, kSmall><<<pairs, kSelectThreads<kSmall>, 0, stream>>>(a);
+  if (how == kLarge) kv_select_kernel<T, D, kLarge><<<pairs, kSelectThreads<kLarge>, 0, stream>>>(a);
+  if (how == kScored) {
     kv_score_kernel<T, D><<<dim3(pairs, chunks), kThreads, 0, stream>>>(a);
-    kv_select_kernel<T, D, false><<<pairs, kThreads, 0, stream>>>(a);
+    kv_select_kernel<T, D, kScored><<<pairs, kSelectThreads<kScored>, 0, stream>>>(a);
   }
 }
 
-void launch_select(hipStream_t stream, uint32_t dtype, int head_dim, int chunks, const SelectArgs& a) {
+void launch_select(hipStream_t stream, uint32_t dtype, int head_dim, Select how, int chunks, const SelectArgs& a) {
   const auto run = [&](auto zero) {
     using T = decltype(zero);
-    if (head_dim == 64) select_dim<T, 64>(stream, chunks, a);
-    if (head_dim == 128) select_dim<T, 128>(stream, chunks, a);
-    if (head_dim == 256) select_dim<T, 256>(stream, chunks, a);
+    if (head_dim == 64) select_dim<T, 64>(stream, how, chunks, a);
+    if (head_dim == 128) select_dim<T, 128>(stream, how, chunks, a);
+    if (head_dim == 256) select_dim<T, 256>(stream, how, chunks, a);
   };
   if (dtype == HLLM_DTYPE_F16) return run(_Float16{});
   if (dtype == HLLM_DTYPE_BF16) return run(bhalf{});
@@ -517,19 +624,21 @@ void update_bounds(int32_t device, void* stream, const Cache& cache, const hllm_
   const uint64_t items = args->rows * places * pages.kv_heads;
   if (args->rows * places > kMostBlocks || items > kMostBlocks) refuse("too many rows for these pages and heads");
   a.wide = cache.page_tokens > 128;
+  // Many pages: a wave takes some heads, which have the page's number and the loads under way in common.
+  a.heads = a.wide || items < 16384 ? 1 : items < 32768 ? 2 : 4;
   OnDevice on(device);
   launch_bounds(static_cast<hipStream_t>(stream), cache.format, cache.head_dim, a);
   HIP_CHECK(hipGetLastError());
 }
 
-// Pages that the workgroup that selects scores itself at most: 64 for each of its waves, twice.
-constexpr uint64_t kHerePages = 512;
-
-// How a selection's rows are scored: `chunks` workgroups a row and KV head before the one that selects, 0: by that one.
+// How a call's rows are scored and selected, and by how many workgroups a row and KV head they are scored (kScored).
 struct SelectPlan {
   uint64_t limit = 0, stride = 0, bytes = 0;
+  Select how = kSmall;
   int chunks = 0;
 };
+
+uint64_t score_pages_of(uint32_t head_dim) { return head_dim == 256 ? kScorePages<256> : head_dim == 128 ? kScorePages<128> : kScorePages<64>; }
 
 SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max_length, uint64_t keep) {
   SelectPlan p;
@@ -537,8 +646,17 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   const uint64_t pages = (p.limit + b.page_tokens - 1) / b.page_tokens, pairs = rows * b.kv_heads;
   if (pairs > kMostBlocks) refuse("too many rows for these heads");
   if (rows == 0 || pages <= keep) return p;
-  if (pages <= kHerePages) return p;
-  p.chunks = (int)((pages + 255) / 256);  // a wave scores 64 pages
+  if (pages <= (uint64_t)kSelectThreads<kSmall> * kSelectOwn<kSmall>) return p;
+  // With few pages, or workgroups for half the card, one launch takes less time than two. Us with workgroups that score
+  // their own pages / with others that do, 8 KV heads of 128 and all rows of as many pages of 16:
+  //   1 row: 600 pages 15.6 / 16.2, 1000 19.9 / 16.9; 4 rows: 600 15.7 / 16.3, 1000 21.1 / 18.0;
+  //   16 rows: 600 17.4 / 20.7, 2000 29.4 / 31.5, 3000 47.6 / 40.8; 32 rows: 600 19.3 / 26.0, 2000 43.9 / 51.3; 64 rows: 1000 48.2 / 59.5
+  if (pages <= 640 || (pairs >= 128 && pages <= 2304)) {
+    p.how = kLarge;
+    return p;
+  }
+  p.how = kScored;
+  p.chunks = (int)((pages + 4 * score_pages_of(b.head_dimension) - 1) / (4 * score_pages_of(b.head_dimension)));
   if (pairs * p.chunks > kMostBlocks) p.chunks = (int)(kMostBlocks / pairs);
   p.stride = (pages + 3) / 4 * 4;
   p.bytes = pairs * p.stride * sizeof(uint32_t);
@@ -594,7 +712,7 @@ void select(int32_t device, void* stream, const hllm_rocm_kv_bounds* bounds, con
   a.first = (int32_t)args->first;
   a.last = (int32_t)args->last;
   OnDevice on(device);
-  launch_select(static_cast<hipStream_t>(stream), args->q.dtype, (int)bounds->head_dimension, plan.chunks, a);
+  launch_select(static_cast<hipStream_t>(stream), args->q.dtype, (int)bounds->head_dimension, plan.how, plan.chunks, a);
   HIP_CHECK(hipGetLastError());
 }
 
