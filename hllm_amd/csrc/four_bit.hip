@@ -32,7 +32,7 @@ __device__ inline float held_scale(const uint32_t* raw, int g) {
 // ---------------------------------------------------------------- reading back
 
 // A thread reads the codes of sixteen bytes of output of a key, and of the value beside it, and writes them. A value's
-// codes lie G bytes apart (two elements of each group beside each other), in a line that the wave reads whole.
+// codes lie G bytes apart (two elements of each group beside each other).
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
   constexpr int kCodes = 16 / sizeof(T), L = D / kCodes, G = D / 32;
@@ -48,12 +48,21 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
   const uint64_t from = (uint64_t)page * c.page_stride + (uint64_t)offset * c.token_stride + (uint64_t)h * c.head_stride;
   const uint64_t scale_at = ((((uint64_t)page * c.kv_heads + h) << c.page_shift) + offset) * G + g;
   uint32_t codes[2] = {0, 0};
-  if constexpr (kCodes == 8)
+  if constexpr (kCodes == 8) {
     codes[0] = *reinterpret_cast<const uint32_t*>(c.keys + from + d / 2);
-  else
+    // A vector's lanes read a word each and take the bytes of their eight elements from one another.
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(c.values + from + d / 2);
+    const int lane = threadIdx.x & 63, base = lane & ~(L - 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = G * (d % 32 / 2 + i) + g;
+      codes[1] |= ((uint32_t)__shfl((int)word, base + at / 4, 64) >> (8 * (at % 4)) & 255u) << (8 * i);
+    }
+  } else {
     codes[0] = *reinterpret_cast<const uint16_t*>(c.keys + from + d / 2);
 #pragma unroll
-  for (int i = 0; i < kCodes / 2; ++i) codes[1] |= (uint32_t)c.values[from + G * (d % 32 / 2 + i) + g] << (8 * i);
+    for (int i = 0; i < 2; ++i) codes[1] |= (uint32_t)c.values[from + G * (d % 32 / 2 + i) + g] << (8 * i);
+  }
   float scale[2];
   if constexpr (F == kE2m1) {
     scale[0] = scale_of<F>(static_cast<const uint8_t*>(c.key_scales)[scale_at]);

@@ -107,8 +107,15 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
 // share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
 // heads of 256: 12.7 us, 4.3 TB/s; 64 rows 4.1 us, one chain of loads, sines, the largest value and the stores.
 // The last part for a 4-bit cache, of every thread of the workgroup. A group's 32 elements lie with two to four lanes, which depends
-// on the rotation's layout, so they meet in LDS: each eight's largest magnitude, then the
-// codes, which are written from there in whole words.
+// on the rotation's layout, so they meet in LDS: each eight's largest magnitude, then the codes, which are written from
+// there in whole words. A head's lanes (4, 8 or 16) lie in one wave, so no barrier is needed.
+// Lanes of one wave see what its lanes have written to LDS: its accesses are made in order.
+__device__ inline void wave_meets() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int F>
 __device__ inline void append_four(const RotateArgs& a, const float* x, int slot, bool cached, bool is_v, int in_block, int u,
                                    int h, int d0, int d1) {
@@ -127,7 +134,7 @@ __device__ inline void append_four(const RotateArgs& a, const float* x, int slot
       most_of[(k ? d1 : d0) / 8] = most;
     }
   }
-  __syncthreads();
+  wave_meets();
   const int page = slot >> c.page_shift, offset = slot & ((1 << c.page_shift) - 1);
   if (cached) {
 #pragma unroll
@@ -154,7 +161,7 @@ __device__ inline void append_four(const RotateArgs& a, const float* x, int slot
       }
     }
   }
-  __syncthreads();
+  wave_meets();
   if (!cached) return;
   uint8_t* to = (is_v ? c.values : c.keys) + (uint64_t)page * c.page_stride + (uint64_t)offset * c.token_stride +
                 (uint64_t)h * c.head_stride + 8 * u;

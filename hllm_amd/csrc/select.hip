@@ -623,7 +623,10 @@ void update_bounds(int32_t device, void* stream, const Cache& cache, const hllm_
   a.places = (int32_t)places;
   const uint64_t items = args->rows * places * pages.kv_heads;
   if (args->rows * places > kMostBlocks || items > kMostBlocks) refuse("too many rows for these pages and heads");
-  a.wide = cache.page_tokens > 128;
+  // Long pages, and pages that a lone wave reads in many steps where there are few of them (9 rows of 4 heads of 256 in pages of 64:
+  // 5.5 us with a wave a page and head).
+  const uint64_t loads = (uint64_t)cache.page_tokens * (cache.head_dim / 8) / 64;  // of a wave for a page and head
+  a.wide = cache.page_tokens > 128 || (items <= 1024 && loads > 4);
   // Many pages: a wave takes some heads, which have the page's number and the loads under way in common.
   a.heads = a.wide || items < 16384 ? 1 : items < 32768 ? 2 : 4;
   OnDevice on(device);
