@@ -256,8 +256,9 @@ __device__ inline void score_pages(const SelectArgs& a, Queries<D>& queries, int
   int4v high[kTiles][KK], low[kTiles][KK];
   float scale = 0.0f;    // of the lane's page
   bool absent = false;   // whether it is outside the cache
+  int id = 0;            // the page of the next load
+  const auto find = [&](int t) { id = table[min(t + lane % kPages, count - 1)]; };
   const auto load = [&](int t) {
-    const int id = table[min(t + lane % kPages, count - 1)];
     absent = id < 0 || id >= a.pages;
     const int own = absent ? 0 : id;
     scale = a.scales[(uint64_t)own * a.kv_heads + kvh];
@@ -271,11 +272,12 @@ __device__ inline void score_pages(const SelectArgs& a, Queries<D>& queries, int
         low[i][kk] = *reinterpret_cast<const int4v*>(from + D + 64 * kk);
       }
     }
+    if (t + kPages * step < count) find(t + kPages * step);
   };
   for (int g0 = 0; g0 < a.group; g0 += 16) {
     const int vectors = min(16, a.group - g0);
     int t = kPages * first;
-    if (t < count) load(t);
+    if (t < count) find(t), load(t);
     if (g0 > 0) __syncthreads();
     // D / 8 threads a query; queries behind the last repeat it.
     constexpr int kEach = D / 8;
@@ -438,7 +440,11 @@ __global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectA
   }
   if (lane == 0) range[wave][0] = all, range[wave][1] = some;
   __syncthreads();
-  for (int w = 0; w < W; ++w) all &= range[w][0], some |= range[w][1];
+  all = range[lane % W][0], some = range[lane % W][1];
+  for (int o = 1; o < W; o <<= 1) {
+    all &= (uint32_t)__shfl_xor((int)all, o, 64);
+    some |= (uint32_t)__shfl_xor((int)some, o, 64);
+  }
   // The scores that are open are those whose upper bits, from `bits` on, are `prefix`; `need` of them are to be selected.
   int bits = all == some ? 0 : 32 - __builtin_clz(all ^ some), need = a.keep - a.first - a.last;
   uint64_t prefix = (uint64_t)all >> bits;
@@ -464,7 +470,9 @@ __global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectA
     sum = wave_scan(own, lane, 64);
     if (lane == 63) sums[wave] = sum;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) sum += sums[w];
+    int earlier = lane < wave ? sums[lane] : 0;
+    for (int o = 1; o < W; o <<= 1) earlier += __shfl_xor(earlier, o, 64);
+    sum += __builtin_amdgcn_readfirstlane(earlier);
     if (sum >= need && sum - own < need) {
       int above = sum - own, i = 0;
       while (above + bins[top - i] < need) above += bins[top - i++];

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+from typing import Callable, NamedTuple
 
 import torch
 
@@ -81,8 +82,18 @@ class Rope:
         capi.check(capi.library().hllm_rocm_rope_plan(C.byref(c), self.address))
 
 
+class _Calls(NamedTuple):
+    """The library's functions for a kind of cache."""
+    append: Callable
+    read: Callable
+    attention: Callable
+    bounds: Callable
+
+
 class _Pages:
     """What both kinds of cache have in common: tensors that are held, and their description for the library."""
+
+    names: tuple[str, ...]
 
     def _describe(self, keys, values, key_scales, value_scales, kind, format, head_dim):
         for x in (values, key_scales, value_scales):
@@ -93,6 +104,7 @@ class _Pages:
         self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
         self.device, self.kv_heads, self.head_dim = keys.device, keys.shape[1], head_dim
         self.pages, self.page_tokens = keys.shape[0], keys.shape[2]
+        self.calls = _Calls(*(getattr(capi.library(), "hllm_rocm_" + name) for name in self.names))
         size = keys.element_size()
         self.c = kind(format, self.pages, self.page_tokens, self.kv_heads, head_dim, keys.stride(0) * size,
                       keys.stride(2) * size, keys.stride(1) * size, keys.data_ptr(), values.data_ptr(),
@@ -107,6 +119,8 @@ class KvPages(_Pages):
     with a contiguous last dimension, so a permuted [pages, page_tokens, kv_heads, head_dim] too)
     and F32 scales [pages, kv_heads, page_tokens]. Position p of a page is slot page * page_tokens
     + p. The tensors are held, and must not be resized."""
+
+    names = "kv_append", "kv_read", "kv_attention_by_head", "kv_bounds_update"
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor,
                  value_scales: torch.Tensor):
@@ -144,6 +158,8 @@ class Kv4Pages(_Pages):
     page_tokens, head_dim / 32], one for 32 elements: torch.uint8 for E2M1 codes (a power of two's exponent + 127) or
     torch.bfloat16 for INT4 codes. include/hllm_rocm.h states the formats and the order of the codes. The
     tensors are held, and must not be resized."""
+
+    names = "kv4_append", "kv4_read", "kv4_attention", "kv4_bounds_update"
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor,
                  value_scales: torch.Tensor):
@@ -199,11 +215,6 @@ class KvBounds:
         """Bounds for this cache, with nothing made yet."""
         return cls(pages, torch.zeros(pages.pages, pages.kv_heads, 2, pages.head_dim, dtype=torch.int8, device=pages.device),
                    torch.zeros(pages.pages, pages.kv_heads, dtype=torch.float32, device=pages.device))
-
-
-def _entry(pages: KvPages | Kv4Pages, name: str, name4: str):
-    """The library's function for this kind of cache."""
-    return getattr(capi.library(), "hllm_rocm_" + (name4 if isinstance(pages, Kv4Pages) else name))
 
 
 def _on_device(x: torch.Tensor, name: str) -> None:
@@ -314,7 +325,7 @@ def kv_append(pages: KvPages | Kv4Pages, slots: torch.Tensor, k: torch.Tensor, v
         q_from, q_to = TENSOR.pack(*c), TENSOR.pack(*d)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    capi.check(_entry(pages, "kv_append", "kv4_append")(device.index, _stream(device), pages.address, to, rows, a, b, plan, at,
+    capi.check(pages.calls.append(device.index, _stream(device), pages.address, to, rows, a, b, plan, at,
                                                        q_from, q_to))
     return q_out
 
@@ -334,7 +345,7 @@ def kv_read(pages: KvPages | Kv4Pages, slots: torch.Tensor, dtype: torch.dtype =
     if k_out is None:
         k_out, v_out = pages.key_scales.new_empty((2, rows, heads, dim), dtype=dtype)
     a, b = _rows(k_out, "k_out", device, rows, dim, heads), _rows(v_out, "v_out", device, rows, dim, heads)
-    capi.check(_entry(pages, "kv_read", "kv4_read")(device.index, _stream(device), pages.address, at, rows, a, b))
+    capi.check(pages.calls.read(device.index, _stream(device), pages.address, at, rows, a, b))
     return k_out, v_out
 
 
@@ -370,7 +381,7 @@ def kv_attention(q: torch.Tensor, pages: KvPages | Kv4Pages, page_table: torch.T
     at, size = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     args = ATTENTION_ARGS.pack(rows, table, width, stride, n, max_length,
                                pages.head_dim ** -0.5 if scale is None else scale, *a, *b, at, size)
-    capi.check(_entry(pages, "kv_attention_by_head", "kv4_attention")(device.index, _stream(device), pages.address, args, head_stride))
+    capi.check(pages.calls.attention(device.index, _stream(device), pages.address, args, head_stride))
     return out
 
 
@@ -383,7 +394,9 @@ def kv_attention_workspace(pages: KvPages | Kv4Pages, rows: int, q_heads: int, m
 
 def _workspace_bytes(pages: KvPages | Kv4Pages, rows: int, q_heads: int, max_length: int) -> int:
     need = C.c_uint64()
-    capi.check(_entry(pages, "kv_attention_workspace", "kv4_attention_workspace")(pages.address, rows, q_heads, max_length, C.byref(need)))
+    lib = capi.library()
+    call = lib.hllm_rocm_kv4_attention_workspace if isinstance(pages, Kv4Pages) else lib.hllm_rocm_kv_attention_workspace
+    capi.check(call(pages.address, rows, q_heads, max_length, C.byref(need)))
     return need.value
 
 
@@ -403,7 +416,7 @@ def kv_bounds(pages: KvPages | Kv4Pages, bounds: KvBounds, page_table: torch.Ten
     if max_new < 0:
         raise ValueError("max_new is negative")
     args = BOUNDS_ARGS.pack(rows, table, width, stride, begin, n, min(max_new, width * pages.page_tokens))
-    capi.check(_entry(pages, "kv_bounds_update", "kv4_bounds_update")(device.index, _stream(device), pages.address, bounds.address, args))
+    capi.check(pages.calls.bounds(device.index, _stream(device), pages.address, bounds.address, args))
 
 
 def kv_select(q: torch.Tensor, bounds: KvBounds, page_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int,
