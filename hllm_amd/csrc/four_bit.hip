@@ -342,9 +342,14 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
             int top = power;
             for (int step = 1; step < 64; step <<= 1) top = max(top, __shfl_xor(top, step, 64));
             top = __builtin_amdgcn_readfirstlane(top);
-            const float rescale = __builtin_amdgcn_ldexpf(1.0f, max(unit - top, -300));
+            // A column's reference comes down by as much as its sum of weights allows: to the new unit, what the wave has
+            // is small, and weights that were nothing beside it are not.
+            const int room = min(top - unit, max(226 - (int)(__float_as_uint(column_max(l)) >> 23), 0));
+            const float rescale = __builtin_amdgcn_ldexpf(1.0f, max(unit + room - top, -300));
 #pragma unroll
             for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
+            l = __builtin_amdgcn_ldexpf(l, room);
+            m -= (float)room;
             unit = top;
           }
           if (mine) {
@@ -466,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       }
       if constexpr (kRatios) {
         // Weights are 2^(score - m) for an m that is seldom changed: where a wave's first scores are found, and where a weight times its
-        // value scales (in `unit`s) is above 2^12, or a weight above 2^100. So most tiles need no
-        // maximum, and F16 holds every weight to 2^-11 or to 2^-25 of the largest.
+        // value scales (in `unit`s) is above 2^14, or a weight above 2^100; the largest is then made 2^6. So most
+        // tiles need no maximum, and F16 holds every weight to 2^-11 or to 2^-31 of the largest.
         float sum, largest;
         const auto weigh = [&] {
           const float base = m == -INFINITY ? 0.0f : m;
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           }
         };
         weigh();
-        const bool raise = largest > 4096.0f || sum > 0x1p100f || m == -INFINITY;
+        const bool raise = largest > 16384.0f || sum > 0x1p100f || m == -INFINITY;
         if (__any(raise)) {
           float top = -INFINITY, high = -INFINITY;
 #pragma unroll
@@ -498,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           }
           // Of the columns that need it: a head's sums do not depend on the heads beside it.
           const bool own_raise = column_max(raise ? 1.0f : 0.0f) > 0.0f;
-          const float raised = own_raise ? fmaxf(m, fmaxf(column_max(high), column_max(top) - 100.0f)) : m;
+          const float raised = own_raise ? fmaxf(m, fmaxf(column_max(high) - 6.0f, column_max(top) - 100.0f)) : m;
           const float rescale = raised == m ? 1.0f : exp2_fast(m - raised);
 #pragma unroll
           for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;

@@ -1108,7 +1108,9 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   if (rows == 0) return p;
   const uint64_t group = query_heads / kv_heads;
   p.head_groups = (group + 15) / 16;
-  // Pairs beside each other that read the same cache lines: sixteens of a KV head's query heads, and heads within 128 bytes.
+  // Pairs beside each other that read the same cache lines: sixteens of a KV head's query heads, and heads within 128 bytes. In
+  // one die's cache at once, their lines are read once: 24 rows of 12000 to 30000 positions, 8 KV heads beside each other,
+  // 166 us to 120 (128), 149 to 85 (64).
   if (four_bits(cache.format)) {
     const uint64_t stride = cache.pages.head_stride, beside = stride > 0 && stride < 128 ? 128 / stride : 1;
     p.cluster = p.head_groups * (kv_heads % beside == 0 ? beside : 1);
@@ -1116,7 +1118,8 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   }
   const uint64_t step = attend_step(cache.format, cache.head_dim), steps = (limit + step - 1) / step, cost = attend_cost(cache.format) + steps;
   const uint64_t pairs = rows * kv_heads * p.head_groups;
-  if (pairs > kMostBlocks) refuse("too many rows for these heads");
+  // Over a 4-bit cache the grid is a multiple of eight clusters.
+  if (pairs + (four_bits(cache.format) ? 8 * p.cluster - 1 : 0) > kMostBlocks) refuse("too many rows for these heads");
   // A workgroup for each pair where rows are short or pairs many: no row has more steps than 5 and 9 for each
   // pair a workgroup of the card. Shares cost 3 to 5 us more (each workgroup sums all rows' steps; the join), and
   // spare waiting for the longest row. Us with a pair each / with shares on either side of the line, BF16, 8 KV heads, groups of
@@ -1131,6 +1134,16 @@ AttendPlan plan_attention(const Cache& cache, uint64_t rows, uint64_t query_head
   // rows to 8000 take 21.8, with 48 padding rows 22.0, with 900, where pairs stay whole, 73.
   const uint64_t fit = attend_blocks(cache.format, cache.head_dim, false);
   bool whole = steps * fit <= 5 * fit + 9 * pairs;
+  // A 4-bit cache's pairs are read faster, and a step is not of 128 positions: no row has more positions than most and 8/5 of it for each pair
+  // a workgroup, of at most 5/4. Us with a pair each / with shares, 8 KV heads (of 256: 4), lengths log-uniform from 32:
+  //   E2M1, BF16, 128: 4 rows to 768 9.1 / 9.6, to 1024 10.3 / 9.9; 16 rows to 1024 12.2 / 12.9, to 1408 14.5 / 13.4; 64 rows to 1408
+  //        17.7 / 19.6, to 2048 22.5 / 21.6; 256 rows to 2048 46.2 / 47.3, to 3000 56.2 / 52.9
+  //   INT4, F16, 128: 4 rows to 512 8.9 / 10.3, to 768 11.1 / 10.0; 16 rows to 768 13.0 / 13.5, to 1024 15.5 / 13.9; 64 rows to 1408
+  //        21.7 / 21.7; 256 rows to 2048 52.7 / 54.2
+  //   E2M1, BF16, 64: 4 rows to 1408 10.2 / 9.9; 16 rows to 1408 12.0 / 12.0; 64 rows to 2048 17.8 / 17.4; 256 rows to 3000 44.2 / 45.3
+  //   E2M1, BF16, 256: 4 rows to 512 10.3 / 11.7, to 768 13.1 / 12.1; 16 rows to 768 14.7 / 14.1; 64 rows to 1024 18.3 / 19.1, to 1408
+  //        22.3 / 20.3; 256 rows to 1408 39.3 / 41.5, to 2048 47.7 / 46.3
+  //   INT4, F32, 128: 4 rows to 512 10.9 / 10.3; 16 rows to 512 13.0 / 13.5; 64 rows to 1024 24.1 / 24.5; 256 rows to 2048 71.5 / 70.9
   if (four_bits(cache.format)) {
     const uint64_t most = cache.head_dim == 256 ? 600 : 750;
     whole = 5 * limit * fit <= most * (5 * fit + 8 * std::min(pairs, fit * 5 / 4));
@@ -1189,9 +1202,8 @@ void attend(int32_t device, void* stream, const Cache& cache, const hllm_rocm_kv
   a.group = a.q_heads / a.pages.kv_heads;
   a.head_groups = (int32_t)plan.head_groups;
   a.limit = (int32_t)limit;
-  // F32 queries take twice the LDS.
-  const bool f32 = args->q.dtype == HLLM_DTYPE_F32;
-  a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks(cache.format, (int)D, f32) / plan.cluster * plan.cluster) : plan.blocks);
+  const bool large = args->q.dtype == HLLM_DTYPE_F32 || (args->q.dtype == HLLM_DTYPE_F16 && cache.format == kE2m1);
+  a.blocks = (int32_t)(plan.shared ? std::min(plan.blocks, attend_blocks(cache.format, (int)D, large) / plan.cluster * plan.cluster) : plan.blocks);
   a.shared = plan.shared;
   a.cluster = (int32_t)plan.cluster;
   a.scale_hi = (float)(args->scale * kLog2e);

@@ -123,18 +123,21 @@ constexpr uint64_t kMostSharedRows = 1024;
 // D / 2); F32 queries of 256 elements leave room for one on a CU.
 template <int D>
 constexpr int kAttendBlocks = D == 64 ? 4 : D == 128 ? 3 : 2;
-// Over a 4-bit cache: positions of a wave's tile, and workgroups on a CU.
-#ifndef A4COST
-#define A4COST 2
-#endif
-constexpr int kPair4Cost = A4COST;
+// Over a 4-bit cache. Positions of a wave's tile, of which there are two in LDS, and workgroups on a CU. Us with tiles of 64 and one
+// buffer / 32 and two / 32 and one / 64 and two, 24 rows of 12000 to 30000 positions:
+//   E2M1, 128: 98.5 / 96.0 / 100.5 / 101.2; INT4, 128: 131 / 120 / 130 / 124; E2M1, 64: 72.2 / 76.9 / 73.3 / 68.4;
+//   E2M1, 256: 94.6 / 96.2 / 96.0 / 93.4; INT4, 256, F32: 255 / 213 / 254 / 214
 template <int D>
 constexpr int kAttend4Tile = D == 64 ? 64 : 32;
 template <int D>
 constexpr int kAttend4Blocks = D == 256 ? 2 : 3;
-inline uint64_t attend_blocks(int format, int head_dim, bool f32) {
-  if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : f32 ? 1 : kAttend4Blocks<256>);
-  return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : f32 ? 1 : kAttendBlocks<256>);
+// Steps that starting a pair is counted as. With 1, 2, 3, 4: 16 rows of 2048 positions 21.2, 19.2, 20.2, 19.9 us; 32 rows of
+// 2048 27.0, 24.6, 26.6, 25.9; 64 rows to 8192 33.4, 32.6, 32.2, 33.3; 128 rows to 8192 of 256 83.6, 84.0, 89.7, 95.8.
+constexpr int kPair4Cost = 2;
+// `large`: queries that leave room for one workgroup where heads are of 256 elements (F32; F16 beside an E2M1 cache, as two BF16 parts).
+inline uint64_t attend_blocks(int format, int head_dim, bool large) {
+  if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : large ? 1 : kAttend4Blocks<256>);
+  return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : large ? 1 : kAttendBlocks<256>);
 }
 inline int attend_cost(int format) { return four_bits(format) ? kPair4Cost : kPairCost; }
 // Positions of a step: one tile for each of a workgroup's four waves.

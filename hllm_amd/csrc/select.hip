@@ -662,13 +662,15 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   // their own pages / with others that do, 8 KV heads of 128 and all rows of as many pages of 16:
   //   1 row: 600 pages 15.6 / 16.2, 1000 19.9 / 16.9; 4 rows: 600 15.7 / 16.3, 1000 21.1 / 18.0;
   //   16 rows: 600 17.4 / 20.7, 2000 29.4 / 31.5, 3000 47.6 / 40.8; 32 rows: 600 19.3 / 26.0, 2000 43.9 / 51.3; 64 rows: 1000 48.2 / 59.5
+  if (pairs * kSelectThreads<kLarge> > kMostBlocks * kThreads) refuse("too many rows for these heads");
   if (pages <= 640 || (pairs >= 128 && pages <= 2304)) {
     p.how = kLarge;
     return p;
   }
   p.how = kScored;
   p.chunks = (int)((pages + 4 * score_pages_of(b.head_dimension) - 1) / (4 * score_pages_of(b.head_dimension)));
-  if (pairs * p.chunks > kMostBlocks) p.chunks = (int)(kMostBlocks / pairs);
+  // More would find nothing to do, or wait for others: `pages` is a bound, which may be far above the rows' own.
+  p.chunks = (int)std::min<uint64_t>(p.chunks, std::max<uint64_t>(1, 65535 / pairs));
   p.stride = (pages + 3) / 4 * 4;
   p.bytes = pairs * p.stride * sizeof(uint32_t);
   return p;

@@ -1,6 +1,7 @@
-"""Operators on device memory, for torch tensors: rotary positions (``Rope``, ``rope``) and an
-8-bit paged KV cache (``KvPages``) that is written (``kv_append``), read back (``kv_read``) and
-attended over by one new token a row (``kv_attention``).
+"""Operators on device memory, for torch tensors: rotary positions (``Rope``, ``rope``) and a paged KV
+cache of 8 bits (``KvPages``) or 4 (``Kv4Pages``) that is written (``kv_append``), read back
+(``kv_read``) and attended over by one new token a row (``kv_attention``): over all of a row's pages, or
+over those that ``kv_select`` takes by the bounds of their keys (``KvBounds``, ``kv_bounds``).
 
 Thin calls of the C ABI (include/hllm_rocm.h, which states what each operator computes): they
 check types, shapes and devices, make the outputs that are not given, and enqueue on the current
@@ -13,6 +14,11 @@ library refuses raises ``capi.StageError``.
     pages = KvPages.empty("e4m3", 4096, kv_heads=8, page_tokens=64, head_dim=128)
     q = kv_append(pages, slots, k, v, q=q, rope=plan, positions=positions)
     out = kv_attention(q, pages, page_table, lengths, max_length)
+
+    bounds = KvBounds.empty(pages)          # long rows: over 64 pages of each
+    kv_bounds(pages, bounds, page_table, starts, lengths, max_new=1)  # after each kv_append
+    some, held = kv_select(q, bounds, page_table, lengths, max_length, keep=64)
+    out = kv_attention(q, pages, some, held, 64 * pages.page_tokens)
 """
 from __future__ import annotations
 
@@ -325,8 +331,7 @@ def kv_append(pages: KvPages | Kv4Pages, slots: torch.Tensor, k: torch.Tensor, v
         q_from, q_to = TENSOR.pack(*c), TENSOR.pack(*d)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    capi.check(pages.calls.append(device.index, _stream(device), pages.address, to, rows, a, b, plan, at,
-                                                       q_from, q_to))
+    capi.check(pages.calls.append(device.index, _stream(device), pages.address, to, rows, a, b, plan, at, q_from, q_to))
     return q_out
 
 
@@ -354,9 +359,9 @@ def kv_attention(q: torch.Tensor, pages: KvPages | Kv4Pages, page_table: torch.T
                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q K^T) V of one new token a row, q [rows, q_heads, head_dim], over the first
     ``lengths`` [rows] (int32) positions of the row's pages in ``page_table`` [rows, width]
-    (int32), or of each KV head's own in [rows, kv_heads, width]. ``max_length`` bounds the lengths on the host; ``scale`` is 1 / sqrt(head_dim) unless
-    given. A length of 0 gives zeros, a negative one leaves the row as it was (in a new output:
-    undefined). ``workspace``: a contiguous uint8 tensor of at least ``kv_attention_workspace``
+    (int32), or of each KV head's own in [rows, kv_heads, width], as ``kv_select`` leaves them.
+    ``max_length`` bounds the lengths on the host; ``scale`` is 1 / sqrt(head_dim) unless given. A
+    length of 0 gives zeros, a negative one leaves the row as it was (in a new output: undefined). ``workspace``: a contiguous uint8 tensor of at least ``kv_attention_workspace``
     bytes that no concurrent call uses; made for the call unless given."""
     device = pages.device
     if not isinstance(q, torch.Tensor) or q.dim() != 3:

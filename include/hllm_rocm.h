@@ -539,9 +539,11 @@ typedef struct {
   void* value_scales;
 } hllm_rocm_kv4_pages;
 
-/* The 8-bit cache's operators over a 4-bit one, to the same rules. In attention a key's scale multiplies its group's
- * part of the score and a value's its weight, in F32; a finite key's and query's products stay finite for keys
- * below 2^115. `table_head_stride` as for hllm_rocm_kv_attention_by_head. */
+/* The 8-bit cache's operators over a 4-bit one, to the same rules. In attention E2M1 keys enter their products exactly, and an INT4
+ * key's scale multiplies its group's part of the score in F32; a finite key's and query's products stay finite for
+ * keys below 2^115. A value's scale enters its weight, which is F16 for 16-bit tensors (rounded once, beside INT4 values
+ * twice; weights below 2^-25 of a wave's largest may be lost) and two F16 parts for F32 ones. `table_head_stride` as for
+ * hllm_rocm_kv_attention_by_head. */
 hllm_status hllm_rocm_kv4_append(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
                                  const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
                                  const hllm_rocm_tensor* v, const hllm_rocm_rope* rope,
@@ -594,7 +596,7 @@ hllm_status hllm_rocm_kv4_bounds_update(int32_t device, void* stream, const hllm
 /* Selects `keep` pages of each row for each KV head: its first `first` and last `last` pages (last at least 1, first + last at
  * most keep), and of the others those with the largest scores, of equal scores the first. A page's score is the largest,
  * over the KV head's query heads, of the sum over channels of max(q high, q low), with q as whole numbers times a power of
- * two by the bounds' rule: a sum of whole numbers below 2^24, times the page's scale, times the query's, in F32. That is exact
+ * two by the bounds' rule: a sum of whole numbers below 2^24, times the query's scale and then the page's, in F32. That is exact
  * where it is in F32's normal range, so a selection depends on nothing but its row. A score that is NaN (a page or query that is not
  * finite) is above all others, a page outside the cache below them.
  *
