@@ -56,9 +56,14 @@ def test_values_that_outweigh_their_positions(ops, kind, dtype, dim, large_first
     for most in (length, 150):
         out = ops.kv_attention(q, pages, table, n, most, scale=scale)
         expect, off = forms.attended(q, cache, kind, table, [length, 150], scale, most)
-        # Relative to the output's own size: what is lost of a weight counts with its value.
-        near(out, expect, off)
-        assert (off[0] < 2.0 ** -4 * expect[0].abs().amax(-1, keepdim=True)).all()
+        # From 65520 on, half a step past F16's largest number, rounding gives an infinity.
+        top = 65520.0 if dtype == torch.float16 else math.inf
+        past = expect.abs() - off >= top
+        assert torch.equal(out[past].double(), expect[past].sign() * math.inf)
+        inside = expect.abs() + off < top
+        near(out[inside], expect[inside], off[inside])
+        # Where both kinds count, the bound is small beside the output: what is lost of a weight counts with its value.
+        assert most == 150 or (off[0] < 2.0 ** -4 * expect[0].abs().amax(-1, keepdim=True)).all()
 
 
 # ------------------------------------------------------------------ heads that share cache lines
@@ -297,7 +302,7 @@ def test_the_most_rows(ops, kind):
     out = torch.full((2, rows, 1, dim), 3.0, dtype=torch.float16, device="cuda")
     ops.kv_read(pages, slots, k_out=out[0], v_out=out[1])
     assert torch.equal(out[:, real], torch.stack(ops.kv_read(alone, slots[real]))) and (out[:, 1:5] == 3).all() and (out[:, -5:-1] == 3).all()
-    n = torch.where(slots < 0, -1, 1)
+    n = torch.where(slots < 0, -1, 1).int()
     table = (slots.clamp_min(0) // 8)[:, None].expand(rows, 3).contiguous()
     table[:, 1:] = 60
     n[real] = ints([17, 8, 0, 24])
