@@ -82,6 +82,8 @@ void launch_kv_attention(hipStream_t stream, uint32_t dtype, int format, int hea
 // Without the join.
 void launch_kv4_attention(hipStream_t stream, uint32_t dtype, int format, int head_dim, const AttendArgs& a);
 
+// What takes a page and KV head.
+enum BoundsBy { kByWorkgroup, kByWave, kBySlot };
 struct BoundsArgs {
   Pages pages;
   int8_t* codes;           // [pages][kv_heads][2][D]
@@ -92,8 +94,7 @@ struct BoundsArgs {
   const int32_t* lengths;  // [rows]
   int32_t rows, limit;
   int32_t places;          // pages of a row at most
-  int32_t wide;            // a workgroup a page and head
-  int32_t heads;           // heads that a wave takes one after the other
+  int32_t by;              // BoundsBy
 };
 
 struct SelectArgs {

@@ -109,39 +109,49 @@ __device__ inline uint32_t wave_max(uint32_t v) {
   return row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
 }
 
-// One wave takes a page and some KV heads one after the other (kWaves = 1), or a workgroup's four share a page and head: a lane has
-// eight channels of every (D = 64: eighth, 128: fourth, 256: second) position. The next positions are under way while some are
-// compared.
-template <int F, int D, int kWaves>
-__global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
-  constexpr int L = D / 8, S = 64 / L, C = 8 / S, kDeep = 4;  // lanes of a vector, positions at once, channels left, loads in flight
-  __shared__ float meet[kWaves > 1 ? kWaves : 1][2][kWaves > 1 ? D : 1];
-  __shared__ int spoiled[kWaves];
+// The largest over the L lanes of a slot.
+template <int L>
+__device__ inline uint32_t slot_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));   // the lane's pair's other
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));   // of its four
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // of its eight
+  if constexpr (L == 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));  // of its sixteen
+  return v;
+}
+
+// A page of a row, found from its place among the rows' `places`; false where there is nothing to make.
+struct BoundsPage {
+  int id, count;
+  template <typename Load>
+  __device__ bool find(const BoundsArgs& a, int row, int j, Load&& number) {
+    const int shift = a.pages.page_shift, length = min(number(a.lengths + row), a.limit), start = max(number(a.starts + row), 0);
+    const int p = (start >> shift) + j;
+    if (start >= length || p > (length - 1) >> shift) return false;
+    id = number(a.table + (uint64_t)row * a.table_stride + p);
+    count = min(1 << shift, length - (p << shift));
+    return id >= 0 && id < a.pages.pages;
+  }
+};
+
+// A page and KV head for each slot of L lanes, a lane eight channels of all positions: nothing is exchanged between lanes but the
+// largest magnitude. For many short pages. Bound by its reads where it is at its best: 8 rows of 10000 positions, 8 KV heads of 128, E2M1,
+// pages of 16: 14.5 us, 3.7 TB/s of what is read and written.
+template <int F, int D>
+__global__ void __launch_bounds__(kThreads) kv_bounds_slots_kernel(BoundsArgs a) {
+  constexpr int L = D / 8, S = 64 / L, kDeep = 8;
   const Pages& c = a.pages;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int parts = (c.kv_heads + a.heads - 1) / a.heads;  // of a page's heads
-  const uint64_t item = kWaves > 1 ? blockIdx.x : (uint64_t)blockIdx.x * 4 + wave;
-  const uint64_t place = item / parts;
-  const int row = (int)(place / a.places), j = (int)(place - (uint64_t)row * a.places);
-  if (row >= a.rows) return;
-  const int shift = c.page_shift, length = min(uniform_load(a.lengths + row), a.limit), start = max(uniform_load(a.starts + row), 0);
-  const int p = (start >> shift) + j;
-  if (start >= length || p > (length - 1) >> shift) return;
-  const int id = uniform_load(a.table + (uint64_t)row * a.table_stride + p);
-  if (id < 0 || id >= c.pages) return;
-  const int count = min(1 << shift, length - (p << shift));
-  const int slot = lane / L, d = lane % L * 8;
-  int h = (int)(item - place * parts) * a.heads;
-  const int last = min(h + a.heads, c.kv_heads);
-  const int first = kWaves > 1 ? wave * S * kDeep : 0;
-  int t = first;
+  const uint32_t item = (blockIdx.x * 4 + (threadIdx.x >> 6)) * S + (threadIdx.x & 63) / L;
+  const uint32_t place = item / (uint32_t)c.kv_heads, row = place / (uint32_t)a.places;
+  const int h = (int)(item - place * c.kv_heads), d = (int)(threadIdx.x % L) * 8;
+  BoundsPage page;
+  if (row >= (uint32_t)a.rows || !page.find(a, (int)row, (int)(place - row * a.places), [](const int32_t* at) { return *at; })) return;
+  const uint8_t* from = c.keys + (uint64_t)page.id * c.page_stride + (uint64_t)h * c.head_stride;
+  const uint64_t own = (uint64_t)page.id * c.kv_heads + h, vector = own << c.page_shift;
   Keys8<F, D> k[kDeep];
-  const auto load = [&] {
-    const uint8_t* from = c.keys + (uint64_t)id * c.page_stride + (uint64_t)h * c.head_stride;
-    const uint64_t vector = ((uint64_t)id * c.kv_heads + h) << shift;
+  const auto load = [&](int t) {
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
-      const int at = min(t + i * S + slot, count - 1);  // the last position again changes nothing
+      const int at = min(t + i, page.count - 1);  // the last position again changes nothing
       k[i].load(c, from + (uint64_t)(uint32_t)at * c.token_stride, vector + at, d);
     }
   };
@@ -149,15 +159,12 @@ __global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
   bool numbers = true;
 #pragma unroll
   for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
-  load();
-  for (;;) {
+  load(0);
+  for (int t = 0; t < page.count; t += kDeep) {
     Keys8<F, D> now[kDeep];
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) now[i] = k[i];
-    const int head = h;
-    t += kWaves * S * kDeep;
-    if (t >= count) ++h, t = first;
-    if (h < last) load();
+    if (t + kDeep < page.count) load(t + kDeep);
 #pragma unroll
     for (int i = 0; i < kDeep; i += 2) {
       float x[8], y[8];
@@ -169,52 +176,110 @@ __global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
         low[e] = fminf(fminf(low[e], x[e]), y[e]);
       }
     }
-    if (h == head) continue;
-    reduce_slots<L>(high, [](float x, float y) { return fmaxf(x, y); });
-    reduce_slots<L>(low, [](float x, float y) { return fminf(x, y); });
-    bool bad = __any(!numbers);
-    const int channel = d + (lane & 32 ? 4 : 0) + (L <= 16 && (lane & 16) ? 2 : 0) + (L == 8 && (lane & 8) ? 1 : 0);
-    if constexpr (kWaves > 1) {
+  }
+  uint32_t most = numbers ? 0u : 0x7f800000u;
 #pragma unroll
-      for (int e = 0; e < C; ++e) meet[wave][0][channel + e] = high[e], meet[wave][1][channel + e] = low[e];
-      if (lane == 0) spoiled[wave] = bad;
-      __syncthreads();
-      if (wave > 0) return;
+  for (int e = 0; e < 8; ++e) most = max(most, max(__float_as_uint(high[e]) & 0x7fffffffu, __float_as_uint(low[e]) & 0x7fffffffu));
+  most = slot_max<L>(most);
+  const bool bad = most >= 0x7f800000u;
+  const uint32_t power = whole_power(most);
+  const float inverse = __uint_as_float((254u - power) << 23);
+  int x[2][8];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        bad |= spoiled[w] != 0;
+  for (int e = 0; e < 8; ++e) x[0][e] = bad ? 0 : (int)rintf(high[e] * inverse), x[1][e] = bad ? 0 : (int)rintf(low[e] * inverse);
 #pragma unroll
-        for (int e = 0; e < C; ++e) high[e] = fmaxf(high[e], meet[w][0][channel + e]), low[e] = fminf(low[e], meet[w][1][channel + e]);
+  for (int which = 0; which < 2; ++which) *reinterpret_cast<uint2v*>(a.codes + (own * 2 + which) * D + d) = bytes8(x[which]);
+  if (d == 0) a.scales[own] = bad ? NAN : __uint_as_float(power << 23);
+}
+
+// A wave (kWaves = 1) or a workgroup's four for a page and KV head, for few pages or long ones: a lane has
+// eight channels of every (D = 64: eighth, 128: fourth, 256: second) position. The next positions are under way while some are
+// compared.
+template <int F, int D, int kWaves>
+__global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
+  constexpr int L = D / 8, S = 64 / L, C = 8 / S, kDeep = 4;  // lanes of a vector, positions at once, channels left, loads in flight
+  __shared__ float meet[kWaves > 1 ? kWaves : 1][2][kWaves > 1 ? D : 1];
+  __shared__ int spoiled[kWaves];
+  const Pages& c = a.pages;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t item = kWaves > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
+  const uint32_t place = item / (uint32_t)c.kv_heads, row = place / (uint32_t)a.places;
+  const int h = (int)(item - place * c.kv_heads), slot = lane / L, d = lane % L * 8;
+  BoundsPage page;
+  if (row >= (uint32_t)a.rows || !page.find(a, (int)row, (int)(place - row * a.places), [](const int32_t* at) { return uniform_load(at); })) return;
+  const uint8_t* from = c.keys + (uint64_t)page.id * c.page_stride + (uint64_t)h * c.head_stride;
+  const uint64_t own = (uint64_t)page.id * c.kv_heads + h, vector = own << c.page_shift;
+  Keys8<F, D> k[kDeep];
+  const auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int at = min(t + i * S + slot, page.count - 1);  // the last position again changes nothing
+      k[i].load(c, from + (uint64_t)(uint32_t)at * c.token_stride, vector + at, d);
+    }
+  };
+  float high[8], low[8];
+  bool numbers = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
+  constexpr int kStep = kWaves * S * kDeep;
+  const int first = kWaves > 1 ? wave * S * kDeep : 0;
+  load(first);
+  for (int t = first; t < page.count; t += kStep) {
+    Keys8<F, D> now[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) now[i] = k[i];
+    if (t + kStep < page.count) load(t + kStep);
+#pragma unroll
+    for (int i = 0; i < kDeep; i += 2) {
+      float x[8], y[8];
+      numbers &= now[i].values(x);
+      numbers &= now[i + 1].values(y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        high[e] = fmaxf(fmaxf(high[e], x[e]), y[e]);
+        low[e] = fminf(fminf(low[e], x[e]), y[e]);
       }
     }
-    uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < C; ++e) most = max(most, max(__float_as_uint(high[e]) & 0x7fffffffu, __float_as_uint(low[e]) & 0x7fffffffu));
-    most = wave_max(most);
-    bad |= most >= 0x7f800000u;
-    const uint32_t power = whole_power(most);
-    const float inverse = __uint_as_float((254u - power) << 23);
-    const uint64_t page = (uint64_t)id * c.kv_heads + head;
-    uint32_t codes[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      codes[0] |= ((uint32_t)(int)rintf(high[e] * inverse) & 255u) << (8 * e);
-      codes[1] |= ((uint32_t)(int)rintf(low[e] * inverse) & 255u) << (8 * e);
-    }
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      int8_t* to = a.codes + (page * 2 + which) * D + channel;
-      const uint32_t w = bad ? 0u : codes[which];
-      if constexpr (C == 1) *reinterpret_cast<uint8_t*>(to) = (uint8_t)w;
-      if constexpr (C == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
-      if constexpr (C == 4) *reinterpret_cast<uint32_t*>(to) = w;
-    }
-    if (lane == 0) a.scales[page] = bad ? NAN : __uint_as_float(power << 23);
-    if (h >= last) return;
-    numbers = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) high[i] = -INFINITY, low[i] = INFINITY;
   }
+  reduce_slots<L>(high, [](float x, float y) { return fmaxf(x, y); });
+  reduce_slots<L>(low, [](float x, float y) { return fminf(x, y); });
+  bool bad = __any(!numbers);
+  const int channel = d + (lane & 32 ? 4 : 0) + (L <= 16 && (lane & 16) ? 2 : 0) + (L == 8 && (lane & 8) ? 1 : 0);
+  if constexpr (kWaves > 1) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) meet[wave][0][channel + e] = high[e], meet[wave][1][channel + e] = low[e];
+    if (lane == 0) spoiled[wave] = bad;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      bad |= spoiled[w] != 0;
+#pragma unroll
+      for (int e = 0; e < C; ++e) high[e] = fmaxf(high[e], meet[w][0][channel + e]), low[e] = fminf(low[e], meet[w][1][channel + e]);
+    }
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < C; ++e) most = max(most, max(__float_as_uint(high[e]) & 0x7fffffffu, __float_as_uint(low[e]) & 0x7fffffffu));
+  most = wave_max(most);
+  bad |= most >= 0x7f800000u;
+  const uint32_t power = whole_power(most);
+  const float inverse = __uint_as_float((254u - power) << 23);
+  uint32_t codes[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < C; ++e) {
+    codes[0] |= ((uint32_t)(int)rintf(high[e] * inverse) & 255u) << (8 * e);
+    codes[1] |= ((uint32_t)(int)rintf(low[e] * inverse) & 255u) << (8 * e);
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    int8_t* to = a.codes + (own * 2 + which) * D + channel;
+    const uint32_t w = bad ? 0u : codes[which];
+    if constexpr (C == 1) *reinterpret_cast<uint8_t*>(to) = (uint8_t)w;
+    if constexpr (C == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
+    if constexpr (C == 4) *reinterpret_cast<uint32_t*>(to) = w;
+  }
+  if (lane == 0) a.scales[own] = bad ? NAN : __uint_as_float(power << 23);
 }
 
 // ---------------------------------------------------------------- scores
@@ -532,13 +597,14 @@ __global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectA
 
 template <int F>
 void bounds_format(hipStream_t stream, int head_dim, const BoundsArgs& a) {
-  const uint64_t items = (uint64_t)a.rows * a.places * ((a.pages.kv_heads + a.heads - 1) / a.heads);
+  const unsigned items = (unsigned)a.rows * a.places * a.pages.kv_heads;
   const auto run = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    if (a.wide)
-      kv_bounds_kernel<F, D, 4><<<(unsigned)items, kThreads, 0, stream>>>(a);
-    else
-      kv_bounds_kernel<F, D, 1><<<(unsigned)((items + 3) / 4), kThreads, 0, stream>>>(a);
+    constexpr unsigned kSlots = 4 * 512 / D;  // of a workgroup
+    if (a.by == kByWorkgroup) kv_bounds_kernel<F, D, 4><<<items, kThreads, 0, stream>>>(a);
+    if (a.by == kByWave) kv_bounds_kernel<F, D, 1><<<(items + 3) / 4, kThreads, 0, stream>>>(a);
+    if constexpr (D <= 128)
+      if (a.by == kBySlot) kv_bounds_slots_kernel<F, D><<<(items + kSlots - 1) / kSlots, kThreads, 0, stream>>>(a);
   };
   if (head_dim == 64) run(std::integral_constant<int, 64>{});
   if (head_dim == 128) run(std::integral_constant<int, 128>{});
@@ -634,9 +700,13 @@ void update_bounds(int32_t device, void* stream, const Cache& cache, const hllm_
   // Long pages, and pages that a lone wave reads in many steps where there are few of them (9 rows of 4 heads of 256 in pages of 64:
   // 5.5 us with a wave a page and head).
   const uint64_t loads = (uint64_t)cache.page_tokens * (cache.head_dim / 8) / 64;  // of a wave for a page and head
-  a.wide = cache.page_tokens > 128 || (items <= 1024 && loads > 4);
-  // Many pages: a wave takes some heads, which have the page's number and the loads under way in common.
-  a.heads = a.wide || items < 16384 ? 1 : items < 32768 ? 2 : 4;
+  // Many short pages: a slot of a wave each, for the maxima over a wave's slots take as long as a short page's elements. Us by waves / by slots:
+  //   E2M1, 128, pages of 16: 1024 items 3.0 / 3.8, 4096 4.1 / 4.0, 8192 6.5 / 5.5, 40000 20.7 / 14.5; of 32: 20032 14.9 / 12.4; E4M3,
+  //   64, of 16: 4096 4.2 / 4.6, 40000 21.9 / 11.5; E2M1, 64, of 8: 32768 16.9 / 6.1; INT8, 128, of 16: 40000 25.1 / 23.2, of 32: 20032
+  //   21.6 / 21.8; longer pages and 256: INT4, 128, of 64: 10048 17.1 / 18.6; E2M1, 64, of 64: 10048 9.2 / 9.9; E4M3, 256, of 16: 20000 22.8 / 23.4
+  a.by = cache.page_tokens > 128 || (items <= 1024 && loads > 4)                        ? kByWorkgroup
+         : cache.page_tokens <= 32 && cache.head_dim <= 128 && items >= 8192            ? kBySlot
+                                                                                        : kByWave;
   OnDevice on(device);
   launch_bounds(static_cast<hipStream_t>(stream), cache.format, cache.head_dim, a);
   HIP_CHECK(hipGetLastError());

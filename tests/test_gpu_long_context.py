@@ -105,7 +105,7 @@ def test_any_sizes(ops, seed):
 @pytest.mark.parametrize("rows,places", [(63, 36), (65, 72), (1, 2100)])
 @pytest.mark.parametrize("kind,heads,dim", [("e2m1", 8, 64), ("int4", 7, 64), ("int8", 7, 128), ("e4m3", 9, 64), ("e2m1", 3, 256)])
 def test_bounds_of_many_pages(ops, kind, rows, places, heads, dim):
-    """One, two and four heads a wave, heads that are no multiple of them, rows that end early."""
+    """A page and head for each wave and for each slot of one, heads that are no multiple of the slots, rows that end early."""
     page = 8
     table = torch.randperm(rows * places, generator=torch.Generator("cuda").manual_seed(1), device="cuda").int().view(rows, places)
     cache = forms.make_pages(kind, rows * places, heads, page, dim)
@@ -124,6 +124,40 @@ def test_bounds_of_many_pages(ops, kind, rows, places, heads, dim):
     at = table[made].long()
     assert torch.equal(bounds.codes[at], codes[at]) and torch.equal(bounds.scales[at].double(), power[at])
     assert (bounds.codes[table[~made].long()] == 55).all()
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("heads,dim,page", [(2, 64, 8), (3, 128, 16), (5, 64, 32)])
+def test_bounds_of_extreme_keys_among_many_pages(ops, kind, heads, dim, page):
+    """Zero, tiny, huge and not finite keys beside each other, last pages that are not whole, pages outside the cache."""
+    rows, places = 70, 60
+    assert rows * places * heads >= 8192
+    table = torch.randperm(rows * places, generator=torch.Generator("cuda").manual_seed(1), device="cuda").int().view(rows, places)
+    table[3, 5], table[4, 6] = -1, rows * places
+    cache = forms.make_pages(kind, rows * places, heads, page, dim, stale=True)
+    lengths = [page * places - r % page for r in range(rows)]
+    x = draw(8 * page, heads, dim, torch.float32, 1).view(8, page, heads, dim)
+    x[1] = 0
+    x[2] *= 2.0 ** -105
+    x[3] *= 1e37
+    x[4, 5, 0, 9] = math.nan
+    x[5, 7, 1, 60] = -math.inf
+    x[6] = -1.5
+    at = torch.arange(page, device="cuda")
+    for r in range(rows):
+        for p in (0, 7, places - 1):
+            n = page if p < places - 1 else lengths[r] - p * page
+            forms.hold(cache, kind, "keys", table[r, p].long().expand(n), at[:n], x[(r + p) % 8, :n])
+    pages = described(ops, kind, cache)
+    bounds = ops.KvBounds.empty(pages)
+    ops.kv_bounds(pages, bounds, table, ints([0] * rows), ints(lengths), page * places)
+    for r in range(0, rows, 3):
+        for p in (0, 7, places - 1):
+            id = int(table[r, p])
+            for h in range(heads):
+                codes, scale = forms.bounds_of(cache, kind, id, h, page if p < places - 1 else lengths[r] - p * page)
+                assert torch.equal(bounds.codes[id, h], codes), (r, p, h)
+                assert bounds.scales[id, h].item() == scale or (math.isnan(scale) and torch.isnan(bounds.scales[id, h]))
 
 
 @pytest.mark.parametrize("rows,heads", [(2, 4), (15, 8), (16, 8)])
