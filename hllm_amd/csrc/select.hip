@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) kv_bounds_slots_kernel(BoundsArgs a)
 
 // A wave (kWaves = 1) or a workgroup's four for a page and KV head, for few pages or long ones: a lane has
 // eight channels of every (D = 64: eighth, 128: fourth, 256: second) position. The next positions are under way while some are
-// compared.
+// compared. After one token a row it is a launch and a chain of row, page, keys: 32 rows of 8 heads of 128 in pages of 16 2.6 us. Prompts in
+// long pages are bound by their reads: 8 rows of 10000 positions, 4 heads of 256, INT8, pages of 64: 22.1 us, 3.9 TB/s.
 template <int F, int D, int kWaves>
 __global__ void __launch_bounds__(kThreads) kv_bounds_kernel(BoundsArgs a) {
   constexpr int L = D / 8, S = 64 / L, C = 8 / S, kDeep = 4;  // lanes of a vector, positions at once, channels left, loads in flight
@@ -413,7 +414,9 @@ __device__ inline int pages_of(const SelectArgs& a, int row, int& length) {
   return length <= 0 ? 0 : ((length - 1) >> a.page_shift) + 1;
 }
 
-// Scores into the workspace, for rows of more pages than one workgroup scores.
+// Scores into the workspace, for rows of more pages than one workgroup scores. 32 rows of 4000 pages, 8 heads of 128 (266 MB of bounds):
+// 86 us with the selection, the bounds read at 3.7 TB/s. What holds it there has not been found: pages in order take 80 us, 1024 to 8192
+// workgroups the same, a row's heads on one die, which then reads the scales' lines once, 84.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 4) kv_score_kernel(SelectArgs a) {
   const int row = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
@@ -442,7 +445,8 @@ constexpr int kDigit = 11;  // bits that a pass over the scores settles
 
 // A workgroup selects a row's pages for one KV head. Passes over the scores, upper bits first, count how many there are of each value of
 // the next bits among those that may still be the last one selected; then the pages above it are written, and of those at
-// it the first ones, in their order.
+// it the first ones, in their order. A selection by itself takes some 8 us, five barriers of sixteen waves a pass over eleven bits; with its
+// scores 32 rows of 12000 to 30000 positions in pages of 16, 8 heads of 128, 35 us: the longest row's workgroup, alone on its CU.
 template <typename T, int D, Select kHow>
 __global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectArgs a) {
   constexpr bool kHere = kHow != kScored;
