@@ -66,6 +66,35 @@ def test_values_that_outweigh_their_positions(ops, kind, dtype, dim, large_first
         assert most == 150 or (off[0] < 2.0 ** -4 * expect[0].abs().amax(-1, keepdim=True)).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("apart", [32, 64, 1024])
+def test_waves_and_parts_of_very_different_values(ops, kind, dtype, dim, apart):
+    """One in four stretches of `apart` positions (a wave's tiles, or a share's steps) holds the output: weights of 2^-80 and values
+    2^190 times the others', behind others of that stretch with weights of 2^-40."""
+    page, length = 64, 8000
+    table, count = paged([length, 1500], page)
+    cache = forms.make_pages(kind, count, 1, page, dim, stale=True)
+    for r, n in enumerate((length, 1500)):
+        at = torch.arange(n, device="cuda")
+        here = at // apart % 4 == 1
+        late = here & (at >= n // 2)
+        x = torch.zeros(n, 1, dim, device="cuda")
+        x[:, :, 0] = torch.where(late, -4.0, torch.where(here, 0.0, 4.0))[:, None]
+        v = draw(n, 1, dim, torch.float32, r + 1) * torch.where(late, 2.0 ** 90, 2.0 ** -100)[:, None, None]
+        for name, y in (("keys", x), ("values", v)):
+            forms.hold(cache, kind, name, table[r].long()[at // page], at % page, y)
+    q = torch.zeros(2, 4, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    scale = 40 * math.log(2) / 4
+    pages = ops.Kv4Pages(**cache)
+    out = ops.kv_attention(q, pages, table, ints([length, 1500]), length, scale=scale)
+    expect, off = forms.attended(q, cache, kind, table, [length, 1500], scale)
+    near(out, expect, off)
+    assert (off < 2.0 ** -3 * expect.abs().amax(-1, keepdim=True)).all()
+
+
 # ------------------------------------------------------------------ heads that share cache lines
 
 
@@ -166,6 +195,19 @@ def test_selection_at_the_plans_borders(ops, rows, heads, pages):
     """Workgroups of 256 and of 1024 threads that score their own pages, and pages that others score."""
     lengths = [8 * (pages - 3 * r if r % 2 else pages) - r % 8 for r in range(rows)]
     select_case(ops, torch.bfloat16, lengths, 2 * heads, heads, 64, 8, 20, 1, 2, ties=pages % 2 == 1)
+
+
+def test_selection_by_workgroups_that_score_many_pages(ops):
+    """More pages than the workgroups of 512 pairs score at once, and than a workgroup holds; other rows are short."""
+    page, width, heads = 8, 20000, 8
+    lengths = [page * width - 3, 500] + [40] * 61 + [page * width]
+    pages = ops.Kv4Pages.empty("e2m1", 3000, heads, page, 128)
+    bounds = random_bounds(ops, pages)
+    table = torch.randint(0, 3000, (64, width), generator=torch.Generator("cuda").manual_seed(1), device="cuda", dtype=torch.int32)
+    q = draw(64, heads, 128, torch.bfloat16, 1)
+    got, n = ops.kv_select(q, bounds, table, ints(lengths), page * width, 9)
+    expect, expect_n = forms.selected(q, bounds.codes, bounds.scales, table, lengths, page, 9, 1, 1)
+    assert torch.equal(got.cpu(), expect) and torch.equal(n.cpu(), expect_n)
 
 
 def test_selection_of_a_bound_far_above_the_rows(ops):
