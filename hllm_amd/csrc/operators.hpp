@@ -135,7 +135,8 @@ constexpr int kAttend4Blocks = D == 256 ? 2 : 3;
 // Steps that starting a pair is counted as. With 1, 2, 3, 4: 16 rows of 2048 positions 21.2, 19.2, 20.2, 19.9 us; 32 rows of
 // 2048 27.0, 24.6, 26.6, 25.9; 64 rows to 8192 33.4, 32.6, 32.2, 33.3; 128 rows to 8192 of 256 83.6, 84.0, 89.7, 95.8.
 constexpr int kPair4Cost = 2;
-// `large`: queries that leave room for one workgroup where heads are of 256 elements (F32; F16 beside an E2M1 cache, as two BF16 parts).
+// `large`: queries that leave room for one workgroup where heads are of 256 elements (F32; F16 beside an E2M1 cache, as two BF16 parts:
+// 24 rows of 12000 to 30000 positions 120 us with shares for one, 128 with shares for two; 64 to 2048 27.2 and 32.5).
 inline uint64_t attend_blocks(int format, int head_dim, bool large) {
   if (four_bits(format)) return 256 * (head_dim == 64 ? kAttend4Blocks<64> : head_dim == 128 ? kAttend4Blocks<128> : large ? 1 : kAttend4Blocks<256>);
   return 256 * (head_dim == 64 ? kAttendBlocks<64> : head_dim == 128 ? kAttendBlocks<128> : large ? 1 : kAttendBlocks<256>);

@@ -574,8 +574,8 @@ typedef struct {
 
 /* Makes the bounds of the pages that hold positions starts[row] .. lengths[row] - 1 of each row (a negative start counts as
  * 0), from all positions of those pages below lengths[row]: after a write of these positions. A row whose start is not
- * below its length, and pages outside the cache, have nothing made. At most max_new positions of a row, and
- * table_width * page_tokens in all, are looked at. Rows may share a page if their lengths agree on it. */
+ * below its length, and pages outside the cache, have nothing made. Pages are made for max_new positions of a row from its start
+ * on (and maybe the page behind them), within table_width pages. Rows may share a page if their lengths agree on it. */
 typedef struct {
   uint64_t rows;
   const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */
