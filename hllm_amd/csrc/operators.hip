@@ -118,8 +118,9 @@ __device__ inline void wave_meets() {
 }
 
 // A thread's two eights of a 4-bit cache's vector, keys turned. The largest magnitude of 32 elements is found over four threads in LDS; a
-// value's bytes go there and back, because those that lie beside each other in the cache are of different threads. Bound by memory and by
-// that exchange: 2011 rows of 20 + 4 heads of 256, BF16 to INT4, 20.1 us (2.6 TB/s; to 8 bits 12.7); 64 rows of 32 + 8 heads of 128 5.2.
+// value's bytes go there and back, because those that lie beside each other in the cache are of different threads. Bound by memory as
+// the 8-bit cache's is: 2011 rows of 20 + 4 heads of 256, BF16 to INT4, 12.9 us, 4.0 TB/s (to INT8 12.6); 16384 rows of 32 + 8 heads of 128, F16
+// 80.7 us, 4.4 TB/s (79.1).
 template <int F>
 __device__ inline void append_four(const RotateArgs& a, const float* x, int slot, bool cached, bool is_v, int in_block, int u,
                                    int h, int d0, int d1) {
