@@ -310,7 +310,8 @@ struct Queries {
 // kPages `first` on in steps of `step`. With a query's positive and negative elements apart, the sum over channels of the
 // larger product is one product [high, low] x [max(q, 0), min(q, 0)] of twice the length, on the matrix units in
 // bytes, with the query heads of a KV head as columns. Sums of whole numbers below 2^24 and powers of two are exact. The first
-// bounds are under way while the workgroup rounds the queries.
+// bounds are under way while the workgroup rounds the queries, and the next ones while some are multiplied (32 rows of 1200 pages of 8 heads of
+// 128: 23.8 us, 26.0 without; 128 of 1000: 87, 95).
 template <int D>
 constexpr int kScorePages = D == 64 ? 64 : D == 128 ? 32 : 16;
 template <typename T, int D, int kWaves, typename Keep>
@@ -382,13 +383,22 @@ __device__ inline void score_pages(const SelectArgs& a, Queries<D>& queries, int
     const float q_scale = queries.scale[col];
     const bool no_query = __any(q_scale != q_scale);
     for (; t < count; t += kPages * step) {
+      int4v high_now[kTiles][KK], low_now[kTiles][KK];
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) high_now[i][kk] = high[i][kk], low_now[i][kk] = low[i][kk];
+      const float scale_now = scale;
+      const bool absent_now = absent;
+      if (t + kPages * step < count) load(t + kPages * step);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         int4v dot = {0, 0, 0, 0};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[i][kk], up[kk], dot, 0, 0, 0);
-          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[i][kk], down[kk], dot, 0, 0, 0);
+          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(high_now[i][kk], up[kk], dot, 0, 0, 0);
+          dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(low_now[i][kk], down[kk], dot, 0, 0, 0);
         }
         float mine = 0.0f;
 #pragma unroll
@@ -398,13 +408,12 @@ __device__ inline void score_pages(const SelectArgs& a, Queries<D>& queries, int
         }
         // A lane of the first four of its row has the page 16 i + 4 quad + col; a page's scale does not change which head is the largest.
         const int of = 16 * i + 4 * quad + (col & 3), place = t + of;
-        const float by = __shfl(scale, of, 64);
-        const bool gone = __shfl((int)absent, of, 64);
+        const float by = __shfl(scale_now, of, 64);
+        const bool gone = __shfl((int)absent_now, of, 64);
         uint32_t key = by != by || no_query ? kNoNumber : ordered(mine * by);
         if (gone) key = 0;
         if (col < 4 && place < count) keep(place, key, g0 > 0);
       }
-      if (t + kPages * step < count) load(t + kPages * step);
     }
   }
 }
@@ -415,8 +424,8 @@ __device__ inline int pages_of(const SelectArgs& a, int row, int& length) {
 }
 
 // Scores into the workspace, for rows of more pages than one workgroup scores. 32 rows of 4000 pages, 8 heads of 128 (266 MB of bounds):
-// 86 us with the selection, the bounds read at 3.7 TB/s. What holds it there has not been found: pages in order take 80 us, 1024 to 8192
-// workgroups the same, a row's heads on one die, which then reads the scales' lines once, 84.
+// 83 us with the selection, the bounds read at 3.8 TB/s, 5.3 with the lines of the pages' scales, of which a KV head uses four bytes. A row's heads
+// on one die, which then reads those lines once, take 81 to 83; pages in order 80.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 4) kv_score_kernel(SelectArgs a) {
   const int row = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
@@ -446,7 +455,7 @@ constexpr int kDigit = 11;  // bits that a pass over the scores settles
 // A workgroup selects a row's pages for one KV head. Passes over the scores, upper bits first, count how many there are of each value of
 // the next bits among those that may still be the last one selected; then the pages above it are written, and of those at
 // it the first ones, in their order. A selection by itself takes some 8 us, five barriers of sixteen waves a pass over eleven bits; with its
-// scores 32 rows of 12000 to 30000 positions in pages of 16, 8 heads of 128, 35 us: the longest row's workgroup, alone on its CU.
+// scores 32 rows of 12000 to 30000 positions in pages of 16, 8 heads of 128, 33 us: the longest row's workgroup, alone on its CU.
 template <typename T, int D, Select kHow>
 __global__ void __launch_bounds__(kSelectThreads<kHow>) kv_select_kernel(SelectArgs a) {
   constexpr bool kHere = kHow != kScored;
@@ -734,8 +743,8 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   if (pages <= (uint64_t)kSelectThreads<kSmall> * kSelectOwn<kSmall>) return p;
   // With few pages, or workgroups for half the card, one launch takes less time than two. Us with workgroups that score
   // their own pages / with others that do, 8 KV heads of 128 and all rows of as many pages of 16:
-  //   1 row: 600 pages 15.6 / 16.2, 1000 19.9 / 16.9; 4 rows: 600 15.7 / 16.3, 1000 21.1 / 18.0;
-  //   16 rows: 600 17.4 / 20.7, 2000 29.4 / 31.5, 3000 47.6 / 40.8; 32 rows: 600 19.3 / 26.0, 2000 43.9 / 51.3; 64 rows: 1000 48.2 / 59.5
+  //   1 row: 600 pages 15.6 / 16.2, 1000 19.9 / 16.9; 4 rows: 600 15.7 / 16.3, 1000 21.1 / 18.0; 16 rows: 700 17.1 / 20.4, 2304 29.3 / 29.6,
+  //   3000 47.6 / 40.8; 32 rows: 700 19.2 / 25.0, 1875 37.0 / 45.9; 64 rows: 1200 51.5 / 64.2, 2304 85.6 / 102; 128 rows: 1000 87.4 / 108
   if (pairs * kSelectThreads<kLarge> > kMostBlocks * kThreads) refuse("too many rows for these heads");
   if (pages <= 640 || (pairs >= 128 && pages <= 2304)) {
     p.how = kLarge;
@@ -743,8 +752,9 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   }
   p.how = kScored;
   p.chunks = (int)((pages + 4 * score_pages_of(b.head_dimension) - 1) / (4 * score_pages_of(b.head_dimension)));
-  // More would find nothing to do, or wait for others: `pages` is a bound, which may be far above the rows' own.
-  p.chunks = (int)std::min<uint64_t>(p.chunks, std::max<uint64_t>(1, 65535 / pairs));
+  // The card holds 1024 of these workgroups. With more, each scores little for its start, and a bound far above the rows' own pages leaves many
+  // idle: 8 rows of 4000 pages 31.4 us, with 1024 28.3; 32 rows 85.4 and 83.4.
+  p.chunks = (int)std::min<uint64_t>(p.chunks, std::max<uint64_t>(1, 1024 / pairs));
   p.stride = (pages + 3) / 4 * 4;
   p.bytes = pairs * p.stride * sizeof(uint32_t);
   return p;
