@@ -361,8 +361,9 @@ def kv_attention(q: torch.Tensor, pages: KvPages | Kv4Pages, page_table: torch.T
     ``lengths`` [rows] (int32) positions of the row's pages in ``page_table`` [rows, width]
     (int32), or of each KV head's own in [rows, kv_heads, width], as ``kv_select`` leaves them.
     ``max_length`` bounds the lengths on the host; ``scale`` is 1 / sqrt(head_dim) unless given. A
-    length of 0 gives zeros, a negative one leaves the row as it was (in a new output: undefined). ``workspace``: a contiguous uint8 tensor of at least ``kv_attention_workspace``
-    bytes that no concurrent call uses; made for the call unless given."""
+    length of 0 gives zeros, a negative one leaves the row as it was (in a new output: undefined).
+    ``workspace``: a contiguous uint8 tensor of at least ``kv_attention_workspace`` bytes that no
+    concurrent call uses; made for the call unless given."""
     device = pages.device
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [rows, heads, head_dim]")

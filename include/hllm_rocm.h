@@ -575,7 +575,8 @@ typedef struct {
 /* Makes the bounds of the pages that hold positions starts[row] .. lengths[row] - 1 of each row (a negative start counts as
  * 0), from all positions of those pages below lengths[row]: after a write of these positions. A row whose start is not
  * below its length, and pages outside the cache, have nothing made. Pages are made for max_new positions of a row from its start
- * on (and maybe the page behind them), within table_width pages. Rows may share a page if their lengths agree on it. */
+ * on (and maybe the page behind them), within table_width pages: rows * these pages * kv_heads below 2^24. Rows may share a page if
+ * their lengths agree on it. */
 typedef struct {
   uint64_t rows;
   const int32_t* page_table;  /* [rows][table_width], rows table_stride entries apart */
@@ -604,7 +605,8 @@ hllm_status hllm_rocm_kv4_bounds_update(int32_t device, void* stream, const hllm
  * where the row has fewer pages, and selected_lengths [rows] the positions that they hold: what
  * hllm_rocm_kv_attention_by_head and hllm_rocm_kv4_attention take as a table of rows kv_heads * keep entries apart
  * and heads `keep` apart. A row's length counts at most max_length and table_width * page_tokens positions. A
- * negative length marks a padding row: it is passed on and the row's part of `selected` left as it was. */
+ * negative length marks a padding row: it is passed on and the row's part of `selected` left as it was. rows * kv_heads is below
+ * 2^24, where rows may have more than 512 pages below 2^22. */
 typedef struct {
   uint64_t rows;
   const int32_t* page_table;

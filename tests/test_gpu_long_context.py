@@ -302,6 +302,28 @@ def test_results_do_not_depend_on_the_run_or_the_workspace(ops, kind, dtype):
                 call(wrong)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("q_heads,heads,dim", [(8, 4, 64), (6, 2, 128), (40, 2, 128), (128, 4, 64), (5, 1, 256)])
+def test_clusters_keep_to_their_workspace(ops, kind, dtype, q_heads, heads, dim):
+    """Calls with heads that share cache lines write nothing behind the bytes that they ask for; INT4 scales may be negative."""
+    lengths = [7000, 30, 2500]
+    table, count = paged(lengths, 16)
+    cache = forms.make_pages(kind, count, heads, 16, dim, True)
+    if kind == "int4":
+        cache["value_scales"][::2] *= -1
+        cache["key_scales"][1::3, :, :, 1] *= -1
+    pages = ops.Kv4Pages(**cache)
+    q = draw(3, q_heads, dim, dtype, 1)
+    need = ops.kv_attention_workspace(pages, 3, q_heads, 7000)
+    assert need > 0
+    work = torch.full((need + 8192,), 0x7b, dtype=torch.uint8, device="cuda")
+    out = ops.kv_attention(q, pages, table, ints(lengths), 7000, workspace=work[:need])
+    near(out, *forms.attended(q, cache, kind, table, lengths, dim ** -0.5))
+    assert (work[need:] == 0x7b).all()
+    assert torch.equal(ops.kv_attention(q, pages, table, ints(lengths), 7000), out)
+
+
 @pytest.mark.parametrize("kind", ALL)
 def test_a_captured_step_is_replayed(ops, kind):
     """Write, bounds, selection, both attentions and read back, captured once and replayed with new inputs and
