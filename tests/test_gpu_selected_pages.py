@@ -92,6 +92,50 @@ def test_bounds_of_extreme_keys(ops, kind):
         assert torch.isnan(bounds.scales[3, 0]) and not torch.isnan(bounds.scales[3, 1]) and torch.isnan(bounds.scales[4, 1])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,page,places", [(128, 16, 9), (64, 8, 1100), (128, 256, 5), (256, 64, 7)])
+def test_bounds_of_the_largest_keys(ops, kind, dim, page, places):
+    """Keys up to the largest numbers of BF16 and F32, as they are written, and scales that a caller's own cache may hold beside
+    small codes: finite where reading back is. A wave, a slot, and a workgroup for a page and KV head."""
+    heads, rows = 2, 4
+    assert rows * places * heads >= 8192 or places < 10
+    table = torch.randperm(rows * places, generator=torch.Generator("cuda").manual_seed(1), device="cuda").int().view(rows, places)
+    cache = forms.make_pages(kind, rows * places, heads, page, dim)
+    most = torch.finfo(torch.float32).max
+    at = torch.arange(page, device="cuda")
+    x = draw(6 * page, heads, dim, torch.float32, 2).clamp(-1, 1).view(6, page, heads, dim)
+    x[0] *= most
+    x[1] *= torch.finfo(torch.bfloat16).max
+    x[2, 3, 1, 40] = 3.2e38
+    x[3, :, :, 32:] *= -2.99e38
+    x[4, 1] *= 2.95e38
+    for r in range(3):
+        for p in range(min(places, 12)):
+            forms.hold(cache, kind, "keys", table[r, p].long().expand(page), at, x[(r + p) % 6])
+    last = table[3].long()
+    if kind in forms.FOUR:  # codes of -1, 0 and 1, or of 0 to 1
+        cache["keys"][last] = torch.randint(0, 3, cache["keys"][last].shape, device="cuda", dtype=torch.uint8) * 0x11 + (0x77 if kind == "int4" else 0)
+        cache["key_scales"][last] = 254 if kind == "e2m1" else 3.3e38
+    else:
+        cache["keys"][last] = torch.randint(0, 2, cache["keys"][last].shape, device="cuda").to(cache["keys"].dtype)
+        cache["key_scales"][last] = 3.3e38
+    pages = described(ops, kind, cache)
+    bounds = ops.KvBounds.empty(pages)
+    lengths = [page * places, page * places - 3, page * places, page * places]
+    ops.kv_bounds(pages, bounds, table, ints([0] * rows), ints(lengths), page * places)
+    for r in range(rows):
+        for p in (*range(min(places, 6)), places - 1):
+            id, count = int(table[r, p]), min(page, lengths[r] - p * page)
+            k, _ = ops.kv_read(pages, ints(list(range(id * page, id * page + count))), torch.float32)
+            for h in range(heads):
+                codes, scale = forms.bounds_of(cache, kind, id, h, count)
+                finite = bool(torch.isfinite(k[:, h]).all())
+                # INT8: 127 times a 127th of the largest number, rounded, may be past it, in reading back too.
+                assert math.isfinite(scale) == finite and (finite or kind == "int8")
+                assert torch.equal(bounds.codes[id, h], codes), (r, p, h)
+                assert bounds.scales[id, h].item() == scale or not finite and torch.isnan(bounds.scales[id, h])
+
+
 # ------------------------------------------------------------------ selection
 
 
