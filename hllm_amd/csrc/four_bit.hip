@@ -615,8 +615,15 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   }
 
   // The four waves' states meet in LDS, each wave's in its own tile.
-  if constexpr (kRatios) r = unit < 0 ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127);
   l = column_sum(l);
+  if constexpr (kRatios) {
+    // References may lie far from their scores, by wave: the sum's exponent goes over to it, or 2^(m - another wave's) could be nothing
+    // where the sum beside it is not.
+    const int power = l > 0.0f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
+    l = __builtin_amdgcn_ldexpf(l, -power);
+    m += (float)power;
+    r = unit < 0 ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127 - power);
+  }
   // Only scores of -inf (an infinite query's): a sum that is not 0 beside that maximum tells them from no positions.
   if (any && l == 0.0f) l = 1.0f;
   if (quad == 0) {

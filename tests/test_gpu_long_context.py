@@ -95,6 +95,37 @@ def test_waves_and_parts_of_very_different_values(ops, kind, dtype, dim, apart):
     assert (off < 2.0 ** -3 * expect.abs().amax(-1, keepdim=True)).all()
 
 
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("apart", [32, 64, 1024])
+def test_waves_and_parts_whose_values_move_their_references(ops, kind, dtype, dim, apart):
+    """Of every four stretches of `apart` positions (a wave's tiles, or a share's steps) one has scores of 0 beside -92 (base 2) with
+    values of 2^88, so that what its weights are divided by lies far below its scores; the others have scores of -12 and values
+    that grow 2^57-fold, so that theirs lies far above. The first has the output."""
+    page, lengths = 64, [8000, 1500, 300]
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 1, page, dim, stale=True)
+    for r, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        here, late = at // apart % 4 == 1, at >= n // 2
+        large = here & (at % 8 == 0)
+        x = torch.zeros(n, 1, dim, device="cuda")
+        x[:, :, 0] = torch.where(large, -4.0, 0.0)[:, None]             # 92 / 4 each
+        x[:, :, 32] = torch.where(here, 0.0, -4.0)[:, None]             # 12 / 4 each
+        size = torch.where(large, 2.0 ** 88, torch.where(here | late, 1.0, 2.0 ** -57))
+        v = draw(n, 1, dim, torch.float32, r + 1) * size[:, None, None]
+        for name, y in (("keys", x), ("values", v)):
+            forms.hold(cache, kind, name, table[r].long()[at // page], at % page, y)
+    q = torch.zeros(3, 4, dim, dtype=dtype, device="cuda")
+    q[:, :, 0], q[:, :, 32] = 1.0, 12 / 92
+    scale = 92 * math.log(2) / 4
+    pages = described(ops, kind, cache)
+    for most in (8000, 300):
+        out = ops.kv_attention(q, pages, table, ints(lengths), most, scale=scale)
+        near(out, *forms.attended(q, cache, kind, table, lengths, scale, most))
+
+
 # ------------------------------------------------------------------ heads that share cache lines
 
 
