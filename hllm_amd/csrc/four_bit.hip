@@ -308,7 +308,15 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 #pragma unroll
   for (int f = 0; f < 2 * G; ++f) o[f] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f, r = 0.0f;
-  int unit = -1000;  // 16-bit tensors: the exponent of the value scales' unit
+  // A position whose values are all 0 has a scale that no other has; kLeast: what counts as its power of two.
+  constexpr int kNoUnit = -1000, kNoScale = 1, kLeast = -190;
+  int unit = kNoUnit;  // 16-bit tensors: the exponent of the value scales' unit
+  // Another unit for the value scales, 2^by as large: the columns' references come down by as much, so that their sums of values stay as they are.
+  const auto move_unit = [&](int by) {
+    unit += by;
+    m -= (float)by;
+    l = __builtin_amdgcn_ldexpf(l, by);
+  };
   bool any = false;  // whether the wave has had a position
   float* key_scale = reinterpret_cast<float*>(tile + Layout::kScales);
   char* value_scale = tile + Layout::kValueScales;
@@ -344,23 +352,28 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           most = fmaxf(most, fabsf(v[g]));  // NaN is not taken
         }
         if constexpr (kRatios) {
-          const int power = mine ? max((int)(__float_as_uint(most) >> 23), 1) : 0;
-          if (__any(power > unit + 60)) {
-            int top = power;
-            for (int step = 1; step < 64; step <<= 1) top = max(top, __shfl_xor(top, step, 64));
+          const bool some = mine && most > 0.0f;
+          const int power = max((int)(__float_as_uint(most) >> 23), 1);
+          if (__any(some && (uint32_t)(power - unit + 125) > 155u)) {
+            int top = some ? power : 0, least = some ? power : 255;
+            for (int step = 1; step < 64; step <<= 1) {
+              top = max(top, __shfl_xor(top, step, 64));
+              least = min(least, __shfl_xor(least, step, 64));
+            }
             top = __builtin_amdgcn_readfirstlane(top);
-            // A column's reference comes down by as much as its sum of weights allows: to the new unit, what the wave has
-            // is small, and weights that were nothing beside it are not.
-            const int room = min(top - unit, max(226 - (int)(__float_as_uint(column_max(l)) >> 23), 0));
-            const float rescale = __builtin_amdgcn_ldexpf(1.0f, max(unit + room - top, -300));
-#pragma unroll
-            for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
-            l = __builtin_amdgcn_ldexpf(l, room);
-            m -= (float)room;
-            unit = top;
+            least = __builtin_amdgcn_readfirstlane(least);
+            // Up as far as the sums of weights leave room for it, to the largest; down to what F32 holds beside the smallest.
+            if (unit == kNoUnit) unit = top;
+            if (top > unit + 30) {
+              int sums = l < INFINITY ? (int)(__float_as_uint(l) >> 23) : 0;
+              for (int step = 1; step < 64; step <<= 1) sums = max(sums, __shfl_xor(sums, step, 64));
+              move_unit(min(top - unit, max(226 - __builtin_amdgcn_readfirstlane(sums), 0)));
+            }
+            if (least < unit - 125) move_unit(min(max(least + 125, top - 120) - unit, 0));
           }
           if (mine) {
-            largest_scale[own] = __uint_as_float((uint32_t)max(power - unit + 127, 1) << 23);
+            const int held = some ? min(max(power - unit + 127, kNoScale), 254) : unit == kNoUnit ? 127 : kNoScale;
+            largest_scale[own] = __uint_as_float((uint32_t)held << 23);
 #pragma unroll
             for (int g = 0; g < G; ++g)
               reinterpret_cast<_Float16*>(value_scale)[g * N + own] = (_Float16)__builtin_amdgcn_ldexpf(v[g], 127 - power);
@@ -479,7 +492,9 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
       if constexpr (kRatios) {
         // Weights are 2^(score - m) for an m that is seldom changed: where a wave's first scores are found, and where a weight times its
         // value scales (in `unit`s) is above 2^14, or a weight above 2^100; the largest is then made 2^6. So most
-        // tiles need no maximum, and F16 holds every weight to 2^-11 or to 2^-31 of the largest.
+        // tiles need no maximum, and F16 holds every weight to 2^-11 or to 2^-31 of the largest. Where a weight would have to be above 2^100
+        // for that, for its value is 2^94 and more times smaller than the unit, the unit comes down. A wave has one unit: F32 holds the sums of
+        // weights of a head whose largest values count and of one whose smallest do if those are at most some 2^180 apart.
         float sum, largest;
         const auto weigh = [&] {
           const float base = m == -INFINITY ? 0.0f : m;
@@ -506,15 +521,34 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           for (int j = 0; j < 8; ++j) {
             const float sc = j < valid ? d[j] * factor : -INFINITY;
             top = fmaxf(top, sc);
-            high = fmaxf(high, sc + (float)((int)(__float_as_uint(ls[j]) >> 23) - 127));
+            const int power = (int)(__float_as_uint(ls[j]) >> 23);
+            high = fmaxf(high, sc + (float)(power == kNoScale ? kLeast : power - 127));
           }
-          // Of the columns that need it: a head's sums do not depend on the heads beside it.
+          // Of the columns that need it: while the unit stays, a head's sums do not depend on the heads beside it.
           const bool own_raise = column_max(raise ? 1.0f : 0.0f) > 0.0f;
-          const float raised = own_raise ? fmaxf(m, fmaxf(column_max(high) - 6.0f, column_max(top) - 100.0f)) : m;
-          const float rescale = raised == m ? 1.0f : exp2_fast(m - raised);
+          float from = column_max(high) - 6.0f;
+          const float least = own_raise ? column_max(top) - 100.0f : -INFINITY;
+          if (__any(least > from && least > m)) {
+            // The scales' unit comes down by what is missing, as far as the tile's largest allows.
+            int by = least > from && least > m ? (int)(least - from) + 1 : 0, held = (int)(__float_as_uint(largest_scale[own]) >> 23), top_held = held;
+            for (int step = 1; step < 64; step <<= 1) {
+              by = max(by, __shfl_xor(by, step, 64));
+              top_held = max(top_held, __shfl_xor(top_held, step, 64));
+            }
+            by = __builtin_amdgcn_readfirstlane(min(by, 254 - top_held));
+            move_unit(-by);
+            from += (float)by;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (held != kNoScale) largest_scale[own] = __uint_as_float((uint32_t)(held + by) << 23);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load8(largest_scale + 32 * s + 8 * quad, ls);
+          }
+          const float raised = own_raise ? fmaxf(m, fmaxf(from, least)) : m;
+          // Twice the root: a sum of up to 2^127 may count beside 2^(m - raised) below F32's range.
+          const float root = raised == m ? 1.0f : exp2_fast(0.5f * (m - raised)), rescale = root * root;
 #pragma unroll
           for (int f = 0; f < 2 * G; ++f) o[f] *= rescale;
-          l *= rescale;
+          l = l * root * root;
           m = raised;
           weigh();
         }
@@ -622,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
     const int power = l > 0.0f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
     l = __builtin_amdgcn_ldexpf(l, -power);
     m += (float)power;
-    r = unit < 0 ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127 - power);
+    r = unit == kNoUnit ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127 - power);
   }
   // Only scores of -inf (an infinite query's): a sum that is not 0 beside that maximum tells them from no positions.
   if (any && l == 0.0f) l = 1.0f;

@@ -542,8 +542,9 @@ typedef struct {
 /* The 8-bit cache's operators over a 4-bit one, to the same rules. In attention E2M1 keys enter their products exactly, and an INT4
  * key's scale multiplies its group's part of the score in F32; a finite key's and query's products stay finite for
  * keys below 2^115. A value's scale enters its weight, which is F16 for 16-bit tensors (rounded once, beside INT4 values
- * twice; weights below 2^-25 of a wave's largest may be lost) and two F16 parts for F32 ones. `table_head_stride` as for
- * hllm_rocm_kv_attention_by_head. */
+ * twice; weights below 2^-25 of a wave's largest may be lost, and so may a group's scale below 2^-25 of the largest of its vector, an
+ * INT4 one's last bits from 2^-17 down) and two F16 parts for F32 ones. Beside 16-bit tensors the values' scales, each
+ * vector's largest one, lie within 2^180 of one another in a row (those of 0 apart): farther apart the output may be off by more. `table_head_stride` as for hllm_rocm_kv_attention_by_head. */
 hllm_status hllm_rocm_kv4_append(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
                                  const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
                                  const hllm_rocm_tensor* v, const hllm_rocm_rope* rope,

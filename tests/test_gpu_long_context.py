@@ -98,6 +98,42 @@ def test_waves_and_parts_of_very_different_values(ops, kind, dtype, dim, apart):
 @pytest.mark.parametrize("kind", ALL)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("values,weights", [(100, 90), (115, 120), (118, 118), (160, 200), (180, 230)])
+def test_values_far_apart(ops, kind, dtype, dim, values, weights):
+    """Some positions' values are 2^`values` times the others' and their weights, in half of the heads, 2^-`weights` (by head up to an
+    eighth less), in others as large or as much larger: larger values first, last, and every other one, in rows of many tiles and
+    of one. Weights below F32's range are not the output."""
+    page, lengths = 32, [2000, 150, 40, 5, 1300, 64]
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim, stale=True)
+    large = 2.0 ** min(values, 120)
+    for r, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        big = [at < n // 2, at >= n // 2, at % 2 == 1][r % 3]
+        x = torch.zeros(n, 2, dim, device="cuda")
+        x[:, :, 0] = torch.where(big, -4.0, 4.0)[:, None]
+        v = draw(n, 2, dim, torch.float32, r + 1) * torch.where(big, large, large * 2.0 ** -values)[:, None, None]
+        for name, y in (("keys", x), ("values", v)):
+            forms.hold(cache, kind, name, table[r].long()[at // page], at % page, y)
+    q = torch.zeros(len(lengths), 16, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0 if weights > 126 else 1 - torch.arange(16, device="cuda").to(dtype) % 5 / 32
+    q[:, 1::4, 0] = 0.0
+    q[:, 2::4, 0] = -1.0
+    scale = weights * math.log(2) / 8
+    pages = described(ops, kind, cache)
+    for most in (2000, 150):
+        out = ops.kv_attention(q, pages, table, ints(lengths), most, scale=scale)
+        expect, off = forms.attended(q, cache, kind, table, lengths, scale, most)
+        top = 65520.0 if dtype == torch.float16 else math.inf
+        past = expect.abs() - off >= top
+        assert torch.equal(out[past].double(), expect[past].sign() * math.inf)
+        inside = expect.abs() + off < top
+        near(out[inside], expect[inside], off[inside])
+
+
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("apart", [32, 64, 1024])
 def test_waves_and_parts_whose_values_move_their_references(ops, kind, dtype, dim, apart):
     """Of every four stretches of `apart` positions (a wave's tiles, or a share's steps) one has scores of 0 beside -92 (base 2) with
