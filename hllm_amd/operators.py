@@ -392,7 +392,8 @@ def kv_attention(q: torch.Tensor, pages: KvPages | Kv4Pages, page_table: torch.T
 
 
 def kv_attention_workspace(pages: KvPages | Kv4Pages, rows: int, q_heads: int, max_length: int) -> int:
-    """Bytes of workspace that ``kv_attention`` needs for these sizes (0: none)."""
+    """Bytes of workspace that ``kv_attention`` needs for these sizes, and for smaller lengths (0: none). Fewer rows may need
+    more: one workspace for batches of several sizes has the largest of their sizes."""
     if min(rows, q_heads, max_length) < 0:
         raise ValueError("rows, q_heads and max_length are not negative")
     return _workspace_bytes(pages, min(rows, _MOST), min(q_heads, _MOST), min(max_length, _MOST))
@@ -470,7 +471,8 @@ def kv_select(q: torch.Tensor, bounds: KvBounds, page_table: torch.Tensor, lengt
 
 
 def kv_select_workspace(bounds: KvBounds, rows: int, max_length: int, keep: int) -> int:
-    """Bytes of workspace that ``kv_select`` needs for these sizes (0: none)."""
+    """Bytes of workspace that ``kv_select`` needs for these sizes, and for smaller lengths and larger ``keep`` (0: none). Fewer rows
+    may need more, as for ``kv_attention_workspace``."""
     if min(rows, max_length, keep) < 0:
         raise ValueError("rows, max_length and keep are not negative")
     need = C.c_uint64()

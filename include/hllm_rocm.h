@@ -503,7 +503,8 @@ hllm_status hllm_rocm_kv_attention_by_head(int32_t device, void* stream, const h
                                            const hllm_rocm_kv_attention_args* args,
                                            uint64_t table_head_stride);
 /* The workspace that does for a call with `rows` rows of `query_heads` heads and this max_length or a
- * smaller one (0: none, and `workspace` may be NULL). Needs no device. */
+ * smaller one (0: none, and `workspace` may be NULL). For this number of rows: of many rows none is cut, and fewer may need more, so
+ * one workspace for batches of several sizes has the largest of their sizes. Needs no device. */
 hllm_status hllm_rocm_kv_attention_workspace(const hllm_rocm_kv_pages* pages, uint64_t rows,
                                              uint32_t query_heads, uint64_t max_length,
                                              uint64_t* bytes);
@@ -544,7 +545,8 @@ typedef struct {
  * keys below 2^115. A value's scale enters its weight, which is F16 for 16-bit tensors (rounded once, beside INT4 values
  * twice; weights below 2^-25 of a wave's largest may be lost, and so may a group's scale below 2^-25 of the largest of its vector, an
  * INT4 one's last bits from 2^-17 down) and two F16 parts for F32 ones. Beside 16-bit tensors the values' scales, each
- * vector's largest one, lie within 2^180 of one another in a row (those of 0 apart): farther apart the output may be off by more. `table_head_stride` as for hllm_rocm_kv_attention_by_head. */
+ * vector's largest one, lie within 2^180 of one another in a row (those of 0 apart): farther apart the output may be off by
+ * more. `table_head_stride` as for hllm_rocm_kv_attention_by_head. */
 hllm_status hllm_rocm_kv4_append(int32_t device, void* stream, const hllm_rocm_kv4_pages* pages,
                                  const int32_t* slots, uint64_t rows, const hllm_rocm_tensor* k,
                                  const hllm_rocm_tensor* v, const hllm_rocm_rope* rope,
@@ -627,8 +629,8 @@ typedef struct {
 
 hllm_status hllm_rocm_kv_select(int32_t device, void* stream, const hllm_rocm_kv_bounds* bounds,
                                 const hllm_rocm_kv_select_args* args);
-/* The workspace that does for `rows` rows, this max_length or a smaller one and this `keep` or a larger one (0: none). Needs
- * no device. */
+/* The workspace that does for `rows` rows, this max_length or a smaller one and this `keep` or a larger one (0: none); fewer
+ * rows may need more, as for hllm_rocm_kv_attention_workspace. Needs no device. */
 hllm_status hllm_rocm_kv_select_workspace(const hllm_rocm_kv_bounds* bounds, uint64_t rows,
                                           uint64_t max_length, uint32_t keep, uint64_t* bytes);
 

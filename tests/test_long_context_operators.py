@@ -284,6 +284,37 @@ def test_select_workspace_needs_no_device():
     refused(lib.hllm_rocm_kv_select_workspace(by(bounds()), (1 << 20) + 1, 8, 100, C.byref(need)), "rows")
 
 
+@pytest.mark.parametrize("kind", ["kv", "kv4", "select"])
+def test_a_workspace_is_for_its_number_of_rows(kind):
+    """Fewer rows may need more: a workspace for several batch sizes has the largest of their sizes, and a smaller one is
+    refused."""
+    lib, need = capi.library(), C.c_uint64(1)
+    length = 1600 if kind != "select" else 64 * 2000
+
+    def size(rows):
+        if kind == "select":
+            capi.check(lib.hllm_rocm_kv_select_workspace(by(bounds()), rows, length, 64, C.byref(need)))
+        else:
+            make, name = (four, "hllm_rocm_kv4_attention_workspace") if kind == "kv4" else (eight, "hllm_rocm_kv_attention_workspace")
+            capi.check(getattr(lib, name)(by(make()), rows, 32, length, C.byref(need)))
+        return need.value
+
+    def call(rows, held):
+        if kind == "select":
+            args = select_args(rows=rows, max_length=length, workspace_bytes=held)
+            return lib.hllm_rocm_kv_select(0, None, by(bounds()), C.byref(args))
+        args = attention_args(rows=rows, max_length=length, workspace_bytes=held)
+        if kind == "kv4":
+            return lib.hllm_rocm_kv4_attention(0, None, by(four()), C.byref(args), 0)
+        return lib.hllm_rocm_kv_attention(0, None, by(eight()), C.byref(args))
+
+    sizes = {rows: size(rows) for rows in range(1, 300)}
+    most = max(sizes, key=sizes.get)
+    assert 1 < most < 299 and sizes[299] == 0 < sizes[most]
+    refused(call(most, sizes[299]), "workspace")
+    refused(call(most, sizes[most] - 1), "workspace")
+
+
 @pytest.mark.parametrize("struct,cname", [(capi.Kv4Pages, "hllm_rocm_kv4_pages"), (capi.KvBounds, "hllm_rocm_kv_bounds"),
                                           (capi.KvBoundsArgs, "hllm_rocm_kv_bounds_args"), (capi.KvSelectArgs, "hllm_rocm_kv_select_args")])
 def test_layouts_match_the_header(struct, cname):
