@@ -94,22 +94,6 @@ __device__ inline float2 turn(int32_t position, uint64_t turns) {
   return float2{quarter == 1 || quarter == 2 ? -a : a, quarter & 2 ? -b : b};
 }
 
-// One workgroup takes up to heads_per_block heads of one row, 16 elements of a head a thread,
-// after its first threads have put the row's cosines and sines into LDS: they are computed once
-// for all heads of the block, and no table is read. In half layout with a rotary
-// dimension of whole sixteens a thread holds both elements of its pairs (eight of either half);
-// interleaved pairs lie beside each other; other half layouts exchange through LDS (kExchange). So
-// every pair is read before it is written and a tensor can be rotated in place. Bound by memory (a copy of
-// 4 GiB reaches 4.8 TB/s): 8192 rows of 40 heads of 128 take 41 us in BF16 and 63 in F32, 4.1 and 5.4
-// TB/s; interleaved pairs 44 and 64. The exchange sends every element through LDS as a word, turned or
-// not: 24 of the 128 rotated 50 and 80 us, 3.4 and 4.2 TB/s.
-//
-// F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
-// share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
-// heads of 256: 12.7 us, 4.3 TB/s; 64 rows 4.1 us, one chain of loads, sines, the largest value and the stores.
-// The last part for a 4-bit cache, of every thread of the workgroup. A group's 32 elements lie with two to four lanes, which depends
-// on the rotation's layout, so they meet in LDS: each eight's largest magnitude, then the codes, which are written from
-// there in whole words. A head's lanes (4, 8 or 16) lie in one wave, so no barrier is needed.
 // Lanes of one wave see what its lanes have written to LDS: its accesses are made in order.
 __device__ inline void wave_meets() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -117,8 +101,10 @@ __device__ inline void wave_meets() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A thread's two eights of a 4-bit cache's vector, keys turned. The largest magnitude of 32 elements is found over four threads in LDS; a
-// value's bytes go there and back, because those that lie beside each other in the cache are of different threads. Bound by memory as
+// rotate_kernel's last part for a 4-bit cache: a thread's two eights of a vector, keys turned; every thread of the workgroup is here. A
+// group's 32 elements lie with two to four threads, which depends on the rotation's layout, so each eight's largest magnitude
+// meets the others in LDS; the codes go there and back in whole words, because those that lie beside each other in the cache are of
+// different threads. A head's lanes (4, 8 or 16) lie in one wave, so no barrier is needed. Bound by memory as
 // the 8-bit cache's is: 2011 rows of 20 + 4 heads of 256, BF16 to INT4, 12.9 us, 4.0 TB/s (to INT8 12.6); 16384 rows of 32 + 8 heads of 128, F16
 // 80.7 us, 4.4 TB/s (79.1).
 template <int F>
@@ -173,6 +159,19 @@ __device__ inline void append_four(const RotateArgs& a, const float* x, int slot
   *reinterpret_cast<uint2v*>(to) = uint2v{codes[2 * u], codes[2 * u + 1]};
 }
 
+// One workgroup takes up to heads_per_block heads of one row, 16 elements of a head a thread,
+// after its first threads have put the row's cosines and sines into LDS: they are computed once
+// for all heads of the block, and no table is read. In half layout with a rotary
+// dimension of whole sixteens a thread holds both elements of its pairs (eight of either half);
+// interleaved pairs lie beside each other; other half layouts exchange through LDS (kExchange). So
+// every pair is read before it is written and a tensor can be rotated in place. Bound by memory (a copy of
+// 4 GiB reaches 4.8 TB/s): 8192 rows of 40 heads of 128 take 41 us in BF16 and 63 in F32, 4.1 and 5.4
+// TB/s; interleaved pairs 44 and 64. The exchange sends every element through LDS as a word, turned or
+// not: 24 of the 128 rotated 50 and 80 us, 3.4 and 4.2 TB/s.
+//
+// F >= 0: q_out is written as above, k is rotated and k and v are quantised: a head's lanes
+// share its largest value by shuffles, and no rotated key is rounded or written in between. 2011 rows of 20 and 4
+// heads of 256: 12.7 us, 4.3 TB/s; 64 rows 4.1 us, one chain of loads, sines, the largest value and the stores.
 template <typename T, int F, bool kExchange>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(RotateArgs a) {
   __shared__ float2 cs[128];
