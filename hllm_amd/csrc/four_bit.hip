@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           sc[j] = d[j] * factor;
-          by_lo[j] = j >= valid || sc[j] == -INFINITY ? 0.0f : fmaf(d[j], factor, -sc[j]) + d[j] * factor_lo;
+          // Past 2^24 it is more than 1, and past 2^31 more than a weight can hold: scores are as good as F32's there.
+          by_lo[j] = j >= valid || sc[j] == -INFINITY ? 0.0f : __builtin_amdgcn_fmed3f(fmaf(d[j], factor, -sc[j]) + d[j] * factor_lo, -1.0f, 1.0f);
           sc[j] = j < valid ? sc[j] : -INFINITY;
           most = fmaxf(most, sc[j]);
         }
@@ -569,6 +570,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
         float sum = 0.0f, largest = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+#pragma clang fp contract(off)
           weight[j] = exp2_fast((sc[j] - base) + by_lo[j]);
           sum += weight[j];
           largest = fmaxf(largest, weight[j] * ls[j]);

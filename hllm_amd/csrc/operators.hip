@@ -593,7 +593,10 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
       const float by = ks[i] * factor;
       sc[i] = d * by;
       if constexpr (P == 2)
-        by_lo[i] = sc[i] == -INFINITY ? 0.0f : fmaf(d, by, -sc[i]) + d * (fmaf(ks[i], factor, -by) + ks[i] * factor_lo);
+        // Past 2^24 it is more than 1, and past 2^31 more than a weight can hold: scores are as good as F32's there.
+        by_lo[i] = sc[i] == -INFINITY
+                       ? 0.0f
+                       : __builtin_amdgcn_fmed3f(fmaf(d, by, -sc[i]) + d * (fmaf(ks[i], factor, -by) + ks[i] * factor_lo), -1.0f, 1.0f);
     }
     if (!whole) {
       const int valid = (gone >> quad) & 1 ? 0 : end - (t + 8 * quad);
@@ -618,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, kAttendBlocks<D>) kv_attention_kerne
     float weight[8], sum = 0.0f, largest = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+#pragma clang fp contract(off)
       const float p = exp2_fast(P == 2 ? (sc[i] - base) + by_lo[i] : sc[i] - base);
       sum += p;
       weight[i] = p * vs[i];

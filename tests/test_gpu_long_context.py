@@ -162,6 +162,35 @@ def test_waves_and_parts_whose_values_move_their_references(ops, kind, dtype, di
         near(out, *forms.attended(q, cache, kind, table, lengths, scale, most))
 
 
+@pytest.mark.parametrize("kind", ALL)
+@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("apart", [0, 60, 120])
+def test_equal_scores_of_any_size(ops, kind, dtype, dim, apart):
+    """Keys that are all the same weigh the same, however large their scores are: past 2^24 (base 2) F32 has no fractions and then no odd
+    numbers left beside them. Values 2^`apart` times as large first, last and every other one."""
+    page, lengths = 32, [2000, 150, 40, 5, 1300, 64]
+    table, count = paged(lengths, page)
+    cache = forms.make_pages(kind, count, 2, page, dim, stale=True)
+    for r, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        big = [at < n // 2, at >= n // 2, at % 2 == 1][r % 3]
+        v = draw(n, 2, dim, torch.float32, r + 1) * torch.where(big, 2.0 ** apart, 1.0)[:, None, None]
+        for name, y in (("keys", torch.ones(n, 2, dim, device="cuda")), ("values", v)):
+            forms.hold(cache, kind, name, table[r].long()[at // page], at % page, y)
+    q = torch.ones(len(lengths), 8, dim, dtype=dtype, device="cuda")
+    pages = described(ops, kind, cache)
+    for most in (2000, 150):
+        expect, off = forms.attended(q, cache, kind, table, lengths, 0.0, most)
+        top = 65520.0 if dtype == torch.float16 else math.inf
+        for scale in (0.0, -3.0, 1e4, 1.7e5, 1e7, -1e9, 1e20):
+            out = ops.kv_attention(q, pages, table, ints(lengths), most, scale=scale)
+            past = expect.abs() - off >= top
+            assert torch.equal(out[past].double(), expect[past].sign() * math.inf)
+            inside = expect.abs() + off < top
+            near(out[inside], expect[inside], off[inside])
+
+
 # ------------------------------------------------------------------ heads that share cache lines
 
 
