@@ -311,11 +311,18 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   // A position whose values are all 0 has a scale that no other has; kLeast: what counts as its power of two.
   constexpr int kNoUnit = -1000, kNoScale = 1, kLeast = -190;
   int unit = kNoUnit;  // 16-bit tensors: the exponent of the value scales' unit
-  // Another unit for the value scales, 2^by as large: the columns' references come down by as much, so that their sums of values stay as they are.
+  const auto largest_of = [](int v) { return __builtin_amdgcn_readfirstlane((int)wave_max((uint32_t)v)); };
+  // References are whole numbers, which F32 adds exactly unless scores are past its fractions; then they stay where they are.
+  const auto moves = [&] { return fabsf(m) < 0x1p23f || m == -INFINITY; };
+  // Another unit for the value scales, 2^by as large: the columns' references come down by as much, or their sums of values do.
   const auto move_unit = [&](int by) {
+    const int step = moves() ? by : 0;
+    const float rest = __builtin_amdgcn_ldexpf(1.0f, step - by);
+#pragma unroll
+    for (int f = 0; f < 2 * G; ++f) o[f] *= rest;
+    l = __builtin_amdgcn_ldexpf(l, step);
+    m -= (float)step;
     unit += by;
-    m -= (float)by;
-    l = __builtin_amdgcn_ldexpf(l, by);
   };
   bool any = false;  // whether the wave has had a position
   float* key_scale = reinterpret_cast<float*>(tile + Layout::kScales);
@@ -354,22 +361,20 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
         if constexpr (kRatios) {
           const bool some = mine && most > 0.0f;
           const int power = max((int)(__float_as_uint(most) >> 23), 1);
-          if (__any(some && (uint32_t)(power - unit + 125) > 155u)) {
-            int top = some ? power : 0, least = some ? power : 255;
-            for (int step = 1; step < 64; step <<= 1) {
-              top = max(top, __shfl_xor(top, step, 64));
-              least = min(least, __shfl_xor(least, step, 64));
-            }
-            top = __builtin_amdgcn_readfirstlane(top);
-            least = __builtin_amdgcn_readfirstlane(least);
+          if (__any(some && (uint32_t)(power - unit + 125) > 133u)) {
+            const int top = largest_of(some ? power : 0);
             // Up as far as the sums of weights leave room for it, to the largest; down to what F32 holds beside the smallest.
             if (unit == kNoUnit) unit = top;
-            if (top > unit + 30) {
-              int sums = l < INFINITY ? (int)(__float_as_uint(l) >> 23) : 0;
-              for (int step = 1; step < 64; step <<= 1) sums = max(sums, __shfl_xor(sums, step, 64));
-              move_unit(min(top - unit, max(226 - __builtin_amdgcn_readfirstlane(sums), 0)));
+            int by = 0;
+            if (top > unit + 8) {
+              const int sums = largest_of(l < INFINITY && moves() ? (int)(__float_as_uint(l) >> 23) : 0);
+              by = min(top - unit, max(226 - sums, 0));
             }
-            if (least < unit - 125) move_unit(min(max(least + 125, top - 120) - unit, 0));
+            if (__any(some && power < unit + by - 125)) {
+              const int least = 255 - largest_of(some ? 255 - power : 0);
+              by = min(by, max(least + 125, top - 120) - unit);
+            }
+            if (by != 0) move_unit(by);
           }
           if (mine) {
             const int held = some ? min(max(power - unit + 127, kNoScale), 254) : unit == kNoUnit ? 127 : kNoScale;
@@ -500,7 +505,12 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           const float base = m == -INFINITY ? 0.0f : m;
           sum = largest = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) weight[j] = exp2_fast(fmaf(d[j], factor, -base));
+          for (int j = 0; j < 8; ++j) {
+            // Rounded as in the reference: where a score is past 2^30, what is left of it would be more than a weight can hold.
+#pragma clang fp contract(off)
+            const float sc = d[j] * factor;
+            weight[j] = exp2_fast(sc - base);
+          }
           if (!whole) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) weight[j] = j < valid ? weight[j] : 0.0f;
@@ -519,6 +529,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           float top = -INFINITY, high = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
+#pragma clang fp contract(off)
             const float sc = j < valid ? d[j] * factor : -INFINITY;
             top = fmaxf(top, sc);
             const int power = (int)(__float_as_uint(ls[j]) >> 23);
@@ -526,16 +537,13 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           }
           // Of the columns that need it: while the unit stays, a head's sums do not depend on the heads beside it.
           const bool own_raise = column_max(raise ? 1.0f : 0.0f) > 0.0f;
-          float from = column_max(high) - 6.0f;
-          const float least = own_raise ? column_max(top) - 100.0f : -INFINITY;
+          // Whole numbers, so that a reference moves exactly.
+          float from = ceilf(column_max(high)) - 6.0f;
+          const float least = own_raise ? ceilf(column_max(top)) - 100.0f : -INFINITY;
           if (__any(least > from && least > m)) {
             // The scales' unit comes down by what is missing, as far as the tile's largest allows.
-            int by = least > from && least > m ? (int)(least - from) + 1 : 0, held = (int)(__float_as_uint(largest_scale[own]) >> 23), top_held = held;
-            for (int step = 1; step < 64; step <<= 1) {
-              by = max(by, __shfl_xor(by, step, 64));
-              top_held = max(top_held, __shfl_xor(top_held, step, 64));
-            }
-            by = __builtin_amdgcn_readfirstlane(min(by, 254 - top_held));
+            const int held = (int)(__float_as_uint(largest_scale[own]) >> 23);
+            const int by = min(largest_of(least > from && least > m ? (int)(least - from) : 0), 254 - largest_of(held));
             move_unit(-by);
             from += (float)by;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   if constexpr (kRatios) {
     // References may lie far from their scores, by wave: the sum's exponent goes over to it, or 2^(m - another wave's) could be nothing
     // where the sum beside it is not.
-    const int power = l > 0.0f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
+    const int power = l > 0.0f && l < INFINITY && moves() ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
     l = __builtin_amdgcn_ldexpf(l, -power);
     m += (float)power;
     r = unit == kNoUnit ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, unit - 127 - power);

@@ -139,6 +139,19 @@ __device__ inline float column_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// The largest over a wave, all of whose lanes are here.
+template <int O>
+__device__ inline uint32_t row_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + O, 0xf, 0xf, false));
+}
+__device__ inline uint32_t wave_max(uint32_t v) {
+  const auto half = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max(half[0], half[1]);
+  const auto row = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(row[0], row[1]);
+  return row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
+}
+
 // Copies into LDS as lds_copy16, of cache lines that are not kept: a step reads a layer's cache once. With nt /
 // without, us, BF16, 8 KV heads of 128, caches not read just before: 3 x 200000 positions 204 / 229 (the first 6.2 TB/s, the
 // read probe 6.3), 64 rows to 8192 43.4 / 49.5, 64 rows of 200 to 1000 18.5 / 20.4; one cache of 67 MB read again and again

@@ -101,18 +101,6 @@ __device__ inline void reduce_slots(float* x, Op&& op) {
   }
 }
 
-template <int O>
-__device__ inline uint32_t row_max(uint32_t v) {
-  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + O, 0xf, 0xf, false));
-}
-__device__ inline uint32_t wave_max(uint32_t v) {
-  const auto half = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  v = max(half[0], half[1]);
-  const auto row = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max(row[0], row[1]);
-  return row_max<1>(row_max<2>(row_max<4>(row_max<8>(v))));
-}
-
 // The largest over the L lanes of a slot.
 template <int L>
 __device__ inline uint32_t slot_max(uint32_t v) {

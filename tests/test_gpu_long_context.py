@@ -163,7 +163,7 @@ def test_waves_and_parts_whose_values_move_their_references(ops, kind, dtype, di
 
 
 @pytest.mark.parametrize("kind", ALL)
-@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("apart", [0, 60, 120])
 def test_equal_scores_of_any_size(ops, kind, dtype, dim, apart):
