@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
   constexpr int kNoUnit = -1000, kNoScale = 1, kLeast = -190;
   int unit = kNoUnit;  // 16-bit tensors: the exponent of the value scales' unit
   const auto largest_of = [](int v) { return __builtin_amdgcn_readfirstlane((int)wave_max((uint32_t)v)); };
-  // References are whole numbers, which F32 adds exactly unless scores are past its fractions; then they stay where they are.
+  // A reference that takes an exponent is rounded by 2^-24 of itself, like a score; past 2^12 they are whole numbers, which F32 adds exactly,
+  // and past 2^23, where it does not, they stay where they are.
   const auto moves = [&] { return fabsf(m) < 0x1p23f || m == -INFINITY; };
   // Another unit for the value scales, 2^by as large: the columns' references come down by as much, or their sums of values do.
   const auto move_unit = [&](int by) {
@@ -537,13 +538,15 @@ __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_ker
           }
           // Of the columns that need it: while the unit stays, a head's sums do not depend on the heads beside it.
           const bool own_raise = column_max(raise ? 1.0f : 0.0f) > 0.0f;
-          // Whole numbers, so that a reference moves exactly.
-          float from = ceilf(column_max(high)) - 6.0f;
-          const float least = own_raise ? ceilf(column_max(top)) - 100.0f : -INFINITY;
+          // 2^6 for the largest weight exactly: where it is most of a softmax, as it often is, its rounding to F16 would be most of the error
+          // (attention over 100 positions: off by 2.4e-4, with whole numbers 3.3e-4).
+          const float largest_of_column = column_max(high), top_of_column = column_max(top);
+          float from = (fabsf(largest_of_column) < 4096.0f ? largest_of_column : ceilf(largest_of_column)) - 6.0f;
+          const float least = own_raise ? ceilf(top_of_column) - 100.0f : -INFINITY;
           if (__any(least > from && least > m)) {
             // The scales' unit comes down by what is missing, as far as the tile's largest allows.
             const int held = (int)(__float_as_uint(largest_scale[own]) >> 23);
-            const int by = min(largest_of(least > from && least > m ? (int)(least - from) : 0), 254 - largest_of(held));
+            const int by = min(largest_of(least > from && least > m ? (int)(least - from) + 1 : 0), 254 - largest_of(held));
             move_unit(-by);
             from += (float)by;
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
