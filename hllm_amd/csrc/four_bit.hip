@@ -132,10 +132,10 @@ __device__ inline int place_of(const AttendArgs& a, int block) {
 // codes lie so that a lane's bytes of a position are two elements of each group: the sixteen rows of an output fragment have one group.
 //
 // Bound by the cache's bytes where it is long and heads lie apart: 24 rows of 12000 to 30000 positions, 32 / 8 heads of 128, E2M1, BF16
-// 98 us, 5.2 TB/s (a streaming read 6.3); INT4, whose scales take a product of their own each, 121 us, 4.5 TB/s; F32, with two
-// or three times the products, 145. Two tiles a wave in LDS, so that one is under way while the other is worked on: 12 waves a CU have 52 KB
-// in flight. With one tile of 64 positions 101 and 131 us. Heads within a cache line, read as clusters, 119 us. Short rows are a
-// chain of start, page, tile and join: 64 rows to 2048 positions 22 us. The native product of E2M1 codes with scales
+// 101 us, 5.1 TB/s (a streaming read 6.3); INT4, whose scales take a product of their own each, 125 us, 4.3 TB/s; F32, with two
+// or three times the products, 149. Two tiles a wave in LDS, so that one is under way while the other is worked on: 12 waves a CU have 52 KB
+// in flight. Heads within a cache line, read as clusters, 121 us. Short rows are a chain of start, page, tile and join: 64 rows to
+// 2048 positions 22 us. The native product of E2M1 codes with scales
 // was measured to err by up to 2^-13 of its sum of magnitudes and is not used.
 template <typename T, int F, int D>
 __global__ void __launch_bounds__(kThreads, kAttend4Blocks<D>) kv4_attention_kernel(AttendArgs a) {

@@ -741,6 +741,11 @@ SelectPlan plan_select(const hllm_rocm_kv_bounds& b, uint64_t rows, uint64_t max
   // their own pages / with others that do, 8 KV heads of 128 and all rows of as many pages of 16:
   //   1 row: 600 pages 15.6 / 16.2, 1000 19.9 / 16.9; 4 rows: 600 15.7 / 16.3, 1000 21.1 / 18.0; 16 rows: 700 17.1 / 20.4, 2304 29.3 / 29.6,
   //   3000 47.6 / 40.8; 32 rows: 700 19.2 / 25.0, 1875 37.0 / 45.9; 64 rows: 1200 51.5 / 64.2, 2304 85.6 / 102; 128 rows: 1000 87.4 / 108
+  // Later, with bounds from the last level; rows of a tenth to all of the pages have the same lines (64 rows to 2304: 53.9 / 63.8):
+  //   128, 8 heads: 1 row: 1000 17.6 / 16.8; 16 rows: 2304 29.6 / 29.1; 64 rows: 1200 42.4 / 51.8, 2304 62.7 / 73.8
+  //   64, 8 heads: 1 row: 600 12.8 / 16.5, 1000 14.7 / 16.6; 16 rows: 2304 23.8 / 25.1; 64 rows: 1200 34.1 / 41.2, 2304 46.3 / 55.5
+  //   256, 4 heads: 2 rows: 600 19.7 / 17.8, 1000 25.5 / 18.0; 32 rows: 700 22.5 / 29.0, 2304 46.6 / 41.3; 128 rows: 1200 63.6 / 73.9
+  // Heads of 64 would have the lines higher and heads of 256 lower, for a page's bytes: at the lines they lose up to 13% and 18%.
   if (pairs * kSelectThreads<kLarge> > kMostBlocks * kThreads) refuse("too many rows for these heads");
   if (pages <= 640 || (pairs >= 128 && pages <= 2304)) {
     p.how = kLarge;
