@@ -472,7 +472,8 @@ hllm_status hllm_rocm_kv_read(int32_t device, void* stream, const hllm_rocm_kv_p
  * K^T) V with the keys and values of positions 0 .. lengths[row] - 1 of the row's pages; query
  * heads share KV heads in groups of q.heads / kv_heads. Scores, softmax and sums are F32; products
  * take codes exactly, and q and the weights as F16 (F16 and BF16 tensors, each vector's largest
- * weight scaled to 1) or as sums of two F16 values (F32 tensors).
+ * weight scaled to 1) or as sums of two F16 values (F32 tensors). Weights below 2^-126 of a row's largest may be lost, scores past
+ * 2^23 (times log2 e) are as F32 rounds them, and outputs may be off by 2^-115 besides.
  *
  * A row's length counts at most max_length and table_width * page_tokens positions; a length
  * of 0 gives zeros and a negative one marks a padding row, which is left as it was. Positions in
